@@ -21,6 +21,7 @@ GDN_ERR_DEVICE = -5
 
 GDN_F32, GDN_BF16, GDN_F16, GDN_I32, GDN_I64 = 0, 1, 2, 3, 4
 GDN_ACT_NONE, GDN_ACT_SILU = 0, 1
+GDN_GATE_SILU, GDN_GATE_SIGMOID = 0, 1
 
 EXPORTED = (
     "gdn_chunk_workspace_size",
@@ -42,6 +43,14 @@ EXPORTED = (
     "gdn_causal_conv1d_update",
     "gdn_conv_chunk_workspace_size",
     "gdn_conv_chunk_fwd",
+    "gdn_causal_conv1d_bwd_workspace_size",
+    "gdn_causal_conv1d_bwd",
+    "gdn_norm_fwd",
+    "gdn_norm_bwd_workspace_size",
+    "gdn_norm_bwd",
+    "gdn_scan_workspace_size",
+    "gdn_scan_fwd",
+    "gdn_scan_update",
     "gdn_last_error",
     "gdn_abi_version",
     "gdn_kernel_launch_count",
@@ -154,6 +163,58 @@ class Conv1dUpdateArgs(ctypes.Structure):
     ]
 
 
+class Conv1dBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("weight", _vp), ("bias", _vp), ("initial_state", _vp), ("dy", _vp),
+        ("dx", _vp), ("dweight", _vp), ("dbias", _vp), ("dinitial_state", _vp), ("cu_seqlens", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("B", _i64), ("T", _i64), ("N", _i64), ("D", _i64),
+        ("stride_x_token", _i64), ("stride_dy_token", _i64),
+        ("W", _i32), ("x_dtype", _i32), ("w_dtype", _i32), ("state_dtype", _i32), ("cu_dtype", _i32),
+        ("activation", _i32),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("z", _vp), ("residual", _vp), ("weight", _vp), ("y", _vp), ("sum", _vp),
+        ("dy", _vp), ("dsum", _vp), ("dx", _vp), ("dz", _vp), ("dresidual", _vp), ("dweight", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("rows", _i64), ("heads", _i64), ("D", _i64),
+        ("stride_x_token", _i64), ("stride_x_head", _i64), ("stride_z_token", _i64), ("stride_z_head", _i64),
+        ("group", _i32), ("dtype", _i32), ("x_dtype", _i32), ("res_dtype", _i32), ("w_dtype", _i32),
+        ("gate_before", _i32), ("zero_centered", _i32), ("activation", _i32),
+        ("eps", ctypes.c_float), ("residual_scale", ctypes.c_float),
+    ]
+
+
+class ScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("dt", _vp), ("A", _vp), ("b", _vp), ("c", _vp), ("D", _vp), ("z", _vp), ("dt_bias", _vp),
+        ("initial_state", _vp), ("y", _vp), ("final_state", _vp), ("cu_seqlens", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("B", _i64), ("T", _i64), ("N", _i64),
+        ("stride_x", _i64), ("stride_dt", _i64), ("stride_b", _i64), ("stride_c", _i64), ("stride_z", _i64),
+        ("H", _i32), ("P", _i32), ("G", _i32), ("S", _i32),
+        ("dtype", _i32), ("dt_dtype", _i32), ("init_dtype", _i32), ("final_dtype", _i32), ("cu_dtype", _i32),
+        ("dt_softplus", _i32), ("force_generic", _i32),
+        ("dt_min", ctypes.c_float), ("dt_max", ctypes.c_float),
+    ]
+
+
+class ScanUpdateArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("dt", _vp), ("A", _vp), ("b", _vp), ("c", _vp), ("D", _vp), ("z", _vp), ("dt_bias", _vp),
+        ("state", _vp), ("y", _vp), ("ssm_state_indices", _vp), ("err", _vp),
+        ("N", _i64), ("num_slots", _i64), ("stride_slot", _i64),
+        ("stride_x", _i64), ("stride_dt", _i64), ("stride_b", _i64), ("stride_c", _i64), ("stride_z", _i64),
+        ("H", _i32), ("P", _i32), ("G", _i32), ("S", _i32),
+        ("dtype", _i32), ("dt_dtype", _i32), ("state_dtype", _i32), ("idx_dtype", _i32),
+        ("dt_softplus", _i32),
+        ("dt_min", ctypes.c_float), ("dt_max", ctypes.c_float),
+    ]
+
+
 _lib = None
 
 
@@ -205,6 +266,17 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.gdn_conv_chunk_workspace_size.restype = ctypes.c_size_t
     lib.gdn_conv_chunk_fwd.argtypes = [ctypes.POINTER(ChunkArgs), ctypes.POINTER(Conv1dFnArgs), _vp]
     lib.gdn_conv_chunk_fwd.restype = ctypes.c_int
+    for name, args in (("gdn_causal_conv1d_bwd", Conv1dBwdArgs), ("gdn_norm_fwd", NormArgs),
+                       ("gdn_norm_bwd", NormArgs), ("gdn_scan_fwd", ScanArgs),
+                       ("gdn_scan_update", ScanUpdateArgs)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(args), _vp]
+        fn.restype = ctypes.c_int
+    for name, args in (("gdn_causal_conv1d_bwd_workspace_size", Conv1dBwdArgs),
+                       ("gdn_norm_bwd_workspace_size", NormArgs), ("gdn_scan_workspace_size", ScanArgs)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(args)]
+        fn.restype = ctypes.c_size_t
     lib.gdn_last_error.argtypes = []
     lib.gdn_last_error.restype = ctypes.c_char_p
     lib.gdn_abi_version.argtypes = []

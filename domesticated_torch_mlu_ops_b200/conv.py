@@ -27,10 +27,13 @@ Differences from the reference, all supersets or stricter checks:
 
 from __future__ import annotations
 
+import ctypes
+from typing import Optional
+
 import torch
 
 from . import _lib
-from .gdn import _DT, _IDT, _cuda, _ptr, _stream
+from .gdn import _DT, _IDT, _call, _cuda, _ptr, _stream
 
 
 def _act(activation):
@@ -108,6 +111,119 @@ def _fn_args(x, weight, bias, conv_states, query_start_loc, cache_indices, has_i
     return args, (w, b, qsl, ci, hi, blocks)
 
 
+def _conv1d_bwd_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], dy: torch.Tensor,
+                     initial_state: Optional[torch.Tensor], activation: int,
+                     cu_seqlens: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor,
+                                                                  torch.Tensor]:
+    """Returns ``(dx, dweight, dbias, dinitial_state)``, the last two empty
+    where there is no bias or initial state."""
+    B, T, D = x.shape
+    W = weight.shape[1]
+    N = B if cu_seqlens is None else cu_seqlens.numel() - 1
+    dev = x.device
+
+    def rows(t):  # token rows may be strided (a view of one projection), else a packed copy
+        if not t.is_contiguous() and t.stride(2) == 1 and t.stride(1) >= D and (B == 1 or t.stride(0) == T * t.stride(1)):
+            return t, t.stride(1) if T > 1 else D
+        return t.contiguous(), D
+
+    (x, sx), (dy, sdy) = rows(x), rows(dy)
+    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
+    dw = torch.empty_like(weight)
+    db = torch.empty(0 if bias is None else D, dtype=weight.dtype, device=dev)
+    dh = torch.empty((0,) if initial_state is None else initial_state.shape,
+                     dtype=x.dtype if initial_state is None else initial_state.dtype, device=dev)
+    args = _lib.Conv1dBwdArgs(
+        x=_ptr(x), weight=_ptr(weight), bias=_ptr(bias), initial_state=_ptr(initial_state), dy=_ptr(dy), dx=_ptr(dx),
+        dweight=_ptr(dw), dbias=None if bias is None else _ptr(db),
+        dinitial_state=None if initial_state is None else _ptr(dh), cu_seqlens=_ptr(cu_seqlens), B=B, T=T, N=N, D=D,
+        stride_x_token=sx, stride_dy_token=sdy, W=W, x_dtype=_fdt(x, "x"), w_dtype=_fdt(weight, "weight"),
+        state_dtype=_fdt(initial_state, "initial_state") if initial_state is not None else _lib.GDN_F32,
+        cu_dtype=_IDT[cu_seqlens.dtype] if cu_seqlens is not None else _lib.GDN_I64, activation=activation)
+    lib = _lib.load()
+    nbytes = lib.gdn_causal_conv1d_bwd_workspace_size(args)
+    if nbytes == 0:
+        # nothing to do is no error; everything else that has no size is
+        _lib.check(_lib.GDN_ERR_INVALID)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ctypes.c_void_p(ws.data_ptr()), nbytes
+    with torch.cuda.device(dev):
+        _lib.check(lib.gdn_causal_conv1d_bwd(args, _stream(dev)))
+    return dx, dw, db, dh
+
+
+_conv1d_bwd_op = torch.library.custom_op("gdn_b200::causal_conv1d_bwd", mutates_args=(),
+                                         device_types="cuda")(_conv1d_bwd_impl)
+
+
+@_conv1d_bwd_op.register_fake
+def _(x, weight, bias, dy, initial_state, activation, cu_seqlens):
+    return (x.new_empty(x.shape), weight.new_empty(weight.shape),
+            weight.new_empty((0,) if bias is None else bias.shape),
+            x.new_empty((0,)) if initial_state is None else initial_state.new_empty(initial_state.shape))
+
+
+def causal_conv1d_bwd(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None,
+    dy: torch.Tensor,
+    initial_state: torch.Tensor | None = None,
+    activation: str | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+):
+    """Functional gradient of :func:`causal_conv1d`: x, dy ``[B, T, D]`` (token
+    rows may be strided), the other arguments as the forward took them.
+    Returns ``(dx, dweight, dbias, dinitial_state)`` in the dtypes of what they
+    are the gradients of, the last two None where there is no bias or initial
+    state.  The residual's gradient is dy itself."""
+    act = _act(activation)
+    if x.dim() != 3 or dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"[CausalConv1d] dy {tuple(dy.shape)} {dy.dtype} must match x {tuple(x.shape)} {x.dtype} [B, T, D]")
+    if weight.dim() != 2 or weight.shape[0] != x.shape[2]:
+        raise ValueError("[CausalConv1d] x.shape[-1] must be equal to weight.shape[0].")
+    if bias is not None and tuple(bias.shape) != (x.shape[2],):
+        raise ValueError(f"[CausalConv1d] bias {tuple(bias.shape)} must be ({x.shape[2]},)")
+    _cuda("causal_conv1d_bwd", x, weight, bias, dy, initial_state, cu_seqlens)
+    _fdt(x, "x"), _fdt(weight, "weight")
+    B, T, D = x.shape
+    W = weight.shape[1]
+    cu = None
+    N = B
+    if cu_seqlens is not None:
+        if B != 1:
+            raise ValueError("[CausalConv1d] cu_seqlens requires batch size 1 (packed sequences)")
+        cu = (cu_seqlens if cu_seqlens.dtype in _IDT else cu_seqlens.to(torch.int64)).contiguous()
+        N = cu.numel() - 1
+    if initial_state is not None and tuple(initial_state.shape) != (N, D, W):
+        raise ValueError(f"[CausalConv1d] initial_state {tuple(initial_state.shape)} must be [N, D, W] = {(N, D, W)}")
+    b_dtype = None if bias is None else bias.dtype
+    dx, dw, db, dh = _call(
+        torch.ops.gdn_b200.causal_conv1d_bwd, _conv1d_bwd_impl, x, weight.contiguous(),
+        None if bias is None else bias.to(weight.dtype).contiguous(), dy,
+        None if initial_state is None else initial_state.contiguous(), act, cu)
+    return dx, dw, None if bias is None else db.to(b_dtype), None if initial_state is None else dh
+
+
+class CausalConv1dFunction(torch.autograd.Function):
+    """Autograd node of :func:`causal_conv1d`: saves its inputs and recomputes
+    the pre-activations in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, initial_state, activation, cu_seqlens):
+        with torch.no_grad():
+            y, _ = causal_conv1d(x, weight, bias, residual, initial_state, activation=activation, cu_seqlens=cu_seqlens)
+        ctx.save_for_backward(x, weight, bias, initial_state, cu_seqlens)
+        ctx.activation, ctx.residual_dtype = activation, None if residual is None else residual.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, bias, initial_state, cu = ctx.saved_tensors
+        dx, dw, db, dh = causal_conv1d_bwd(x, weight, bias, dy, initial_state, ctx.activation, cu)
+        return dx, dw, db, None if ctx.residual_dtype is None else dy.to(ctx.residual_dtype), dh, None, None
+
+
 def causal_conv1d(
     x: torch.Tensor,
     weight: torch.Tensor | None = None,
@@ -128,7 +244,8 @@ def causal_conv1d(
     sequence (column j = token j - W).  Returns ``(y, None)``
     (``triton_ops.py:287-363``).  ``backend`` is accepted for signature
     compatibility ('triton' is the reference's only value; the work runs in
-    CUDA here)."""
+    CUDA here).  Differentiable in x, weight, bias, residual and initial_state
+    (:func:`causal_conv1d_bwd`)."""
     if cp_context is not None:
         raise ValueError("[CausalConv1d] CP Context not supported.")
     if output_final_state is True:
@@ -142,6 +259,9 @@ def causal_conv1d(
     if x.shape[-1] != weight.shape[0]:
         raise ValueError("[CausalConv1d] x.shape[-1] must be equal to weight.shape[0].")
     _cuda("causal_conv1d", x, weight, bias, residual, initial_state, cu_seqlens)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, weight, bias, residual, initial_state)):
+        return CausalConv1dFunction.apply(x, weight, bias, residual, initial_state, activation, cu_seqlens), None
     B, T, D = x.shape
     W = weight.shape[1]
     x = x.contiguous()

@@ -36,58 +36,6 @@ constexpr int kU = 8;          // tokens loaded ahead per thread (vector path)
 constexpr int kThreads = 128;  // threads per CTA (each owns one channel vector)
 constexpr int kMaxW = 16;
 
-__device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
-  if (dtype == GDN_F32) return static_cast<const float*>(p)[i];
-  if (dtype == GDN_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
-  if (dtype == GDN_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == GDN_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
-
-// VEC consecutive elements <-> floats; one 128-bit access when VEC fills 16 B.
-template <typename T, int VEC>
-__device__ __forceinline__ void ldv(const T* p, float* v) {
-  if constexpr (VEC * sizeof(T) == 16) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = to_f<T>(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = to_f<T>(p[i]);
-  }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void stv(T* p, const float* v) {
-  if constexpr (VEC * sizeof(T) == 16 && sizeof(T) == 2) {  // two lanes per rounding instruction
-    uint4 u;
-    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-    for (int i = 0; i < VEC; i += 2) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[i], v[i + 1]);
-        w[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
-      } else {
-        const __half2 b = __floats2half2_rn(v[i], v[i + 1]);
-        w[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
-      }
-    }
-    *reinterpret_cast<uint4*>(p) = u;
-  } else if constexpr (VEC * sizeof(T) == 16) {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) e[i] = from_f<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) p[i] = from_f<T>(v[i]);
-  }
-}
-
 struct FwdParams {
   const void* x;
   void* y;

@@ -1,0 +1,503 @@
+// The selective state space scan: the recurrent prompt kernel for every type
+// and head size, the kernel that hands states from segment to segment, and
+// the C entry points.  The tensor-core prompt kernels are in gdn_scan_tc.cu.
+//
+// A prompt is cut into segments when there are too few (sequence, head)
+// pairs to fill the GPU: the first pass computes the state that each
+// segment but the last of a sequence adds, starting from zero, and its log
+// decay; scan_pass_kernel turns those into the states the segments start
+// from; the second pass computes the outputs (and the last segment's final
+// state).  With one segment per sequence the second pass is the only one.
+
+#include "gdn_scan.h"
+#include "scan_common.cuh"
+
+#include <algorithm>
+
+namespace gdn {
+namespace scan {
+
+constexpr int kTok = 16;  // tokens staged together
+
+// One CTA per (segment, head, slice of ROWS state rows).  LPR lanes share a
+// state row; each holds SPT of its columns (columns i*4*LPR + 4*lane + e, so
+// that the lanes read 16-byte pieces of B and C side by side).  Per token and
+// thread: 2 SPT multiply-adds for the state, SPT for the output, a shuffle
+// reduction over LPR lanes.  Everything in fp32; issue-bound.
+template <typename T, int SPT, int LPR, bool OUT>
+__global__ void __launch_bounds__(256) scan_rec_kernel(const ScanParams p) {
+  constexpr int SP = SPT * LPR;  // padded state width
+  constexpr int ROWS = 256 / LPR;
+  __shared__ __align__(16) float sb[kTok][SP], sc[OUT ? kTok : 1][SP];
+  __shared__ float sx[kTok][ROWS + 1], sy[OUT ? kTok : 1][ROWS + 1], sdt[kTok], sda[kTok], sdecay[kTok];
+  __shared__ int64_t seg_n, seg_t0, seg_t1;
+  __shared__ int seg_ok, seg_last;
+  const int64_t id = blockIdx.x;
+  const int h = blockIdx.y, g = h / (p.H / p.G);
+  const int row0 = blockIdx.z * ROWS;
+  clear_error(p);
+  if (threadIdx.x < 32) {
+    int64_t n = 0, ls = 0, t0 = 0, t1 = 0;
+    bool last = false;
+    const bool ok = find_segment(p, id, n, ls, t0, t1, last);
+    if (threadIdx.x == 0) {
+      seg_n = n; seg_t0 = t0; seg_t1 = t1;
+      seg_ok = ok; seg_last = last;
+    }
+  }
+  __syncthreads();
+  if (!seg_ok || (!OUT && seg_last)) return;
+  const int64_t n = seg_n, t0 = seg_t0, t1 = seg_t1;
+  const bool last = seg_last;
+  const int lane = threadIdx.x % LPR, r = threadIdx.x / LPR, row = row0 + r;
+  const bool live = row < p.P;
+  const float A = p.A[h], D = p.D ? p.D[h] : 0.f, bias = p.dt_bias ? p.dt_bias[h] : 0.f;
+  float st[SPT];
+  const int64_t at_seq = ((n * p.H + h) * p.P + row) * p.S;
+  const int64_t at_seg = ((id * p.H + h) * p.P + row) * p.S;
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
+    st[i] = 0.f;
+    if (OUT && live && s < p.S) {
+      if (p.seg_state) st[i] = p.seg_state[at_seg + s];
+      else if (p.init) st[i] = ld_any(p.init, p.init_dtype, at_seq + s);
+    }
+  }
+  float logd = 0.f;
+  for (int64_t t = t0; t < t1; t += kTok) {
+    const int cnt = static_cast<int>(min64(kTok, t1 - t));
+    for (int i = threadIdx.x; i < kTok * SP; i += 256) {
+      const int k = i / SP, s = i % SP;
+      const bool in = k < cnt && s < p.S;
+      sb[k][s] = in ? to_f<T>(static_cast<const T*>(p.b)[(t + k) * p.sb + static_cast<int64_t>(g) * p.S + s]) : 0.f;
+      if (OUT) sc[k][s] = in ? to_f<T>(static_cast<const T*>(p.c)[(t + k) * p.sc + static_cast<int64_t>(g) * p.S + s]) : 0.f;
+    }
+    for (int i = threadIdx.x; i < kTok * ROWS; i += 256) {
+      const int k = i / ROWS, q = i % ROWS;
+      sx[k][q] = k < cnt && row0 + q < p.P
+                     ? to_f<T>(static_cast<const T*>(p.x)[(t + k) * p.sx + static_cast<int64_t>(h) * p.P + row0 + q])
+                     : 0.f;
+    }
+    if (threadIdx.x < kTok) {
+      float d = 0.f;
+      if (threadIdx.x < cnt)
+        d = step_of(ld_any(p.dt, p.dt_dtype, (t + threadIdx.x) * p.sdt + h), bias, p.softplus, p.dt_lo, p.dt_hi);
+      sdt[threadIdx.x] = d;
+      sda[threadIdx.x] = d * A;
+      sdecay[threadIdx.x] = expf(d * A);
+    }
+    __syncthreads();
+    for (int k = 0; k < cnt; ++k) {
+      const float decay = sdecay[k], u = sdt[k] * sx[k][r];
+      logd += sda[k];
+      float acc = 0.f;
+#pragma unroll
+      for (int i = 0; i < SPT; i += 4) {
+        const int s = i * LPR + lane * 4;
+        const float4 bv = *reinterpret_cast<const float4*>(&sb[k][s]);
+        st[i] = fmaf(decay, st[i], u * bv.x);
+        st[i + 1] = fmaf(decay, st[i + 1], u * bv.y);
+        st[i + 2] = fmaf(decay, st[i + 2], u * bv.z);
+        st[i + 3] = fmaf(decay, st[i + 3], u * bv.w);
+        if (OUT) {
+          const float4 cv = *reinterpret_cast<const float4*>(&sc[k][s]);
+          acc = fmaf(st[i], cv.x, acc);
+          acc = fmaf(st[i + 1], cv.y, acc);
+          acc = fmaf(st[i + 2], cv.z, acc);
+          acc = fmaf(st[i + 3], cv.w, acc);
+        }
+      }
+      if (OUT) {
+        acc = group_sum<LPR>(acc);
+        if (lane == 0) sy[k][r] = fmaf(D, sx[k][r], acc);
+      }
+    }
+    __syncthreads();
+    if (OUT) {
+      for (int i = threadIdx.x; i < cnt * ROWS; i += 256) {
+        const int k = i / ROWS, q = i % ROWS;
+        if (row0 + q >= p.P) continue;
+        float v = sy[k][q];
+        const int64_t col = static_cast<int64_t>(h) * p.P + row0 + q;
+        if (p.z) v *= silu(to_f<T>(static_cast<const T*>(p.z)[(t + k) * p.sz + col]));
+        static_cast<T*>(p.y)[(t + k) * p.H * p.P + col] = from_f<T>(v);
+      }
+      // sx and sy are rewritten after the next tile's first barrier only
+      // when that tile's loads are done: keep the two phases apart
+      __syncthreads();
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
+    if (s >= p.S) continue;
+    if (!OUT) p.seg_state[at_seg + s] = st[i];
+    else if (last && p.final_state) st_any(p.final_state, p.final_dtype, at_seq + s, st[i]);
+  }
+  if (!OUT && row == 0 && lane == 0) p.seg_decay[id * p.H + h] = logd;
+}
+
+// States between segments: for each sequence, head and state element, in
+// order, seg_state[i] <- h and h <- exp(log decay of i) h + seg_state[i].
+// One thread per four elements; a stream over the segments' states.
+__global__ void __launch_bounds__(256) scan_pass_kernel(const ScanParams p) {
+  __shared__ int64_t first_sh, count_sh;
+  const int64_t n = blockIdx.z;
+  const int h = blockIdx.y;
+  if (threadIdx.x < 32) {  // the sequence's first segment and their number
+    int64_t sum = 0, mine = 0;
+    for (int64_t m = threadIdx.x; m <= n; m += 32) {
+      int64_t bos, eos;
+      seq_bounds(p.cu, p.cu_dtype, m, p.T, bos, eos);
+      bos = min64(max(bos, static_cast<int64_t>(0)), p.total);
+      eos = min64(max(eos, bos), p.total);
+      const int64_t k = max((eos - bos + p.seg - 1) / p.seg, static_cast<int64_t>(1));
+      if (m == n) mine = k;
+      else sum += k;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    }
+    if (threadIdx.x == 0) {
+      first_sh = sum;
+      count_sh = mine;
+    }
+  }
+  __syncthreads();
+  const int64_t PS = static_cast<int64_t>(p.P) * p.S;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= PS) return;
+  const int64_t first = first_sh, count = min64(count_sh, p.segments - first);
+  float cur = p.init ? ld_any(p.init, p.init_dtype, (n * p.H + h) * PS + i) : 0.f;
+  float* st = p.seg_state + (first * p.H + h) * PS + i;
+  const float* ld = p.seg_decay + first * p.H + h;
+  const int64_t step = p.H * PS;
+  int64_t k = 0;
+  for (; k + 4 < count; k += 4) {  // four segments' loads in flight
+    float v[4], d[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = st[(k + j) * step];
+      d[j] = expf(ld[(k + j) * p.H]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      st[(k + j) * step] = cur;
+      cur = fmaf(d[j], cur, v[j]);
+    }
+  }
+  for (; k < count; ++k) {
+    const float v = k + 1 < count ? st[k * step] : 0.f;
+    const float d = k + 1 < count ? expf(ld[k * p.H]) : 1.f;
+    st[k * step] = cur;
+    cur = fmaf(d, cur, v);
+  }
+}
+
+// ---- single tokens ---------------------------------------------------------
+struct UpdateParams {
+  const void *x, *dt, *b, *c, *z;
+  const float *A, *D, *dt_bias;
+  void *state, *y;
+  const void* idx;
+  int* err;
+  int64_t N, slots, s_slot;
+  int64_t sx, sdt, sb, sc, sz;
+  int H, P, G, S;
+  int dt_dtype, idx_dtype, softplus;
+  float dt_lo, dt_hi;
+};
+
+// The state line of (token, head) is read and written once; nothing else is
+// of its size, so HBM bounds the kernel.  LPR lanes hold one row of S (VEC
+// columns each, ITER times); a warp moves R rows at a time, all of whose
+// loads are in flight together.
+template <typename T, typename CT, int VEC, int LPR, int ITER, int R>
+__global__ void __launch_bounds__(128) scan_update_kernel(const UpdateParams p) {
+  constexpr int RW = 32 / LPR;  // rows side by side in a warp
+  constexpr int BLK = 4 * RW * R;
+  const int64_t n = blockIdx.z;
+  const int h = blockIdx.y, g = h / (p.H / p.G);
+  const int lane = threadIdx.x % LPR, sub = (threadIdx.x & 31) / LPR, warp = threadIdx.x >> 5;
+  const int row0 = blockIdx.x * BLK + warp * RW * R + sub;
+  const int64_t slot = p.idx ? load_index(p.idx, p.idx_dtype, n) : n;
+  T* y = static_cast<T*>(p.y) + (n * p.H + h) * p.P;
+  if (slot < 0 || slot >= p.slots) {  // padding, or an index out of the cache: no state, output zero
+    if (slot >= p.slots && threadIdx.x == 0 && blockIdx.x == 0 && h == 0)
+      record_device_error(p.err, kErrSlotRange, kSiteSlotInitial, static_cast<int>(n), static_cast<int>(slot));
+    for (int r = threadIdx.x; r < BLK; r += 128)
+      if (blockIdx.x * BLK + r < p.P) y[blockIdx.x * BLK + r] = from_f<T>(0.f);
+    return;
+  }
+  CT* st = static_cast<CT*>(p.state) + slot * p.s_slot + static_cast<int64_t>(h) * p.P * p.S;
+  float v[R][ITER][VEC];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      const int row = row0 + r * RW, s = (k * LPR + lane) * VEC;
+      if (row < p.P && s < p.S) conv::ldv<CT, VEC>(st + static_cast<int64_t>(row) * p.S + s, v[r][k]);
+      else
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[r][k][e] = 0.f;
+    }
+  const float dt = step_of(ld_any(p.dt, p.dt_dtype, n * p.sdt + h), p.dt_bias ? p.dt_bias[h] : 0.f, p.softplus,
+                           p.dt_lo, p.dt_hi);
+  const float decay = expf(dt * p.A[h]), D = p.D ? p.D[h] : 0.f;
+  const T* B = static_cast<const T*>(p.b) + n * p.sb + static_cast<int64_t>(g) * p.S;
+  const T* C = static_cast<const T*>(p.c) + n * p.sc + static_cast<int64_t>(g) * p.S;
+  float bv[ITER][VEC], cv[ITER][VEC];
+#pragma unroll
+  for (int k = 0; k < ITER; ++k)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int s = (k * LPR + lane) * VEC + e;
+      bv[k][e] = s < p.S ? to_f<T>(B[s]) : 0.f;
+      cv[k][e] = s < p.S ? to_f<T>(C[s]) : 0.f;
+    }
+  float out = 0.f;  // row row0 + lane * RW's output, in lane `lane` < R
+  const T* x = static_cast<const T*>(p.x) + n * p.sx + static_cast<int64_t>(h) * p.P;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row0 + r * RW;
+    const float xv = row < p.P ? to_f<T>(x[row]) : 0.f, u = dt * xv;
+    float acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      const int s = (k * LPR + lane) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[r][k][e] = fmaf(decay, v[r][k][e], u * bv[k][e]);
+        acc = fmaf(v[r][k][e], cv[k][e], acc);
+      }
+      if (row < p.P && s < p.S) conv::stv<CT, VEC>(st + static_cast<int64_t>(row) * p.S + s, v[r][k]);
+    }
+    acc = group_sum<LPR>(acc);
+    if (lane == r % LPR) {
+      float yv = fmaf(D, xv, acc);
+      out = yv;
+    }
+  }
+  static_assert(LPR >= R, "a lane per row");
+  if (lane < R) {
+    const int row = row0 + lane * RW;
+    if (row < p.P) {
+      if (p.z) out *= silu(to_f<T>(static_cast<const T*>(p.z)[n * p.sz + static_cast<int64_t>(h) * p.P + row]));
+      y[row] = from_f<T>(out);
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------
+bool fdtype_ok(int d) { return d == GDN_F32 || d == GDN_BF16 || d == GDN_F16; }
+bool idtype_ok(int d) { return d == GDN_I32 || d == GDN_I64; }
+
+int check(const gdn_scan_args* a) {
+  if (!a) return set_last_error(GDN_ERR_INVALID, "null args");
+  if (a->B < 0 || a->T < 0 || a->N < 0 || a->H <= 0 || a->P <= 0 || a->G <= 0 || a->S <= 0)
+    return set_last_error(GDN_ERR_INVALID, "non-positive dimension (B=%lld T=%lld N=%lld H=%d P=%d G=%d S=%d)",
+                          (long long)a->B, (long long)a->T, (long long)a->N, a->H, a->P, a->G, a->S);
+  if (a->H % a->G != 0) return set_last_error(GDN_ERR_INVALID, "H=%d is not a multiple of G=%d", a->H, a->G);
+  if (a->P > 256 || a->S > 256) return set_last_error(GDN_ERR_UNSUPPORTED, "P=%d, S=%d: both must be <= 256", a->P, a->S);
+  if (a->H > 65535 || a->N > 65535) return set_last_error(GDN_ERR_UNSUPPORTED, "H and N must be at most 65535");
+  if (a->cu_seqlens) {
+    if (!idtype_ok(a->cu_dtype)) return set_last_error(GDN_ERR_INVALID, "cu_seqlens dtype must be I32 or I64");
+    if (a->B != 1) return set_last_error(GDN_ERR_INVALID, "cu_seqlens requires B == 1 (got B=%lld)", (long long)a->B);
+  } else if (a->N != a->B) {
+    return set_last_error(GDN_ERR_INVALID, "without cu_seqlens N must equal B (N=%lld B=%lld)", (long long)a->N,
+                          (long long)a->B);
+  }
+  if (!fdtype_ok(a->dtype) || !fdtype_ok(a->dt_dtype) || !fdtype_ok(a->init_dtype) || !fdtype_ok(a->final_dtype))
+    return set_last_error(GDN_ERR_INVALID, "dtypes must be F32, BF16 or F16");
+  const int64_t hp = static_cast<int64_t>(a->H) * a->P, gs = static_cast<int64_t>(a->G) * a->S;
+  if (a->stride_x < hp || (a->z && a->stride_z < hp) || a->stride_b < gs || a->stride_c < gs || a->stride_dt < a->H)
+    return set_last_error(GDN_ERR_INVALID, "token strides must cover a token's packed row");
+  if (!(a->dt_min <= a->dt_max)) return set_last_error(GDN_ERR_INVALID, "dt_min must not exceed dt_max");
+  return GDN_OK;
+}
+
+struct Plan {
+  int64_t seg, segments;  // tokens per segment; at most so many segments
+  bool split;
+  size_t state_off, decay_off, bytes;  // the error word comes first
+};
+
+// Segment length: as many (segment, head, row slice) CTAs as fill the GPU
+// a few times, but no segment under `least` tokens (below it the passes over
+// states cost more than the tokens).  Without a device query, so the result
+// depends on the shapes alone.
+Plan plan(const gdn_scan_args& a) {
+  Plan pl{};
+  const bool tc = tc_applies(a);
+  const int64_t total = a.B * a.T;
+  const int64_t slices = tc ? tc_slices(a) : (a.P + 63) / 64;
+  const int64_t want = 148 * 4, least = 512;
+  const int64_t per_token = std::max<int64_t>(1, a.H * slices);
+  int64_t pieces = std::max<int64_t>(1, (want + per_token - 1) / per_token);
+  pl.seg = std::max(least, (total + pieces - 1) / pieces);
+  pl.seg = (pl.seg + 127) / 128 * 128;
+  pl.split = a.N > 0 && a.N * per_token < want && total > least;
+  if (!pl.split) pl.seg = std::max<int64_t>(128, (total + 127) / 128 * 128);
+  // every sequence has at most ceil(len / seg) segments, and at least one
+  pl.segments = pl.split ? total / pl.seg + a.N : a.N;
+  pl.state_off = pl.bytes = 256;
+  if (pl.split) {
+    const size_t states = static_cast<size_t>(pl.segments) * a.H * a.P * a.S * sizeof(float);
+    pl.decay_off = pl.state_off + (states + 255) / 256 * 256;
+    pl.bytes = pl.decay_off + static_cast<size_t>(pl.segments) * a.H * sizeof(float);
+  }
+  return pl;
+}
+
+template <typename T, int SPT, int LPR>
+void launch_rec(ScanParams p, const Plan& pl, cudaStream_t s) {
+  constexpr int ROWS = 256 / LPR;
+  const dim3 grid(static_cast<unsigned>(pl.segments), static_cast<unsigned>(p.H),
+                  static_cast<unsigned>((p.P + ROWS - 1) / ROWS));
+  if (pl.split) {
+    note_launch();
+    scan_rec_kernel<T, SPT, LPR, false><<<grid, 256, 0, s>>>(p);
+    launch_pass(p, s);
+    p.clear_err = 0;
+  }
+  note_launch();
+  scan_rec_kernel<T, SPT, LPR, true><<<grid, 256, 0, s>>>(p);
+}
+
+template <typename T>
+void launch_t(const ScanParams& p, const Plan& pl, cudaStream_t s) {
+  if (p.S <= 16) launch_rec<T, 4, 4>(p, pl, s);
+  else if (p.S <= 32) launch_rec<T, 8, 4>(p, pl, s);
+  else if (p.S <= 64) launch_rec<T, 16, 4>(p, pl, s);
+  else if (p.S <= 128) launch_rec<T, 32, 4>(p, pl, s);
+  else launch_rec<T, 32, 8>(p, pl, s);
+}
+
+void launch_pass(const ScanParams& p, cudaStream_t s) {
+  const int64_t PS = static_cast<int64_t>(p.P) * p.S;
+  note_launch();
+  scan_pass_kernel<<<dim3(static_cast<unsigned>((PS + 255) / 256), static_cast<unsigned>(p.H), static_cast<unsigned>(p.N)),
+                     256, 0, s>>>(p);
+}
+
+template <typename T, typename CT, int VEC, int LPR, int ITER, int R>
+void launch_upd(const UpdateParams& p, cudaStream_t s) {
+  constexpr int BLK = 4 * (32 / LPR) * R;
+  const dim3 grid(static_cast<unsigned>((p.P + BLK - 1) / BLK), static_cast<unsigned>(p.H), static_cast<unsigned>(p.N));
+  scan_update_kernel<T, CT, VEC, LPR, ITER, R><<<grid, 128, 0, s>>>(p);
+}
+
+// Lanes per row: S in 16-byte vectors where the rows allow them, else
+// single columns.
+template <typename T, typename CT>
+void update_t(const UpdateParams& p, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(CT);
+  const bool vec = p.S % V == 0 && p.s_slot % V == 0 && (reinterpret_cast<uintptr_t>(p.state) & 15) == 0;
+  if (vec) {
+    const int n = p.S / V;
+    if (n <= 4) launch_upd<T, CT, V, 4, 1, 4>(p, s);
+    else if (n <= 8) launch_upd<T, CT, V, 8, 1, 4>(p, s);
+    else if (n <= 16) launch_upd<T, CT, V, 16, 1, 4>(p, s);
+    else if (n <= 32) launch_upd<T, CT, V, 32, 1, 8>(p, s);
+    else launch_upd<T, CT, V, 32, 2, 4>(p, s);
+  } else {
+    if (p.S <= 32) launch_upd<T, CT, 1, 32, 1, 8>(p, s);
+    else if (p.S <= 128) launch_upd<T, CT, 1, 32, 4, 4>(p, s);
+    else launch_upd<T, CT, 1, 32, 8, 4>(p, s);
+  }
+}
+
+template <typename T>
+void update_c(const UpdateParams& p, int state_dtype, cudaStream_t s) {
+  if (state_dtype == GDN_F32) update_t<T, float>(p, s);
+  else if (state_dtype == GDN_BF16) update_t<T, __nv_bfloat16>(p, s);
+  else update_t<T, __half>(p, s);
+}
+
+}  // namespace scan
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::scan;
+
+extern "C" GDN_API size_t gdn_scan_workspace_size(const gdn_scan_args* a) {
+  if (check(a)) return 0;
+  return plan(*a).bytes;
+}
+
+extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
+  const int rc = check(a);
+  if (rc != GDN_OK) return rc;
+  const int64_t total = a->B * a->T;
+  if (!a->A || (total > 0 && (!a->x || !a->dt || !a->b || !a->c || !a->y)))
+    return set_last_error(GDN_ERR_INVALID, "x, dt, A, b, c and y must be non-null");
+  const Plan pl = plan(*a);
+  if (!a->workspace || a->workspace_bytes < pl.bytes)
+    return set_last_error(GDN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", a->workspace_bytes, pl.bytes);
+  if (a->N == 0) return GDN_OK;
+  ScanParams p{};
+  p.x = a->x; p.dt = a->dt; p.b = a->b; p.c = a->c; p.z = a->z; p.A = a->A; p.D = a->D; p.dt_bias = a->dt_bias;
+  p.init = a->initial_state; p.y = a->y; p.final_state = a->final_state; p.cu = a->cu_seqlens;
+  if (pl.split) {
+    p.seg_state = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.state_off);
+    p.seg_decay = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.decay_off);
+  }
+  p.err = static_cast<int*>(a->workspace);
+  p.clear_err = 1;
+  p.T = a->T; p.N = a->N; p.total = total; p.seg = pl.seg; p.segments = pl.segments;
+  p.sx = a->stride_x; p.sdt = a->stride_dt; p.sb = a->stride_b; p.sc = a->stride_c; p.sz = a->stride_z;
+  p.H = a->H; p.P = a->P; p.G = a->G; p.S = a->S;
+  p.dt_dtype = a->dt_dtype; p.init_dtype = a->init_dtype; p.final_dtype = a->final_dtype; p.cu_dtype = a->cu_dtype;
+  p.softplus = a->dt_softplus; p.dt_lo = a->dt_min; p.dt_hi = a->dt_max;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == GDN_F32) launch_t<float>(p, pl, s);
+  else if (a->dtype == GDN_BF16) launch_t<__nv_bfloat16>(p, pl, s);
+  else launch_t<__half>(p, pl, s);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_last_error(GDN_ERR_CUDA, "gdn_scan_fwd: %s", cudaGetErrorString(e));
+  return GDN_OK;
+}
+
+extern "C" GDN_API int gdn_scan_update(const gdn_scan_update_args* a, void* stream) {
+  if (!a) return set_last_error(GDN_ERR_INVALID, "null args");
+  if (a->N < 0 || a->H <= 0 || a->P <= 0 || a->G <= 0 || a->S <= 0 || a->num_slots < 0)
+    return set_last_error(GDN_ERR_INVALID, "non-positive dimension (N=%lld H=%d P=%d G=%d S=%d)", (long long)a->N, a->H,
+                          a->P, a->G, a->S);
+  if (a->H % a->G != 0) return set_last_error(GDN_ERR_INVALID, "H=%d is not a multiple of G=%d", a->H, a->G);
+  if (a->S > 256) return set_last_error(GDN_ERR_UNSUPPORTED, "S=%d must be <= 256", a->S);
+  if (a->H > 65535 || a->N > 65535) return set_last_error(GDN_ERR_UNSUPPORTED, "H and N must be at most 65535");
+  if (!fdtype_ok(a->dtype) || !fdtype_ok(a->dt_dtype) || !fdtype_ok(a->state_dtype))
+    return set_last_error(GDN_ERR_INVALID, "dtypes must be F32, BF16 or F16");
+  if (a->ssm_state_indices && !idtype_ok(a->idx_dtype))
+    return set_last_error(GDN_ERR_INVALID, "ssm_state_indices dtype must be I32 or I64");
+  if (!a->ssm_state_indices && a->num_slots < a->N)
+    return set_last_error(GDN_ERR_INVALID, "%lld cache lines for %lld tokens", (long long)a->num_slots, (long long)a->N);
+  const int64_t hp = static_cast<int64_t>(a->H) * a->P, gs = static_cast<int64_t>(a->G) * a->S;
+  if (a->stride_x < hp || (a->z && a->stride_z < hp) || a->stride_b < gs || a->stride_c < gs || a->stride_dt < a->H ||
+      a->stride_slot < hp * a->S)
+    return set_last_error(GDN_ERR_INVALID, "strides must cover a token's packed row and a cache line");
+  if (!(a->dt_min <= a->dt_max)) return set_last_error(GDN_ERR_INVALID, "dt_min must not exceed dt_max");
+  if (a->N == 0) return GDN_OK;
+  if (!a->x || !a->dt || !a->A || !a->b || !a->c || !a->state || !a->y)
+    return set_last_error(GDN_ERR_INVALID, "x, dt, A, b, c, state and y must be non-null");
+  UpdateParams p{};
+  p.x = a->x; p.dt = a->dt; p.b = a->b; p.c = a->c; p.z = a->z; p.A = a->A; p.D = a->D; p.dt_bias = a->dt_bias;
+  p.state = a->state; p.y = a->y; p.idx = a->ssm_state_indices; p.err = a->err;
+  p.N = a->N; p.slots = a->num_slots; p.s_slot = a->stride_slot;
+  p.sx = a->stride_x; p.sdt = a->stride_dt; p.sb = a->stride_b; p.sc = a->stride_c; p.sz = a->stride_z;
+  p.H = a->H; p.P = a->P; p.G = a->G; p.S = a->S;
+  p.dt_dtype = a->dt_dtype; p.idx_dtype = a->idx_dtype; p.softplus = a->dt_softplus;
+  p.dt_lo = a->dt_min; p.dt_hi = a->dt_max;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  note_launch();
+  if (a->dtype == GDN_F32) update_c<float>(p, a->state_dtype, s);
+  else if (a->dtype == GDN_BF16) update_c<__nv_bfloat16>(p, a->state_dtype, s);
+  else update_c<__half>(p, a->state_dtype, s);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_last_error(GDN_ERR_CUDA, "gdn_scan_update: %s", cudaGetErrorString(e));
+  return GDN_OK;
+}

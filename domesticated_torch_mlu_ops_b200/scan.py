@@ -1,0 +1,277 @@
+"""Selective state space scan with one decay per head: the sibling of the
+delta rule in hybrid models, for prompts (``chunk_selective_scan``) and for
+single tokens on a slot-indexed cache (``selective_scan_update``).
+
+Per head, with the step ``dt = clamp(softplus(raw + dt_bias))``::
+
+    h_t = exp(dt_t A) h_{t-1} + dt_t x_t B_t^T        state [P, S], fp32
+    y_t = (h_t C_t + D x_t) silu(z_t)
+
+The work runs in ``libgdn_b200.so`` (``gdn_scan.cu``, ``gdn_scan_tc.cu``)
+through its C ABI; there is no CPU path.  The ops are the ``torch.library``
+custom ops ``gdn_b200::scan_fwd`` and ``gdn_b200::scan_update`` (which declares
+the cache as mutated).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .gdn import _DT, _IDT, _call, _cuda, _err_word, _f32, _idx, _ptr, _raise_err_word, _stream
+
+Tensor = torch.Tensor
+_INF = float("inf")
+
+
+def _packed_rows(t, tail):
+    """(tensor, distance between token rows) of ``t`` whose last ``tail``
+    dimensions are one packed row: in place when only the token rows are
+    strided (views of one projection), else a packed copy."""
+    width = 1
+    for n in t.shape[t.dim() - tail:]:
+        width *= n
+    if t.is_contiguous():
+        return t, width
+    want, ok = 1, True
+    for n, st in zip(reversed(t.shape[t.dim() - tail:]), reversed(t.stride()[t.dim() - tail:])):
+        ok = ok and (n == 1 or st == want)
+        want *= n
+    lead = [(n, st) for n, st in zip(t.shape[:t.dim() - tail], t.stride()) if n != 1]
+    if len(lead) == 2 and lead[0][1] == lead[1][0] * lead[1][1]:
+        lead = lead[1:]
+    if ok and not lead:
+        return t, width
+    if ok and len(lead) == 1 and lead[0][1] >= width:
+        return t, lead[0][1]
+    return t.contiguous(), width
+
+
+def _scan_fwd_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor], z: Optional[Tensor],
+                   dt_bias: Optional[Tensor], dt_softplus: bool, dt_min: float, dt_max: float,
+                   initial_state: Optional[Tensor], output_final_state: bool, state_dtype: torch.dtype,
+                   cu_seqlens: Optional[Tensor], force_generic: bool, check_errors: bool) -> tuple[Tensor, Tensor]:
+    """Returns ``(y, final_state)``; final_state is empty when not requested."""
+    Bt, T, H, P = x.shape
+    G, S = B.shape[2], B.shape[3]
+    N = Bt if cu_seqlens is None else cu_seqlens.numel() - 1
+    dev = x.device
+    (x, sx), (dt, sdt), (B, sb), (C, sc) = _packed_rows(x, 2), _packed_rows(dt, 1), _packed_rows(B, 2), _packed_rows(C, 2)
+    z, sz = (None, 0) if z is None else _packed_rows(z, 2)
+    y = torch.empty((Bt, T, H, P), dtype=x.dtype, device=dev)
+    fin = torch.empty((N, H, P, S) if output_final_state else (0,), dtype=state_dtype, device=dev)
+    args = _lib.ScanArgs(
+        x=_ptr(x), dt=_ptr(dt), A=_ptr(A), b=_ptr(B), c=_ptr(C), D=_ptr(D), z=_ptr(z), dt_bias=_ptr(dt_bias),
+        initial_state=_ptr(initial_state), y=_ptr(y), final_state=_ptr(fin) if output_final_state else None,
+        cu_seqlens=_ptr(cu_seqlens), B=Bt, T=T, N=N, stride_x=sx, stride_dt=sdt, stride_b=sb, stride_c=sc, stride_z=sz,
+        H=H, P=P, G=G, S=S, dtype=_DT[x.dtype], dt_dtype=_DT[dt.dtype],
+        init_dtype=_DT[initial_state.dtype] if initial_state is not None else _lib.GDN_F32,
+        final_dtype=_DT[state_dtype], cu_dtype=_IDT[cu_seqlens.dtype] if cu_seqlens is not None else _lib.GDN_I64,
+        dt_softplus=int(dt_softplus), force_generic=int(force_generic), dt_min=dt_min, dt_max=dt_max)
+    lib = _lib.load()
+    nbytes = lib.gdn_scan_workspace_size(args)
+    if nbytes == 0:
+        _lib.check(_lib.GDN_ERR_INVALID)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ctypes.c_void_p(ws.data_ptr()), nbytes
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        _lib.check(lib.gdn_scan_fwd(args, stream))
+        if check_errors:
+            _lib.check(lib.gdn_chunk_check_device_error(args.workspace, stream))
+    return y, fin
+
+
+_scan_fwd_op = torch.library.custom_op("gdn_b200::scan_fwd", mutates_args=(), device_types="cuda")(_scan_fwd_impl)
+
+
+@_scan_fwd_op.register_fake
+def _(x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, initial_state, output_final_state, state_dtype,
+      cu_seqlens, force_generic, check_errors):
+    N = x.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    shape = (N, x.shape[2], x.shape[3], B.shape[3]) if output_final_state else (0,)
+    return x.new_empty(x.shape), x.new_empty(shape, dtype=state_dtype)
+
+
+def _scan_update_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor],
+                      z: Optional[Tensor], dt_bias: Optional[Tensor], dt_softplus: bool, dt_min: float, dt_max: float,
+                      state: Tensor, ssm_state_indices: Optional[Tensor], check_errors: bool) -> Tensor:
+    """One token per sequence; updates ``state`` in place and returns y."""
+    N, H, P = x.shape
+    G, S = B.shape[1], B.shape[2]
+    dev = x.device
+    (x, sx), (dt, sdt), (B, sb), (C, sc) = _packed_rows(x, 2), _packed_rows(dt, 1), _packed_rows(B, 2), _packed_rows(C, 2)
+    z, sz = (None, 0) if z is None else _packed_rows(z, 2)
+    y = torch.empty((N, H, P), dtype=x.dtype, device=dev)
+    if N == 0:
+        return y
+    err = _err_word(dev)
+    args = _lib.ScanUpdateArgs(
+        x=_ptr(x), dt=_ptr(dt), A=_ptr(A), b=_ptr(B), c=_ptr(C), D=_ptr(D), z=_ptr(z), dt_bias=_ptr(dt_bias),
+        state=_ptr(state), y=_ptr(y), ssm_state_indices=_ptr(ssm_state_indices), err=_ptr(err),
+        N=N, num_slots=state.shape[0], stride_slot=state.stride(0) if state.shape[0] > 1 else H * P * S,
+        stride_x=sx, stride_dt=sdt, stride_b=sb, stride_c=sc, stride_z=sz, H=H, P=P, G=G, S=S, dtype=_DT[x.dtype],
+        dt_dtype=_DT[dt.dtype], state_dtype=_DT[state.dtype],
+        idx_dtype=_IDT[ssm_state_indices.dtype] if ssm_state_indices is not None else _lib.GDN_I64,
+        dt_softplus=int(dt_softplus), dt_min=dt_min, dt_max=dt_max)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().gdn_scan_update(args, _stream(dev)))
+        if check_errors:
+            _raise_err_word(err)
+    return y
+
+
+_scan_update_op = torch.library.custom_op("gdn_b200::scan_update", mutates_args=("state",),
+                                          device_types="cuda")(_scan_update_impl)
+
+
+@_scan_update_op.register_fake
+def _(x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, state, ssm_state_indices, check_errors):
+    return x.new_empty(x.shape)
+
+
+def _check(name, lead, x, dt, A, B, C, D, z, dt_bias, dt_limit):
+    H, P = x.shape[-2:]
+    if x.dtype not in _DT:
+        raise ValueError(f"{name}: x dtype {x.dtype} must be float32, bfloat16 or float16")
+    if B.dim() != x.dim() or B.shape != C.shape or B.shape[:-2] != x.shape[:-2]:
+        raise ValueError(f"{name}: B {tuple(B.shape)} and C {tuple(C.shape)} must be [{lead}, G, S]")
+    if B.shape[-2] == 0 or H % B.shape[-2] != 0:
+        raise ValueError(f"{name}: {H} heads are no multiple of {B.shape[-2]} groups")
+    if B.dtype != x.dtype or C.dtype != x.dtype or (z is not None and z.dtype != x.dtype):
+        raise ValueError(f"{name}: x, B, C and z must share a dtype")
+    if z is not None and z.shape != x.shape:
+        raise ValueError(f"{name}: z {tuple(z.shape)} must match x {tuple(x.shape)}")
+    if dt.shape != x.shape[:-1] or dt.dtype not in _DT:
+        raise ValueError(f"{name}: dt {tuple(dt.shape)} {dt.dtype} must be {tuple(x.shape[:-1])} of a float type")
+    for what, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
+        if t is not None and tuple(t.shape) != (H,):
+            raise ValueError(f"{name}: {what} {tuple(t.shape)} must be ({H},), one value per head")
+    lo, hi = float(dt_limit[0]), float(dt_limit[1])
+    if not lo <= hi:
+        raise ValueError(f"{name}: dt_limit {dt_limit} must be (least, most)")
+    return lo, hi
+
+
+def _no_grad(name, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
+def chunk_selective_scan(
+    x: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None = None,
+    z: torch.Tensor | None = None,
+    dt_bias: torch.Tensor | None = None,
+    dt_softplus: bool = False,
+    dt_limit: tuple[float, float] = (0.0, _INF),
+    initial_state: torch.Tensor | None = None,
+    output_final_state: bool = False,
+    cu_seqlens: torch.LongTensor | None = None,
+    *,
+    state_dtype: torch.dtype = torch.float32,
+    force_generic: bool = False,
+    check_errors: bool = False,
+):
+    """Selective scan over prompts.
+
+    x, z ``[B, T, H, P]``; dt ``[B, T, H]``; B, C ``[B, T, G, S]`` (head h uses
+    group ``h // (H // G)``); A, D, dt_bias ``[H]``; initial_state
+    ``[N, H, P, S]`` of any float type; with ``cu_seqlens [N + 1]`` the batch
+    size is 1 and the tokens are N packed sequences.  Token rows may be strided
+    (views of one projection).  ``dt_limit`` clamps the steps after softplus.
+    Returns ``(y [B, T, H, P] in x's dtype, final_state [N, H, P, S] of
+    state_dtype or None)``.
+
+    bf16 with S of 64 or 128 and P a multiple of 64 runs on the tensor cores;
+    other types and sizes (P, S <= 256) on an fp32 recurrence.
+    ``check_errors=True`` synchronises and raises on a recorded device error.
+    Serving only: inputs that require grad are refused."""
+    _cuda("chunk_selective_scan", x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens)
+    _no_grad("chunk_selective_scan", x, dt, A, B, C, D, z, dt_bias, initial_state)
+    if x.dim() != 4:
+        raise ValueError(f"chunk_selective_scan: x {tuple(x.shape)} must be [B, T, H, P]")
+    lo, hi = _check("chunk_selective_scan", "B, T", x, dt, A, B, C, D, z, dt_bias, dt_limit)
+    if cu_seqlens is not None and x.shape[0] != 1:
+        raise ValueError("cu_seqlens requires batch size 1 (packed sequences)")
+    if state_dtype not in _DT:
+        raise ValueError(f"chunk_selective_scan: state_dtype {state_dtype} must be float32, bfloat16 or float16")
+    cu, _ = _idx(cu_seqlens)
+    if cu is not None:
+        cu = cu.contiguous()
+    N = x.shape[0] if cu is None else cu.shape[0] - 1
+    shape = (N, x.shape[2], x.shape[3], B.shape[3])
+    if initial_state is not None:
+        if tuple(initial_state.shape) != shape or initial_state.dtype not in _DT:
+            raise ValueError(f"initial_state must be {shape} of a float type, got {tuple(initial_state.shape)} "
+                             f"{initial_state.dtype}")
+        initial_state = initial_state.contiguous()
+    y, fin = _call(torch.ops.gdn_b200.scan_fwd, _scan_fwd_impl, x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias),
+                   bool(dt_softplus), lo, hi, initial_state, bool(output_final_state), state_dtype, cu,
+                   bool(force_generic), bool(check_errors))
+    return y, (fin if output_final_state else None)
+
+
+def selective_scan_update(
+    x: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None = None,
+    z: torch.Tensor | None = None,
+    dt_bias: torch.Tensor | None = None,
+    dt_softplus: bool = False,
+    dt_limit: tuple[float, float] = (0.0, _INF),
+    state: torch.Tensor | None = None,
+    ssm_state_indices: torch.Tensor | None = None,
+    *,
+    check_errors: bool = False,
+):
+    """One decode token per sequence, on a cache that is updated in place.
+
+    x, z ``[N, H, P]``; dt ``[N, H]``; B, C ``[N, G, S]``; A, D, dt_bias
+    ``[H]``; state ``[slots, H, P, S]`` of any float type (lines packed, the
+    distance between lines free); token i works on line
+    ``ssm_state_indices[i]`` (int32 / int64), or on line i without indices.  A
+    negative index is padding: output zero, no line touched; one past the
+    cache is treated the same and, with ``check_errors=True`` (synchronises),
+    raises :class:`GdnError`.  The indices of one call must differ.  Returns
+    ``(y [N, H, P], state)``."""
+    if state is None:
+        raise ValueError("selective_scan_update: state is required")
+    _cuda("selective_scan_update", x, dt, A, B, C, D, z, dt_bias, state, ssm_state_indices)
+    _no_grad("selective_scan_update", x, dt, A, B, C, D, z, dt_bias, state)
+    if x.dim() != 3:
+        raise ValueError(f"selective_scan_update: x {tuple(x.shape)} must be [N, H, P]")
+    lo, hi = _check("selective_scan_update", "N", x, dt, A, B, C, D, z, dt_bias, dt_limit)
+    N, H, P = x.shape
+    S = B.shape[2]
+    if state.dim() != 4 or tuple(state.shape[1:]) != (H, P, S) or state.dtype not in _DT:
+        raise ValueError(f"selective_scan_update: state {tuple(state.shape)} {state.dtype} must be [slots, {H}, {P}, {S}] "
+                         "of a float type")
+    want = 1
+    for n, st in zip(reversed(state.shape[1:]), reversed(state.stride()[1:])):
+        if n != 1 and st != want:
+            raise ValueError("selective_scan_update: a cache line [H, P, S] must be packed")
+        want *= n
+    if state.shape[0] > 1 and state.stride(0) < want:
+        raise ValueError("selective_scan_update: cache lines must not overlap")
+    idx = ssm_state_indices
+    if idx is None:
+        if state.shape[0] < N:
+            raise ValueError(f"selective_scan_update: {state.shape[0]} cache lines for {N} tokens")
+    else:
+        if tuple(idx.shape) != (N,):
+            raise ValueError(f"selective_scan_update: ssm_state_indices {tuple(idx.shape)} must be ({N},)")
+        idx = _idx(idx)[0].contiguous()
+    y = _call(torch.ops.gdn_b200.scan_update, _scan_update_impl, x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias),
+              bool(dt_softplus), lo, hi, state, idx, bool(check_errors))
+    return y, state

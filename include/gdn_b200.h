@@ -499,6 +499,159 @@ GDN_API int gdn_causal_conv1d_update(const gdn_conv1d_update_args* args, void* s
 GDN_API size_t gdn_conv_chunk_workspace_size(const gdn_chunk_args* args);
 GDN_API int gdn_conv_chunk_fwd(const gdn_chunk_args* args, const gdn_conv1d_fn_args* conv, void* stream);
 
+/* Gradient of causal_conv1d (gdn_causal_conv1d_fwd).
+ *   x, dy [B, T, D] of x_dtype with unit channel stride and token strides
+ *     stride_x_token, stride_dy_token (B*T rows); dx [B, T, D] contiguous;
+ *   weight [D, W], dweight [D, W], bias and dbias [D] (both or neither) of
+ *     w_dtype; initial_state, dinitial_state [N, D, W] of state_dtype (both
+ *     or neither; column 0 reaches no output, its gradient is 0);
+ *   the residual's gradient is dy.  dweight and dbias are fp32 sums in a
+ *   fixed order, rounded once. */
+typedef struct gdn_conv1d_bwd_args {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* initial_state;
+  const void* dy;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  void* dinitial_state;
+  const void* cu_seqlens;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, T, N, D;
+  int64_t stride_x_token, stride_dy_token;
+  int32_t W;
+  int32_t x_dtype, w_dtype, state_dtype, cu_dtype;
+  int32_t activation; /* GDN_ACT_* */
+} gdn_conv1d_bwd_args;
+GDN_API size_t gdn_causal_conv1d_bwd_workspace_size(const gdn_conv1d_bwd_args* args);
+GDN_API int gdn_causal_conv1d_bwd(const gdn_conv1d_bwd_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Gated RMS norm with residual sum (the norm behind the mixer, or before a
+ * block), and its gradient
+ * ------------------------------------------------------------------------ */
+#define GDN_GATE_SILU 0
+#define GDN_GATE_SIGMOID 1
+
+/* r = residual + residual_scale * x (r = x without a residual); u = r act(z)
+ * when gate_before, else r; y = u / sqrt(mean of u^2 over each group + eps)
+ * * weight (1 + weight when zero_centered), times act(z) when z is given and
+ * not gate_before.  rows = tokens * heads rows of D elements, in groups of
+ * `group` elements (group divides D).
+ *   x, z: row (t, h) at t * stride_*_token + h * stride_*_head; everything
+ *     else [rows, D] contiguous; weight, dweight [D] of w_dtype.
+ *   Forward: x, z, y of dtype; residual and sum (= r, stored) of res_dtype
+ *     (dtype or F32), both or neither.  sum == residual is allowed.
+ *   Backward: x is what was normed (the forward's sum, or its x) of x_dtype
+ *     (dtype or F32); dy, dz, dx of dtype; dsum (gradient of the sum, or
+ *     NULL) and dresidual (or NULL) of res_dtype; dx = residual_scale *
+ *     dresidual.  dweight is an fp32 sum in a fixed order, rounded once. */
+typedef struct gdn_norm_args {
+  const void* x;
+  const void* z;
+  const void* residual;
+  const void* weight;
+  void* y;
+  void* sum;
+  const void* dy;
+  const void* dsum;
+  void* dx;
+  void* dz;
+  void* dresidual;
+  void* dweight;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t rows, heads, D;
+  int64_t stride_x_token, stride_x_head, stride_z_token, stride_z_head;
+  int32_t group;
+  int32_t dtype, x_dtype, res_dtype, w_dtype;
+  int32_t gate_before, zero_centered, activation; /* GDN_GATE_* */
+  float eps, residual_scale;
+} gdn_norm_args;
+GDN_API int gdn_norm_fwd(const gdn_norm_args* args, void* stream);
+GDN_API size_t gdn_norm_bwd_workspace_size(const gdn_norm_args* args);
+GDN_API int gdn_norm_bwd(const gdn_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Selective state space scan with one decay per head
+ * ------------------------------------------------------------------------ */
+
+/* Prompts.  Per sequence and head, with dt = clamp(softplus(raw + dt_bias),
+ * dt_min, dt_max) (softplus when dt_softplus) and state h [P, S]:
+ *   h <- exp(dt A) h + dt x B^T;   y = (h C + D x) silu(z)
+ *   x, z (or NULL), y [B, T, H, P]; b, c [B, T, G, S] (head h uses group
+ *     h / (H / G)), all of dtype; dt [B, T, H] of dt_dtype.  Heads and groups
+ *     are packed within a token; stride_* is the distance of a token's row
+ *     to the next (B*T rows), so views of one projection are read in place;
+ *     y is contiguous.
+ *   A [H]; D, dt_bias [H] or NULL, all F32;
+ *   initial_state [N, H, P, S] of init_dtype or NULL (zeros); final_state
+ *     [N, H, P, S] of final_dtype or NULL;
+ *   cu_seqlens [N+1] (I32/I64): B == 1 and the T tokens are N packed
+ *     sequences (an empty one passes its state on); or NULL, N == B.
+ *   P, S <= 256.  bf16 with S of 64 or 128 and P a multiple of 64 runs on the
+ *   tensor cores (unless force_generic): bf16 products, states and sums in
+ *   fp32.  The first 16 bytes of the workspace are the device error word
+ *   (see gdn_chunk_check_device_error). */
+typedef struct gdn_scan_args {
+  const void* x;
+  const void* dt;
+  const float* A;
+  const void* b;
+  const void* c;
+  const float* D;
+  const void* z;
+  const float* dt_bias;
+  const void* initial_state;
+  void* y;
+  void* final_state;
+  const void* cu_seqlens;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, T, N;
+  int64_t stride_x, stride_dt, stride_b, stride_c, stride_z;
+  int32_t H, P, G, S;
+  int32_t dtype, dt_dtype, init_dtype, final_dtype, cu_dtype;
+  int32_t dt_softplus, force_generic;
+  float dt_min, dt_max;
+} gdn_scan_args;
+GDN_API size_t gdn_scan_workspace_size(const gdn_scan_args* args);
+GDN_API int gdn_scan_fwd(const gdn_scan_args* args, void* stream);
+
+/* One token per sequence on a cache of states, in place.
+ *   x, z (or NULL), y [N, H, P]; b, c [N, G, S] of dtype; dt [N, H] of
+ *     dt_dtype; row strides as above; y contiguous;
+ *   state: line l at l * stride_slot, [H, P, S] of state_dtype; token i works
+ *     on line ssm_state_indices[i] (or i without indices).  A negative index
+ *     is padding: its output is zero and no line is touched.  An index at or
+ *     past num_slots is treated the same and recorded in err (int32[4], zeroed
+ *     by the caller; may be NULL).  Indices of one call must differ.
+ *   S <= 256. */
+typedef struct gdn_scan_update_args {
+  const void* x;
+  const void* dt;
+  const float* A;
+  const void* b;
+  const void* c;
+  const float* D;
+  const void* z;
+  const float* dt_bias;
+  void* state;
+  void* y;
+  const void* ssm_state_indices;
+  int32_t* err;
+  int64_t N, num_slots, stride_slot;
+  int64_t stride_x, stride_dt, stride_b, stride_c, stride_z;
+  int32_t H, P, G, S;
+  int32_t dtype, dt_dtype, state_dtype, idx_dtype;
+  int32_t dt_softplus;
+  float dt_min, dt_max;
+} gdn_scan_update_args;
+GDN_API int gdn_scan_update(const gdn_scan_update_args* args, void* stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 GDN_API const char* gdn_last_error(void);
 

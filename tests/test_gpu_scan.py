@@ -1,0 +1,378 @@
+"""Selective scan (prompts and single tokens) against the recurrence in 64
+bits, token by token.
+
+Tolerances (relative RMS).  fp32 recurrence: a state is a sum over its memory
+(a few hundred tokens at most here) of fp32 products, 64 roundings of 2^-24
+allowed, plus the output type's rounding u.  Tensor-core path: y has two parts
+whose operands (scores, state) are rounded to bf16 once, plus the output's
+rounding: three roundings of u = 2^-8, each at most u per element and 0.6 u in
+RMS, so 2 u of the RMS of the parts; final states are sums of products with a
+three-way bf16 split of x (24 bits): 64 roundings of 2^-24 allowed."""
+
+import pytest
+import torch
+
+import domesticated_torch_mlu_ops_b200 as ops
+
+pytestmark = pytest.mark.gpu
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+F32 = 2.0 ** -24
+bf16, f16, f32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def steps(dt, bias, softplus, limit):
+    v = dt + (0 if bias is None else bias)
+    if softplus:
+        v = torch.nn.functional.softplus(v, threshold=1e9)
+    return v.clamp(*limit)
+
+
+def ref_token(h, x, dt, A, B, C, D, z):
+    """h [H, P, S]; x [H, P]; dt [H]; B, C [G, S]."""
+    r = x.shape[0] // B.shape[0]
+    Bh, Ch = B.repeat_interleave(r, 0), C.repeat_interleave(r, 0)
+    h = torch.exp(dt * A)[:, None, None] * h + (dt[:, None] * x)[..., None] * Bh[:, None, :]
+    y = torch.einsum("hps,hs->hp", h, Ch)
+    if D is not None:
+        y = y + D[:, None] * x
+    if z is not None:
+        y = y * z * torch.sigmoid(z)
+    return h, y
+
+
+def ref_scan(x, dt, A, B, C, D, z, bias, softplus, limit, h0, lens):
+    x, dt, A, B, C = (t.double() for t in (x, dt, A, B, C))
+    D, z, bias, h0 = (None if t is None else t.double() for t in (D, z, bias, h0))
+    dt = steps(dt, bias, softplus, limit)
+    ys, hs, at = [], [], 0
+    for n, length in enumerate(lens):
+        h = h0[n].clone() if h0 is not None else torch.zeros(x.shape[1], x.shape[2], B.shape[2], dtype=torch.float64)
+        for t in range(at, at + length):
+            h, y = ref_token(h, x[t], dt[t], A, B[t], C[t], D, None if z is None else z[t])
+            ys.append(y)
+        at += length
+        hs.append(h)
+    return torch.stack(ys) if ys else x, torch.stack(hs)
+
+
+def make(tokens, H, P, G, S, dtype, gate, seed=0, fast=False):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    xbc = r(tokens, H * P + 2 * G * S)
+    xbc[:, H * P:] *= 0.5
+    xbc = xbc.to(dtype)
+    zdt = r(tokens, H * P + H).to(dtype)
+    x, B, C = (xbc[:, :H * P].unflatten(-1, (H, P)), xbc[:, H * P:H * P + G * S].unflatten(-1, (G, S)),
+               xbc[:, H * P + G * S:].unflatten(-1, (G, S)))
+    A = -torch.exp(torch.rand(H, generator=g) * (6.0 if fast else 2.77))
+    bias = torch.rand(H, generator=g) * 4.6 - 6.9
+    return dict(x=x, dt=zdt[:, H * P:], A=A, B=B, C=C, D=1 + 0.1 * r(H), z=zdt[:, :H * P].unflatten(-1, (H, P)) if gate else None,
+                dt_bias=bias)
+
+
+def rel(got, want):
+    got, want = got.double().cpu(), want.double()
+    if want.numel() == 0:
+        return 0.0
+    return ((got - want).square().mean().sqrt() / want.square().mean().sqrt().clamp_min(1e-30)).item()
+
+
+def cuda(d):
+    """To the GPU with the views' strides kept (x, B, C, z, dt are views of two projections)."""
+    out = {}
+    for k, t in d.items():
+        if t is None or not t._is_view():
+            out[k] = None if t is None else t.cuda()
+        else:
+            base = t._base.cuda()
+            out[k] = base.as_strided(t.shape, t.stride(), t.storage_offset())
+    return out
+
+
+def run(i, lens, h0=None, final=True, sdtype=f32, **kw):
+    c = cuda(i)
+    lead = lambda t: None if t is None else t[None]  # noqa: E731
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32).cuda()
+    y, h = ops.chunk_selective_scan(
+        lead(c["x"]), lead(c["dt"]), c["A"], lead(c["B"]), lead(c["C"]), c["D"], lead(c["z"]), c["dt_bias"],
+        dt_softplus=True, initial_state=None if h0 is None else h0.cuda(), output_final_state=final, cu_seqlens=cu,
+        state_dtype=sdtype, check_errors=True, **kw)
+    return y[0], h
+
+
+def tolerances(dtype, tensor_cores):
+    return 2 * U[bf16] if tensor_cores else U[dtype] + 64 * F32
+
+
+SHAPES = [
+    # lens, H, P, G, S, dtype, gate, init, state dtype, tensor cores
+    ([1], 2, 64, 1, 128, bf16, True, False, f32, True),
+    ([7, 1, 0, 64, 65], 4, 64, 2, 128, bf16, True, True, f32, True),
+    ([127, 128, 129, 2], 4, 64, 1, 128, bf16, False, False, bf16, True),
+    ([300], 3, 64, 3, 128, bf16, True, True, f32, True),
+    ([130, 40], 2, 128, 1, 128, bf16, True, True, f32, True),
+    ([200, 33], 6, 64, 2, 64, bf16, False, True, f32, True),
+    ([256, 1], 2, 192, 2, 64, bf16, True, False, f16, True),
+    ([70, 3], 2, 64, 1, 128, f16, True, True, f32, False),
+    ([70, 0, 3], 3, 48, 1, 40, f32, True, True, f32, False),
+    ([33, 17], 4, 5, 2, 3, f32, False, False, f32, False),
+    ([50], 2, 80, 1, 16, bf16, True, True, bf16, False),
+    ([40, 20], 2, 256, 1, 256, f32, True, True, f32, False),
+    ([40, 20], 2, 130, 2, 129, bf16, False, True, f32, False),
+    ([16, 16], 5, 33, 5, 31, f16, True, False, f16, False),
+]
+
+
+@pytest.mark.parametrize("lens,H,P,G,S,dtype,gate,init,sdtype,tc", SHAPES)
+def test_prompt(lens, H, P, G, S, dtype, gate, init, sdtype, tc):
+    i = make(sum(lens), H, P, G, S, dtype, gate)
+    h0 = (torch.randn(len(lens), H, P, S, generator=torch.Generator().manual_seed(9)) * 0.3).to(sdtype) if init else None
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["dt_bias"], True, (0.0, float("inf")),
+                      h0, lens)
+    y, h = run(i, lens, h0, sdtype=sdtype)
+    assert y.dtype == dtype and h.dtype == sdtype and h.shape == rh.shape
+    assert rel(y, ry) <= tolerances(dtype, tc)
+    assert rel(h, rh) <= U[sdtype] + 64 * F32
+    # the recurrent kernel on the same call
+    y, h = run(i, lens, h0, sdtype=sdtype, force_generic=True)
+    assert rel(y, ry) <= U[dtype] + 64 * F32 and rel(h, rh) <= U[sdtype] + 64 * F32
+
+
+@pytest.mark.parametrize("dtype,P,S", [(bf16, 64, 128), (bf16, 64, 64), (f32, 24, 20)])
+def test_long_prompts_in_segments(dtype, P, S):
+    """Few heads and many tokens: the sequences are cut into segments."""
+    lens = [1500, 0, 700, 513, 1]
+    i = make(sum(lens), 2, P, 1, S, dtype, True, seed=1)
+    h0 = torch.randn(len(lens), 2, P, S, generator=torch.Generator().manual_seed(2)) * 0.3
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["dt_bias"], True, (0.0, float("inf")),
+                      h0, lens)
+    y, h = run(i, lens, h0)
+    assert rel(y, ry) <= tolerances(dtype, dtype == bf16)
+    assert rel(h, rh) <= 64 * F32
+    assert torch.equal(h[1].cpu(), h0[1])  # an empty sequence passes its state on
+    again, hh = run(i, lens, h0)
+    assert torch.equal(again, y) and torch.equal(hh, h)
+
+
+@pytest.mark.parametrize("dtype", [bf16, f32])
+def test_fast_decays(dtype):
+    """Log decays of several hundred within a chunk: no overflow, old tokens vanish."""
+    lens = [400, 90]
+    i = make(sum(lens), 4, 64, 1, 128, dtype, False, seed=3, fast=True)
+    i["dt_bias"] = i["dt_bias"] + 5.0
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], None, i["dt_bias"], True, (0.0, float("inf")),
+                      None, lens)
+    y, h = run(i, lens)
+    assert torch.isfinite(y.float()).all() and rel(y, ry) <= tolerances(dtype, dtype == bf16)
+    assert rel(h, rh) <= 64 * F32
+
+
+def test_no_decay_and_growth():
+    """A = 0 (sums) and A > 0 (growth) are ordinary values."""
+    lens = [150]
+    i = make(150, 2, 64, 1, 128, bf16, False, seed=4)
+    i["A"] = torch.tensor([0.0, 0.5])
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], None, i["dt_bias"], True, (0.0, float("inf")),
+                      None, lens)
+    y, h = run(i, lens)
+    assert rel(y, ry) <= tolerances(bf16, True) and rel(h, rh) <= 64 * F32
+
+
+@pytest.mark.parametrize("generic", [False, True])
+def test_equal_length_batch_without_options(generic):
+    """[B, T] without cu_seqlens, D, z, bias, softplus; dt in fp32; limits."""
+    Bt, T, H, P, G, S = 3, 100, 2, 64, 1, 128
+    i = make(Bt * T, H, P, G, S, bf16, False, seed=5)
+    dt = torch.rand(Bt * T, H, generator=torch.Generator().manual_seed(6)) * 0.2
+    ry, rh = ref_scan(i["x"], dt, i["A"], i["B"], i["C"], None, None, None, False, (0.01, 0.1), None, [T] * Bt)
+    c = cuda(i)
+    r = lambda t: t.unflatten(0, (Bt, T))  # noqa: E731
+    y, h = ops.chunk_selective_scan(r(c["x"]), r(dt.cuda()), c["A"], r(c["B"]), r(c["C"]), dt_limit=(0.01, 0.1),
+                                    output_final_state=True, force_generic=generic)
+    assert rel(y.flatten(0, 1), ry) <= tolerances(bf16, not generic) and rel(h, rh) <= 64 * F32
+    y2, none = ops.chunk_selective_scan(r(c["x"]), r(dt.cuda()), c["A"], r(c["B"]), r(c["C"]), dt_limit=(0.01, 0.1),
+                                        force_generic=generic)
+    assert none is None and torch.equal(y2, y)
+
+
+def test_layouts_give_the_same_values():
+    """Strided views, packed copies and misaligned rows of the same numbers."""
+    lens = [90, 140]
+    i = make(sum(lens), 2, 64, 1, 128, bf16, True, seed=7)
+    y, h = run(i, lens)
+    packed = {k: None if t is None else t.clone(memory_format=torch.contiguous_format) for k, t in i.items()}
+    y2, h2 = run(packed, lens)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+    odd = dict(packed)
+    base = torch.zeros(packed["x"].numel() + 1, dtype=bf16)
+    base[1:] = packed["x"].flatten()
+    odd["x"] = base[1:].view(packed["x"].shape)  # 2-byte aligned
+    y3, h3 = run(odd, lens)
+    assert torch.equal(y, y3) and torch.equal(h, h3)
+
+
+@pytest.mark.parametrize("generic", [False, True])
+def test_neighbours_stay_out(generic):
+    """NaN and infinity in one sequence reach no other, although tiles overlap them."""
+    lens = [70, 60, 70]
+    i = make(sum(lens), 2, 64, 1, 128, bf16, True, seed=8)
+    clean, hc = run(i, lens, force_generic=generic)
+    for k, v in (("x", float("nan")), ("B", float("inf")), ("C", float("nan")), ("z", float("nan")), ("dt", float("inf"))):
+        i[k][70:130] = v
+    y, h = run(i, lens, force_generic=generic)
+    keep = list(range(70)) + list(range(130, 200))
+    assert torch.equal(y[keep], clean[keep]) and torch.equal(h[[0, 2]], hc[[0, 2]])
+
+
+def test_other_stream():
+    lens = [600]
+    i = make(600, 2, 64, 1, 128, bf16, True, seed=10)
+    y, h = run(i, lens)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        y2, h2 = run(i, lens)
+    s.synchronize()
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
+def test_empty_batches():
+    e = lambda *s: torch.empty(*s, device="cuda", dtype=bf16)  # noqa: E731
+    A = -torch.ones(2, device="cuda")
+    h0 = torch.randn(3, 2, 64, 128, device="cuda")
+    y, h = ops.chunk_selective_scan(e(1, 0, 2, 64), e(1, 0, 2), A, e(1, 0, 1, 128), e(1, 0, 1, 128), initial_state=h0,
+                                    output_final_state=True, cu_seqlens=torch.zeros(4, dtype=torch.int64).cuda())
+    assert y.shape == (1, 0, 2, 64) and torch.equal(h, h0)
+    y, h = ops.chunk_selective_scan(e(0, 5, 2, 64), e(0, 5, 2), A, e(0, 5, 1, 128), e(0, 5, 1, 128), output_final_state=True)
+    assert y.shape == (0, 5, 2, 64) and h.shape == (0, 2, 64, 128)
+
+
+# ---- single tokens ---------------------------------------------------------
+UPDATES = [
+    # N, slots, H, P, G, S, dtype, cache dtype, gate
+    (1, 1, 1, 1, 1, 1, f32, f32, True),
+    (3, 5, 4, 64, 1, 128, bf16, f32, True),
+    (17, 40, 6, 80, 2, 64, bf16, bf16, True),
+    (5, 9, 3, 33, 1, 31, f32, f32, False),
+    (4, 4, 2, 64, 2, 256, f16, f32, True),
+    (4, 6, 2, 130, 1, 255, bf16, f16, False),
+    (2, 3, 2, 16, 1, 16, bf16, f32, True),
+    (2, 3, 2, 100, 1, 8, f16, f16, True),
+    (2, 3, 2, 7, 1, 100, f32, bf16, True),
+    (3, 3, 2, 65, 1, 32, f32, f32, True),
+]
+
+
+@pytest.mark.parametrize("N,slots,H,P,G,S,dtype,cdtype,gate", UPDATES)
+def test_update(N, slots, H, P, G, S, dtype, cdtype, gate):
+    i = make(N, H, P, G, S, dtype, gate, seed=11)
+    g = torch.Generator().manual_seed(12)
+    cache = (torch.randn(slots, H, P, S, generator=g) * 0.5).to(cdtype)
+    idx = torch.randperm(slots, generator=g)[:N]
+    dt = steps(i["dt"].double(), i["dt_bias"].double(), True, (0.0, float("inf")))
+    want_y, want_c = [], cache.double().clone()
+    for n in range(N):
+        h, y = ref_token(want_c[idx[n]], i["x"][n].double(), dt[n], i["A"].double(), i["B"][n].double(),
+                         i["C"][n].double(), i["D"].double(), None if i["z"] is None else i["z"][n].double())
+        want_c[idx[n]] = h
+        want_y.append(y)
+    c, dev = cuda(i), cache.cuda()
+    y, same = ops.selective_scan_update(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"],
+                                        dt_softplus=True, state=dev, ssm_state_indices=idx.to(torch.int32).cuda(),
+                                        check_errors=True)
+    assert same is dev and y.dtype == dtype
+    assert rel(y, torch.stack(want_y)) <= U[dtype] + 64 * F32  # of the state before it is rounded into the cache
+    assert rel(dev, want_c) <= U[cdtype] + 64 * F32
+    untouched = [s for s in range(slots) if s not in idx.tolist()]
+    assert torch.equal(dev[untouched].cpu(), cache[untouched])
+
+
+def test_update_padding_and_bad_index():
+    i = make(4, 2, 64, 1, 128, bf16, True, seed=13)
+    c = cuda(i)
+    cache = torch.randn(3, 2, 64, 128, device="cuda")
+    before = cache.clone()
+    args = (c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"])
+    y, _ = ops.selective_scan_update(*args, dt_softplus=True, state=cache, ssm_state_indices=torch.tensor([-1, 2, -1, 0]).cuda(),
+                                     check_errors=True)
+    assert torch.count_nonzero(y[[0, 2]]) == 0 and torch.count_nonzero(y[1]) > 0
+    assert torch.equal(cache[1], before[1]) and not torch.equal(cache[2], before[2])
+    cache = before.clone()
+    with pytest.raises(ops._lib.GdnError, match="slot"):
+        ops.selective_scan_update(*args, dt_softplus=True, state=cache, ssm_state_indices=torch.tensor([-1, -1, 3, -1]).cuda(),
+                                  check_errors=True)
+    assert torch.equal(cache, before)
+
+
+def test_update_strided_lines_and_no_index():
+    i = make(2, 2, 16, 1, 32, f32, False, seed=14)
+    c = cuda(i)
+    wide = torch.randn(2, 2, 2, 16, 32, device="cuda")
+    lines = wide[:, 1]
+    packed = lines.clone()
+    args = (c["x"], c["dt"], c["A"], c["B"], c["C"])
+    y, _ = ops.selective_scan_update(*args, state=lines, dt_softplus=True)
+    y2, _ = ops.selective_scan_update(*args, state=packed, dt_softplus=True)
+    assert torch.equal(y, y2) and torch.equal(lines, packed)
+
+
+def test_tokens_continue_a_prompt():
+    """A prompt of n tokens and one of n - 3 followed by three updates agree."""
+    i = make(200, 2, 64, 1, 128, bf16, True, seed=15)
+    y, h = run(i, [200])
+    head = {k: t[:197] if t is not None and t.dim() > 1 else t for k, t in i.items()}
+    _, state = run(head, [197])
+    c = cuda(i)
+    for t in range(197, 200):
+        yt, _ = ops.selective_scan_update(c["x"][t:t + 1], c["dt"][t:t + 1], c["A"], c["B"][t:t + 1], c["C"][t:t + 1], c["D"],
+                                          c["z"][t:t + 1], c["dt_bias"], dt_softplus=True, state=state)
+        assert rel(yt[0], y[t].double().cpu()) <= 3 * U[bf16]
+    assert rel(state, h.double().cpu()) <= 128 * F32
+
+
+def test_refusals():
+    i = cuda(make(8, 4, 64, 2, 128, bf16, True, seed=16))
+    u = {k: t if t is None or t.dim() == 1 else t[None] for k, t in i.items()}
+    good = [u[k] for k in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")]
+    call = lambda **kw: ops.chunk_selective_scan(*[kw.pop(k, u[k]) for k in  # noqa: E731
+                                                   ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")], **kw)
+    with pytest.raises(ValueError, match="CUDA"):
+        call(x=u["x"].cpu())
+    with pytest.raises(ValueError, match=r"\[B, T, H, P\]"):
+        call(x=u["x"][0])
+    with pytest.raises(ValueError, match="one value per head"):
+        call(A=torch.ones(4, 128, device="cuda"))
+    with pytest.raises(ValueError, match="multiple"):
+        call(B=u["B"][:, :, :1].expand(1, 8, 3, 128), C=u["C"][:, :, :1].expand(1, 8, 3, 128))
+    with pytest.raises(ValueError, match="share a dtype"):
+        call(B=u["B"].float())
+    with pytest.raises(ValueError, match="z "):
+        call(z=u["z"][:, :4])
+    with pytest.raises(ValueError, match="dt "):
+        call(dt=u["dt"][:, :4])
+    with pytest.raises(ValueError, match="dt_limit"):
+        call(dt_limit=(1.0, 0.5))
+    with pytest.raises(ValueError, match="initial_state"):
+        call(initial_state=torch.zeros(1, 4, 64, 64, device="cuda"))
+    with pytest.raises(ValueError, match="state_dtype"):
+        call(state_dtype=torch.float64)
+    with pytest.raises(ValueError, match="no backward"):
+        call(A=u["A"].clone().requires_grad_(True))
+    big = torch.zeros(1, 2, 1, 300, device="cuda")
+    with pytest.raises(ValueError, match="256"):
+        ops.chunk_selective_scan(big, big[..., 0], u["A"][:1], big, big)
+    del good
+    t = {k: v[0] if v.dim() > 1 else v for k, v in u.items()}
+    upd = lambda **kw: ops.selective_scan_update(*[kw.pop(k, t[k]) for k in  # noqa: E731
+                                                   ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")], **kw)
+    line = torch.zeros(9, 4, 64, 128, device="cuda")
+    with pytest.raises(ValueError, match="state is required"):
+        upd()
+    with pytest.raises(ValueError, match="state "):
+        upd(state=line[:, :3])
+    with pytest.raises(ValueError, match="packed"):
+        upd(state=line.transpose(2, 3).contiguous().transpose(2, 3))
+    with pytest.raises(ValueError, match="cache lines"):
+        upd(state=line[:3])
+    with pytest.raises(ValueError, match="ssm_state_indices"):
+        upd(state=line, ssm_state_indices=torch.zeros(3, dtype=torch.int64, device="cuda"))
