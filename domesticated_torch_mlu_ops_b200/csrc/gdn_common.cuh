@@ -99,7 +99,9 @@ enum ErrSite {
   kSiteStLoad = 4, kSiteStMma1 = 5, kSiteStMma2 = 6,       // tc_state3_kernel
   kSiteDecodeRelease = 7, kSiteDecodeLoad = 8,             // decode_stream_kernel waits
   kSiteSlotInitial = 9, kSiteSlotFinal = 10,               // state index >= num_slots
-  kSiteFzReady = 11                                        // tc_fused_kernel: stage-ready wait
+  kSiteFzReady = 11,                                       // tc_fused_kernel: stage-ready wait
+  kSiteScanLoad = 12, kSiteScanScores = 13,                // scan_tc_kernel waits
+  kSiteScanOut = 14, kSiteScanState = 15
 };
 
 __device__ __forceinline__ void record_device_error(int* err, int code, int site, int block, int info) {

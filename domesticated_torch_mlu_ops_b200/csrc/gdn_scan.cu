@@ -326,18 +326,18 @@ struct Plan {
   size_t state_off, decay_off, bytes;  // the error word comes first
 };
 
-// Segment length: as many (segment, head, row slice) CTAs as fill the GPU
-// a few times, but no segment under `least` tokens (below it the passes over
-// states cost more than the tokens).  Without a device query, so the result
-// depends on the shapes alone.
+// Segment length: enough (segment, head, row slice) CTAs to fill the GPU (two
+// per SM on the tensor cores, four of the recurrent kernel), but no segment
+// under `least` tokens (below it the passes over states cost more than the
+// tokens).  Without a device query, so the result depends on the shapes alone.
 Plan plan(const gdn_scan_args& a) {
   Plan pl{};
-  const bool tc = tc_applies(a);
+  const bool tc = tc_shape(a);
   const int64_t total = a.B * a.T;
   const int64_t slices = tc ? tc_slices(a) : (a.P + 63) / 64;
-  const int64_t want = 148 * 4, least = 512;
+  const int64_t want = 148 * (tc ? 2 : 4), least = 512;
   const int64_t per_token = std::max<int64_t>(1, a.H * slices);
-  int64_t pieces = std::max<int64_t>(1, (want + per_token - 1) / per_token);
+  const int64_t pieces = std::max<int64_t>(1, want / per_token);
   pl.seg = std::max(least, (total + pieces - 1) / pieces);
   pl.seg = (pl.seg + 127) / 128 * 128;
   pl.split = a.N > 0 && a.N * per_token < want && total > least;
@@ -454,10 +454,12 @@ extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
   p.dt_dtype = a->dt_dtype; p.init_dtype = a->init_dtype; p.final_dtype = a->final_dtype; p.cu_dtype = a->cu_dtype;
   p.softplus = a->dt_softplus; p.dt_lo = a->dt_min; p.dt_hi = a->dt_max;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == GDN_F32) launch_t<float>(p, pl, s);
+  cudaError_t e = cudaSuccess;
+  if (total > 0 && tc_shape(*a) && tc_layout(*a)) e = launch_tc(p, *a, s);
+  else if (a->dtype == GDN_F32) launch_t<float>(p, pl, s);
   else if (a->dtype == GDN_BF16) launch_t<__nv_bfloat16>(p, pl, s);
   else launch_t<__half>(p, pl, s);
-  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_last_error(GDN_ERR_CUDA, "gdn_scan_fwd: %s", cudaGetErrorString(e));
   return GDN_OK;
 }

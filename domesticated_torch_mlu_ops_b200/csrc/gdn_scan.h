@@ -9,8 +9,12 @@ namespace scan {
 
 struct ScanParams;
 
-inline bool tc_applies(const gdn_scan_args&) { return false; }
-inline int64_t tc_slices(const gdn_scan_args&) { return 1; }
+// Whether types and sizes suit the tensor-core kernels, and whether the
+// buffers' alignment does (the recurrent kernels run otherwise).
+bool tc_shape(const gdn_scan_args& a);
+bool tc_layout(const gdn_scan_args& a);
+int64_t tc_slices(const gdn_scan_args& a);
+cudaError_t launch_tc(const ScanParams& p, const gdn_scan_args& a, cudaStream_t s);
 // The states that segments start from, from those they add.
 void launch_pass(const ScanParams& p, cudaStream_t s);
 

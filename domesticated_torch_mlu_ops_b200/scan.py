@@ -50,6 +50,19 @@ def _packed_rows(t, tail):
     return t.contiguous(), width
 
 
+def _aligned_rows(t, tail):
+    """:func:`_packed_rows` whose rows start on 16 bytes (what the tensor-core
+    kernels read in place): other rows are copied, which costs far less than
+    the recurrent kernel."""
+    t, st = _packed_rows(t, tail)
+    if t.data_ptr() % 16 or st * t.element_size() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = 1
+        for n in t.shape[t.dim() - tail:]:
+            st *= n
+    return t, st
+
+
 def _scan_fwd_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor], z: Optional[Tensor],
                    dt_bias: Optional[Tensor], dt_softplus: bool, dt_min: float, dt_max: float,
                    initial_state: Optional[Tensor], output_final_state: bool, state_dtype: torch.dtype,
@@ -59,8 +72,9 @@ def _scan_fwd_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Op
     G, S = B.shape[2], B.shape[3]
     N = Bt if cu_seqlens is None else cu_seqlens.numel() - 1
     dev = x.device
-    (x, sx), (dt, sdt), (B, sb), (C, sc) = _packed_rows(x, 2), _packed_rows(dt, 1), _packed_rows(B, 2), _packed_rows(C, 2)
-    z, sz = (None, 0) if z is None else _packed_rows(z, 2)
+    rows = _aligned_rows if x.dtype == torch.bfloat16 else _packed_rows
+    (x, sx), (dt, sdt), (B, sb), (C, sc) = rows(x, 2), _packed_rows(dt, 1), rows(B, 2), rows(C, 2)
+    z, sz = (None, 0) if z is None else rows(z, 2)
     y = torch.empty((Bt, T, H, P), dtype=x.dtype, device=dev)
     fin = torch.empty((N, H, P, S) if output_final_state else (0,), dtype=state_dtype, device=dev)
     args = _lib.ScanArgs(
