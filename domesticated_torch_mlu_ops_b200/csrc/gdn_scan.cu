@@ -323,7 +323,7 @@ int check(const gdn_scan_args* a) {
 struct Plan {
   int64_t seg, segments;  // tokens per segment; at most so many segments
   bool split;
-  size_t state_off, decay_off, bytes;  // the error word comes first
+  size_t scratch_off, state_off, decay_off, bytes;  // the error word comes first
 };
 
 // Segment length: enough (segment, head, row slice) CTAs to fill the GPU (two
@@ -344,7 +344,8 @@ Plan plan(const gdn_scan_args& a) {
   if (!pl.split) pl.seg = std::max<int64_t>(128, (total + 127) / 128 * 128);
   // every sequence has at most ceil(len / seg) segments, and at least one
   pl.segments = pl.split ? total / pl.seg + a.N : a.N;
-  pl.state_off = pl.bytes = 256;
+  pl.scratch_off = 256;
+  pl.state_off = pl.bytes = 256 + (tc ? (tc_scratch_bytes(a) + 255) / 256 * 256 : 0);
   if (pl.split) {
     const size_t states = static_cast<size_t>(pl.segments) * a.H * a.P * a.S * sizeof(float);
     pl.decay_off = pl.state_off + (states + 255) / 256 * 256;
@@ -455,7 +456,7 @@ extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
   p.softplus = a->dt_softplus; p.dt_lo = a->dt_min; p.dt_hi = a->dt_max;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (total > 0 && tc_shape(*a) && tc_layout(*a)) e = launch_tc(p, *a, s);
+  if (total > 0 && tc_shape(*a) && tc_layout(*a)) e = launch_tc(p, *a, reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.scratch_off), s);
   else if (a->dtype == GDN_F32) launch_t<float>(p, pl, s);
   else if (a->dtype == GDN_BF16) launch_t<__nv_bfloat16>(p, pl, s);
   else launch_t<__half>(p, pl, s);

@@ -265,6 +265,13 @@ __device__ __forceinline__ void tma_load_2d(void* dst_smem, const void* tmap, in
       :: "r"(smem_u32(dst_smem)), "l"(tmap), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
 
+// 2-D tiled tensor store (bulk-group completion).  c0 * element size must be a
+// multiple of 16 bytes, no coordinate negative.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src_smem, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+               :: "l"(tmap), "r"(c0), "r"(c1), "r"(smem_u32(src_smem)) : "memory");
+}
+
 // 1-D bulk copy shared -> global (bulk-group completion).
 __device__ __forceinline__ void bulk_s2g(void* dst, const void* src_smem, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
