@@ -50,6 +50,9 @@ constexpr int kL = 128;             // tokens per chunk
 constexpr int kTile = kL * 128;     // 128 rows x 128 bytes (64 bf16 columns)
 constexpr int kTcThreads = 256;
 constexpr long long kWaitLimit = 2000000000LL;
+// The warp that issues copies and products: tokens 0-31 against 64-127, whose
+// part of P is all zeros, so it has the least to do while the scores run.
+constexpr int kLead = 4;
 
 struct PrepOut {
   float *a, *k, *dt;  // [H][tokens]
@@ -189,6 +192,10 @@ __device__ __forceinline__ float pick4(const float* v, int q) {
   return q < 2 ? (q == 0 ? v[0] : v[1]) : (q == 2 ? v[2] : v[3]);
 }
 
+// What k-step ks of 16 adds to an operand descriptor.
+__host__ __device__ constexpr uint64_t k_step(int ks) { return ((ks >> 2) * kTile + (ks & 3) * 32) >> 4; }
+__host__ __device__ constexpr uint64_t mn_step(int ks) { return (ks * 2048) >> 4; }
+
 // The swizzled tiles need a 1024-byte-aligned base; there is no static shared
 // memory to shift it.
 __device__ __forceinline__ bool base_ok(const ScanParams& p, uint32_t sbase) {
@@ -209,9 +216,11 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   const uint32_t sbase = umma::smem_u32(sm);
   const uint32_t bar_cb = umma::smem_u32(bars), bar_x = bar_cb + 8, bar_s = bar_cb + 16, bar_dh = bar_cb + 24,
                  bar_y = bar_cb + 32;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int quad = warp & 3, half = warp >> 2;  // TMEM lane quadrant; column half
   const int row = quad * 32 + lane;             // token of the chunk, or state column s
+  // the thread that issues every copy and product (elect.sync picks the same lane each time)
+  const bool leader = warp == kLead && umma::elect_one();
   if (!base_ok(p, sbase)) return;
   // Block = segment * units + unit: the CTAs that read the same B and C are
   // adjacent and run together, so those come from L2.
@@ -246,7 +255,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     umma::mbar_arrive_expect_tx(bar_x, kTile);
     umma::tma_load_2d(sm + M::kX, &tx, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_x);
   };
-  if (tid == 0) {
+  if (leader) {
 #pragma unroll
     for (int i = 0; i < 5; ++i) umma::mbar_init(bars + i, 1);
     umma::mbar_fence_init();
@@ -256,7 +265,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       fetch_x(0);
     }
   }
-  if (warp == 0) {
+  if (warp == kLead) {
     umma::tmem_alloc(tslot, M::kCols);
     umma::fence_before_sync();
   }
@@ -288,28 +297,29 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   constexpr uint32_t id_s = umma::idesc_f16(128, 128, true, false, false);
   constexpr uint32_t id_y = umma::idesc_f16(128, 64, true, false, true);
   constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
-  auto kmajor = [&](int off, int ks) {
-    return umma::smem_desc_sw128(sbase + off + (ks >> 2) * kTile + (ks & 3) * 32, 16, 1024);
-  };
-  auto mnmajor = [&](int off, int ks) { return umma::smem_desc_sw128(sbase + off + ks * 2048, kTile, 1024); };
+  // operand descriptors: x's and the parts' rows are tokens (K) with 64 columns
+  // (N), B is read both ways; a k-step of 16 advances 32 bytes within a
+  // K-major atom of 64 columns and 2048 bytes over MN-major rows
+  const uint64_t d_c = umma::smem_desc_sw128(sbase + M::kC, 16, 1024), d_bk = umma::smem_desc_sw128(sbase + M::kB, 16, 1024);
+  const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_x = umma::smem_desc_sw128(sbase + M::kX, kTile, 1024);
+  const uint64_t d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024), d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024);
 
   bool mine = true;
-  int commits_s = 0, commits_dh = 0, commits_y = 0, loads_cb = nch > 0, loads_x = nch > 0;  // so far (thread 0)
+  int commits_s = 0, commits_dh = 0, commits_y = 0, loads_cb = nch > 0, loads_x = nch > 0;  // so far (leader)
   auto wait = [&](uint32_t bar, uint32_t parity, int site) {
     // one answer per warp: what follows holds warp-wide instructions
-    const bool got = __all_sync(0xffffffffu, mine && umma::mbar_wait(bar, parity, kWaitLimit));
+    const bool got = __all_sync(0xffffffffu, mine && (umma::mbar_test(bar, parity) || umma::mbar_wait(bar, parity, kWaitLimit)));
     if (mine && !got) record_device_error(p.err, kErrWaitTimeout, site, static_cast<int>(blockIdx.x), tid);
     mine = got;
   };
   uint32_t par_dh = 0, tmem = 0, tl = 0;
   // dH (+)= B^T part.  With S = 64 rows 64-127 of the accumulator are the
   // product of the tile after B: never read.
-  auto mma_dh = [&](int part_off, bool first) {
+  auto mma_dh = [&](uint64_t d_part, bool first) {
 #pragma unroll
     for (int ks = 0; ks < kL / 16; ++ks)
-      umma::mma_f16(tmem + M::kDH, mnmajor(M::kB, ks), mnmajor(part_off, ks), id_h, !first || ks > 0);
+      umma::mma_f16(tmem + M::kDH, d_bm + mn_step(ks), d_part + mn_step(ks), id_h, !first || ks > 0);
   };
-  bool stored = false;  // (thread 0) a TMA store reads x's tile
   bool ok = true;
   for (int c = 0; c < nch; ++c) {
     const int64_t tc0 = t0 + static_cast<int64_t>(c) * kL;
@@ -323,22 +333,26 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     if (__syncthreads_or(!mine)) { ok = false; break; }
     umma::fence_after_sync();
     if (c == 0) {
-      tmem = *tslot;
+      tmem = __shfl_sync(0xffffffffu, *tslot, 0);
       tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     }
-    if (warp == 0) {
+    if (warp == kLead) {
+      if (c > 0 && umma::elect_one()) {  // y of the last chunk (a whole one) leaves from x's tile
+        umma::tma_store_2d(&ty, sm + M::kX, h * p.P + p0, static_cast<int>(tc0 - kL));
+        umma::bulk_commit();
+      }
       wait(bar_cb, c & 1, kSiteScanLoad);
-      if (tid == 0 && mine) {
+      if (mine && umma::elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < S_ / 16; ++ks) umma::mma_f16(tmem, kmajor(M::kC, ks), kmajor(M::kB, ks), id_s, ks > 0);
+        for (int ks = 0; ks < S_ / 16; ++ks) umma::mma_f16(tmem, d_c + k_step(ks), d_bk + k_step(ks), id_s, ks > 0);
         if (has_h)
 #pragma unroll
           for (int ks = 0; ks < S_ / 16; ++ks)
-            umma::mma_f16(tmem + M::kYi, kmajor(M::kC, ks), mnmajor(M::kH, ks), id_y, ks > 0);
+            umma::mma_f16(tmem + M::kYi, d_c + k_step(ks), d_h + mn_step(ks), id_y, ks > 0);
         umma::mma_commit(bar_s);
         ++commits_s;
         if (c > 0) {  // x goes where y was
-          if (stored) umma::bulk_wait_read_all();
+          umma::bulk_wait_read_all();
           fetch_x(c);
           ++loads_x;
         }
@@ -436,14 +450,14 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     umma::fence_before_sync();
     if (__syncthreads_or(!mine)) { ok = false; break; }
     umma::fence_after_sync();
-    if (tid == 0) {
+    if (warp == kLead && umma::elect_one()) {
 #pragma unroll
       for (int ks = 0; ks < kL / 16; ++ks)
-        umma::mma_f16(tmem + M::kYa, kmajor(M::kC, ks), mnmajor(M::kX, ks), id_y, ks > 0);
+        umma::mma_f16(tmem + M::kYa, d_c + k_step(ks), d_x + mn_step(ks), id_y, ks > 0);
       umma::mma_commit(bar_y);
       ++commits_y;
-      mma_dh(M::kXs, true);
-      mma_dh(M::kH, false);
+      mma_dh(d_xs, true);
+      mma_dh(d_h, false);
       umma::mma_commit(bar_dh);
       ++commits_dh;
     }
@@ -451,7 +465,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     // ---- outputs ----
     wait(bar_y, c & 1, kSiteScanOut);
     umma::fence_after_sync();
-    if (tid == 0 && mine && c + 1 < nch) {
+    if (leader && mine && c + 1 < nch) {
       fetch_c(c + 1);
       ++loads_cb;
     }
@@ -494,7 +508,6 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       }
     }
     // ---- state ----
-    if (len == kL) umma::fence_proxy_async();
     wait(bar_dh, par_dh, kSiteScanState);
     par_dh ^= 1;
     if (want_state) {  // the third part, in the first one's tile
@@ -504,8 +517,8 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       umma::fence_before_sync();
       if (__syncthreads_or(!mine)) { ok = false; break; }
       umma::fence_after_sync();
-      if (tid == 0) {
-        mma_dh(M::kXs, false);
+      if (warp == kLead && umma::elect_one()) {
+        mma_dh(d_xs, false);
         umma::mma_commit(bar_dh);
         ++commits_dh;
       }
@@ -514,7 +527,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       par_dh ^= 1;
     }
     umma::fence_after_sync();
-    if (tid == 0 && mine && c + 1 < nch) fetch_b(c + 1);
+    if (leader && mine && c + 1 < nch) fetch_b(c + 1);
     __syncwarp();
     const float decay = ex2(all);
     {
@@ -526,22 +539,25 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     }
     if (c + 1 < nch) store_h();
     has_h = true;
-    if (len == kL) {  // y leaves from x's tile once every thread has written its part
-      umma::named_sync(1, kTcThreads);
-      if (tid == 0) {
-        umma::tma_store_2d(&ty, sm + M::kX, h * p.P + p0, static_cast<int>(tc0));
+  }
+  if (nch > 0) {  // the last chunk's y
+    umma::fence_proxy_async();
+    umma::fence_before_sync();
+    if (ok) ok = !__syncthreads_or(!mine);
+    if (ok && leader) {
+      if (length(nch - 1) == kL) {
+        umma::tma_store_2d(&ty, sm + M::kX, h * p.P + p0, static_cast<int>(t1) - kL);
         umma::bulk_commit();
-        stored = true;
       }
-      __syncwarp();
     }
+    __syncwarp();
   }
   if (ok && row < S_ && want_state)
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       st_any(p.final_state, p.final_dtype, at_seq + static_cast<int64_t>(j) * S_, j & 1 ? hr[j / 2].y : hr[j / 2].x);
-  if (tid == 0 && stored) umma::bulk_wait_all();
-  if (!ok && tid == 0) {
+  if (leader) umma::bulk_wait_all();
+  if (!ok && leader) {
     // copies and products that this CTA issued may be in flight: wait
     // (bounded) for the last of each before memory is released
     const long long drain = 20000000LL;
@@ -554,7 +570,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  if (warp == 0) umma::tmem_dealloc(*tslot, M::kCols);
+  if (warp == kLead) umma::tmem_dealloc(*tslot, M::kCols);
 }
 
 template <int S_>
@@ -567,8 +583,10 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + M::kTmem);
   const uint32_t sbase = umma::smem_u32(sm);
   const uint32_t bar_ld = umma::smem_u32(bars), bar_dh = bar_ld + 8;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+  // the thread that issues every copy and product (elect.sync picks the same lane each time)
+  const bool leader = warp == 0 && umma::elect_one();
   if (!base_ok(p, sbase)) return;
   const int units = p.H * slices;
   const int64_t id = blockIdx.x / units;
@@ -586,7 +604,7 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     for (int q = 0; q < S_ / 64; ++q) umma::tma_load_2d(sm + M::kB + q * kTile, &tb, g * S_ + q * 64, t, bar_ld);
     umma::tma_load_2d(sm + M::kX, &tx, h * p.P + p0, t, bar_ld);
   };
-  if (tid == 0) {
+  if (leader) {
     umma::mbar_init(bars, 1);
     umma::mbar_init(bars + 1, 1);
     umma::mbar_fence_init();
@@ -598,13 +616,13 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   }
   __syncthreads();
   umma::fence_after_sync();
-  const uint32_t tmem = *tslot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tslot, 0);
   constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
-  auto mnmajor = [&](int off, int ks) { return umma::smem_desc_sw128(sbase + off + ks * 2048, kTile, 1024); };
+  const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
   bool ok = true, mine = true;
   int loads = 1, commits = 0;
   auto wait = [&](uint32_t bar, uint32_t parity, int site) {
-    const bool got = __all_sync(0xffffffffu, mine && umma::mbar_wait(bar, parity, kWaitLimit));
+    const bool got = __all_sync(0xffffffffu, mine && (umma::mbar_test(bar, parity) || umma::mbar_wait(bar, parity, kWaitLimit)));
     if (mine && !got) record_device_error(p.err, kErrWaitTimeout, site, static_cast<int>(blockIdx.x), tid);
     mine = got;
   };
@@ -630,19 +648,19 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     umma::fence_before_sync();
     if (__syncthreads_or(!mine)) { ok = false; break; }
     umma::fence_after_sync();
-    if (tid == 0) {
+    if (warp == 0 && umma::elect_one()) {
 #pragma unroll
       for (int part = 0; part < 3; ++part)
 #pragma unroll
         for (int ks = 0; ks < kL / 16; ++ks)
-          umma::mma_f16(tmem, mnmajor(M::kB, ks), mnmajor(M::kXs + part * kTile, ks), id_h, i > 0 || part > 0 || ks > 0);
+          umma::mma_f16(tmem, d_bm + mn_step(ks), d_xs + ((part * kTile) >> 4) + mn_step(ks), id_h, i > 0 || part > 0 || ks > 0);
       umma::mma_commit(bar_dh);
       ++commits;
     }
     __syncwarp();
     wait(bar_dh, i & 1, kSiteScanState);
     umma::fence_after_sync();
-    if (tid == 0 && mine && c > 0) {
+    if (leader && mine && c > 0) {
       fetch(c - 1);
       ++loads;
     }
@@ -659,7 +677,7 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     }
     if (tid == 0 && p0 == 0) p.seg_decay[id * p.H + h] = later * 0.6931471805599453f;
   }
-  if (!ok && tid == 0) {
+  if (!ok && leader) {
     const long long drain = 20000000LL;
     umma::mbar_wait(bar_ld, (loads - 1) & 1, drain);
     if (commits) umma::mbar_wait(bar_dh, (commits - 1) & 1, drain);
