@@ -326,7 +326,7 @@ struct Plan {
   size_t scratch_off, state_off, decay_off, bytes;  // the error word comes first
 };
 
-// Segment length: enough (segment, head, row slice) CTAs to fill the GPU (two
+// Segment length: enough (segment, head, row slice) CTAs to fill the GPU (one
 // per SM on the tensor cores, four of the recurrent kernel), but no segment
 // under `least` tokens (below it the passes over states cost more than the
 // tokens).  Without a device query, so the result depends on the shapes alone.
@@ -335,7 +335,7 @@ Plan plan(const gdn_scan_args& a) {
   const bool tc = tc_shape(a);
   const int64_t total = a.B * a.T;
   const int64_t slices = tc ? tc_slices(a) : (a.P + 63) / 64;
-  const int64_t want = 148 * (tc ? 2 : 4), least = 512;
+  const int64_t want = 148 * (tc ? 1 : 4), least = 512;
   const int64_t per_token = std::max<int64_t>(1, a.H * slices);
   const int64_t pieces = std::max<int64_t>(1, want / per_token);
   pl.seg = std::max(least, (total + pieces - 1) / pieces);

@@ -6,24 +6,25 @@
 // 32 (scan_prep_kernel).
 //
 // scan_tc_kernel: one CTA per (segment of a sequence, head, 64 columns of P),
-// two CTAs per SM.  It walks the segment in chunks of 128 tokens:
+// one per SM: sixteen warps that share the elementwise work and one that
+// issues copies and products.  It walks the segment in chunks of 128 tokens:
 //   S  = C B^T                                   [128, 128]
 //   Yi = C h                                     [128, 64], h as bf16
 //   P_ij = S_ij exp(a_i - a_j) dt'_j  (j <= i)   rounded to bf16 once
 //   Ya = P x;   y = exp(a_i) Yi + Ya + D x       in fp32, then the gate
 //   dH = B^T (w x),  w_j = exp(a_end - a_j) dt'_j
 //   h <- exp(a_end) h + dH                       fp32, in registers
-// Four products with fp32 accumulators in TMEM (S and Ya share columns); x, B
-// and C come by TMA into 128-byte-swizzled tiles that serve as operands in
-// both directions, P replaces C's tile, the second part of w x h's, and y x's
-// (from where a TMA store takes it).  The tiles fill half an SM's shared
-// memory to the last kilobyte, so there is no second stage; the other CTA
-// works while this one waits.
+// Four products with fp32 accumulators in TMEM; x, B and C come by TMA, a
+// chunk ahead, into 128-byte-swizzled tiles that serve as operands in both
+// directions, y takes x's place (from where a TMA store moves it), the second
+// and third part of w x those of C and h once Yi has read them.  A chunk's
+// chain is P and w x from the scores (which run behind the previous chunk's
+// products), Ya and dH, and the new h.
 //
 // scan_tc_state_kernel, the first pass over split sequences: dH of a whole
 // segment in one accumulator, chunks from the last to the first, each
 // weighted by the decay to the segment's end.
-//
+
 // Rounding.  x, B and C are bf16 already.  P and h are rounded to bf16 as
 // operands, as y is rounded to bf16 in the end.  w x is split into bf16 parts
 // whose products are summed: two parts (16 bits) where the state only feeds
@@ -48,11 +49,10 @@ namespace scan {
 
 constexpr int kL = 128;             // tokens per chunk
 constexpr int kTile = kL * 128;     // 128 rows x 128 bytes (64 bf16 columns)
-constexpr int kTcThreads = 256;
+constexpr int kWork = 512;                // threads of the sixteen working warps
+constexpr int kTcThreads = kWork + 32;    // and the issuing warp
+constexpr int kLead = kWork / 32;
 constexpr long long kWaitLimit = 2000000000LL;
-// The warp that issues copies and products: tokens 0-31 against 64-127, whose
-// part of P is all zeros, so it has the least to do while the scores run.
-constexpr int kLead = 4;
 
 struct PrepOut {
   float *a, *k, *dt;  // [H][tokens]
@@ -60,42 +60,43 @@ struct PrepOut {
 
 template <int S_>
 struct Smem {
-  static constexpr int kB = 0;
-  static constexpr int kX = kB + S_ / 64 * kTile;  // x, then y
-  static constexpr int kXs = kX + kTile;           // first part of w x (with a third: that, later)
-  static constexpr int kH = kXs + kTile;           // h, then the second part of w x
-  static constexpr int kC = kH + kTile;            // C, then P
-  static constexpr int kCf = kC + 2 * kTile;       // k of the chunk's tokens
-  static constexpr int kBar = kCf + kL * 4;        // C and B, x, S and Yi, dH, Ya
-  static constexpr int kTmem = kBar + 5 * 8;
+  // two stages of operands
+  static constexpr int kC = 0;                              // C, then the second part of w x
+  static constexpr int kB = S_ / 64 * kTile;
+  static constexpr int kX = 2 * kB;                         // x, then y
+  static constexpr int kStage = kX + kTile;
+  static constexpr int kXs = 2 * kStage;                    // first part of w x
+  static constexpr int kH = kXs + kTile;                    // h, then the third part of w x
+  static constexpr int kP = kH + kTile;
+  static constexpr int kCf = kP + 2 * kTile;                // k of one block of 32 tokens per warp
+  static constexpr int kBar = kCf + kWork / 32 * 32 * 4;    // loads[2], S, Yi, Ya, dH, h ready, P and w x ready
+  static constexpr int kBars = 8;
+  static constexpr int kTmem = kBar + kBars * 8;
   static constexpr int kBytes = kTmem + 8;
-  static constexpr int kCols = 256, kYa = 0, kYi = 128, kDH = 192;  // TMEM columns: S (then Ya), Yi, dH
-  // two CTAs per SM: 228 KB less 1 KB per CTA
-  static_assert(kBytes <= (228 * 1024 - 2 * 1024) / 2, "shared memory");
+  static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile;
+  static constexpr int kCols = 512, kYi = 256, kYa = 320, kDH = 384;  // TMEM columns: S[2] first
+  static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
-// First pass: B, x, three parts of w x.
+// First pass: two stages of B and x and, beside each, three parts of w x.
 template <int S_>
 struct StateSmem {
   static constexpr int kB = 0;
-  static constexpr int kX = kB + S_ / 64 * kTile;
+  static constexpr int kX = S_ / 64 * kTile;
   static constexpr int kXs = kX + kTile;
-  static constexpr int kBar = kXs + 3 * kTile;  // loads, dH
-  static constexpr int kTmem = kBar + 2 * 8;
+  static constexpr int kStage = kXs + 3 * kTile;
+  static constexpr int kBar = 2 * kStage;  // loads[2], parts ready[2], products[2]
+  static constexpr int kTmem = kBar + 6 * 8;
   static constexpr int kBytes = kTmem + 8;
   static constexpr int kCols = 64;
   static constexpr uint32_t kTx = (S_ / 64 + 1) * kTile;
+  static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// 16-byte piece q (of 8) of row r of a swizzled tile.
-__device__ __forceinline__ uint4* tile16(uint8_t* tile, int r, int q) {
-  return reinterpret_cast<uint4*>(tile + r * 128 + ((q ^ (r & 7)) << 4));
 }
 
 __device__ __forceinline__ void unpack8(uint4 u, float2* v) {
@@ -175,21 +176,67 @@ __global__ void __launch_bounds__(256) scan_prep_kernel(const ScanParams p, cons
   }
 }
 
+// Loads that stay where they are written, a chunk ahead of their use: the
+// compiler otherwise moves plain ones down to it and the full latency shows
+// (measured: 1-2 K cycles per chunk).
+__device__ __forceinline__ float ld_now(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_now16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // What a thread (token `row` of a chunk) needs of a and k.
 struct TokenScalars {
-  float a, k;       // its own (0 past the end)
-  float end[4];     // a at the end of each block of 32 (of the chunk, past its end)
+  float a, k;    // its own (0 past the end)
+  float end[4];  // a at the end of each block of 32 (of the chunk, past its end)
 };
-__device__ __forceinline__ TokenScalars load_scalars(const PrepOut& o, int64_t base, int64_t t, int len, int row) {
+__device__ __forceinline__ TokenScalars load_scalars(const PrepOut& o, int64_t at, int len, int row) {
   TokenScalars s;
-  s.a = row < len ? __ldg(o.a + base + t + row) : 0.f;
-  s.k = row < len ? __ldg(o.k + base + t + row) : 0.f;
+  const float *a = o.a + at, *k = o.k + at;
+  s.a = s.k = 0.f;
+  if (row < len) {
+    s.a = ld_now(a + row);
+    s.k = ld_now(k + row);
+  }
 #pragma unroll
-  for (int b = 0; b < 4; ++b) s.end[b] = __ldg(o.a + base + t + min(b * 32 + 31, len - 1));
+  for (int b = 0; b < 4; ++b) s.end[b] = ld_now(a + min(b * 32 + 31, len - 1));
   return s;
 }
 __device__ __forceinline__ float pick4(const float* v, int q) {
   return q < 2 ? (q == 0 ? v[0] : v[1]) : (q == 2 ? v[2] : v[3]);
+}
+
+// Byte offsets of a thread's two 16-byte pieces (columns 16 cq .. 16 cq + 15
+// of 64) in row `row` of a swizzled tile.
+struct Pieces {
+  uint32_t at[2];
+  __device__ __forceinline__ Pieces(int row, int cq) {
+    at[0] = row * 128 + (((cq * 2) ^ (row & 7)) << 4);
+    at[1] = at[0] ^ 16;
+  }
+};
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// All of this warp's writes to shared memory, for the products: then one
+// arrival per warp.
+__device__ __forceinline__ void publish(uint32_t bar) {
+  umma::fence_proxy_async();
+  umma::fence_before_sync();
+  __syncwarp();
+  if (umma::elect_one()) umma::mbar_arrive(bar);
+  __syncwarp();
 }
 
 // What k-step ks of 16 adds to an operand descriptor.
@@ -205,7 +252,7 @@ __device__ __forceinline__ bool base_ok(const ScanParams& p, uint32_t sbase) {
 }
 
 template <int S_>
-__global__ void __launch_bounds__(kTcThreads, 2)
+__global__ void __launch_bounds__(kTcThreads, 1)
 scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const __grid_constant__ CUtensorMap tx,
                const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tcm,
                const __grid_constant__ CUtensorMap ty) {
@@ -214,13 +261,9 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::kBar);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + M::kTmem);
   const uint32_t sbase = umma::smem_u32(sm);
-  const uint32_t bar_cb = umma::smem_u32(bars), bar_x = bar_cb + 8, bar_s = bar_cb + 16, bar_dh = bar_cb + 24,
-                 bar_y = bar_cb + 32;
+  const uint32_t bar_ld = umma::smem_u32(bars), bar_s = bar_ld + 16, bar_yi = bar_ld + 24, bar_y = bar_ld + 32,
+                 bar_dh = bar_ld + 40, bar_h = bar_ld + 48, bar_px = bar_ld + 56;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int quad = warp & 3, half = warp >> 2;  // TMEM lane quadrant; column half
-  const int row = quad * 32 + lane;             // token of the chunk, or state column s
-  // the thread that issues every copy and product (elect.sync picks the same lane each time)
-  const bool leader = warp == kLead && umma::elect_one();
   if (!base_ok(p, sbase)) return;
   // Block = segment * units + unit: the CTAs that read the same B and C are
   // adjacent and run together, so those come from L2.
@@ -233,52 +276,174 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   if (!find_segment(p, id, n, ls, t0, t1, last)) return;  // every warp finds the same
   const int nch = static_cast<int>((t1 - t0 + kL - 1) / kL);
   const bool want_state = last && p.final_state;
-  const int64_t at_seq = ((n * p.H + h) * p.P + p0 + half * 32) * S_ + row;
-  const int64_t at_seg = ((id * p.H + h) * p.P + p0 + half * 32) * S_ + row;
-  const float D = p.D ? p.D[h] : 0.f;
-  const int64_t prow = static_cast<int64_t>(h) * p.total;
+  // an all-zero state needs no product
+  const bool seg = p.seg_state != nullptr, ini = !seg && p.init;
   auto length = [&](int c) { return static_cast<int>(min64(kL, t1 - t0 - static_cast<int64_t>(c) * kL)); };
 
-  // operands of chunk c (one thread)
-  auto fetch_c = [&](int c) {
-    umma::mbar_arrive_expect_tx(bar_cb, 2 * (S_ / 64) * kTile);
-#pragma unroll
-    for (int q = 0; q < S_ / 64; ++q)
-      umma::tma_load_2d(sm + M::kC + q * kTile, &tcm, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar_cb);
-  };
-  auto fetch_b = [&](int c) {
-#pragma unroll
-    for (int q = 0; q < S_ / 64; ++q)
-      umma::tma_load_2d(sm + M::kB + q * kTile, &tb, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar_cb);
-  };
-  auto fetch_x = [&](int c) {
-    umma::mbar_arrive_expect_tx(bar_x, kTile);
-    umma::tma_load_2d(sm + M::kX, &tx, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_x);
-  };
-  if (leader) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) umma::mbar_init(bars + i, 1);
-    umma::mbar_fence_init();
-    if (nch > 0) {
-      fetch_c(0);
-      fetch_b(0);
-      fetch_x(0);
-    }
-  }
   if (warp == kLead) {
+    if (umma::elect_one()) {
+#pragma unroll
+      for (int i = 0; i < M::kBars; ++i) umma::mbar_init(bars + i, i < 6 ? 1 : kLead);
+      umma::mbar_fence_init();
+    }
+    __syncwarp();
     umma::tmem_alloc(tslot, M::kCols);
     umma::fence_before_sync();
   }
-  TokenScalars sc;
-  if (nch > 0) sc = load_scalars(prep, prow, t0, length(0), row);
-  // h[s = row][32 columns of P]
-  float2 hr[16];
-  bool has_h;  // block-uniform: an all-zero state needs no product
-  {
-    const bool seg = p.seg_state != nullptr, ini = !seg && p.init;
-    has_h = seg || ini;
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tslot, 0);
+
+  bool mine = true;
+  auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+    // one answer per warp: what follows holds warp-wide instructions
+    const bool got = __all_sync(0xffffffffu, mine && (umma::mbar_test(bar, parity) || umma::mbar_wait(bar, parity, kWaitLimit)));
+    if (mine && !got) record_device_error(p.err, kErrWaitTimeout, site, static_cast<int>(blockIdx.x), tid);
+    mine = got;
+    return got;
+  };
+
+  if (warp == kLead) {
+    // ---- copies and products ----
+    constexpr uint32_t id_s = umma::idesc_f16(128, 128, true, false, false);
+    constexpr uint32_t id_y = umma::idesc_f16(128, 64, true, false, true);
+    constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
+    // operand descriptors: rows of x and of the parts are tokens (K) with 64
+    // columns (N), B is read both ways; a k-step of 16 advances 32 bytes
+    // within a K-major atom of 64 columns and 2048 bytes over MN-major rows
+    const uint64_t d_c = umma::smem_desc_sw128(sbase + M::kC, 16, 1024), d_bk = umma::smem_desc_sw128(sbase + M::kB, 16, 1024);
+    const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_x = umma::smem_desc_sw128(sbase + M::kX, kTile, 1024);
+    const uint64_t d_cm = umma::smem_desc_sw128(sbase + M::kC, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
+    const uint64_t d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024), d_p = umma::smem_desc_sw128(sbase + M::kP, 16, 1024);
+    auto fetch_cb = [&](int c) {
+      const uint32_t bar = bar_ld + (c & 1) * 8;
+      uint8_t* st = sm + (c & 1) * M::kStage;
+      umma::mbar_arrive_expect_tx(bar, M::kTx);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+      for (int q = 0; q < S_ / 64; ++q) {
+        umma::tma_load_2d(st + M::kC + q * kTile, &tcm, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
+        umma::tma_load_2d(st + M::kB + q * kTile, &tb, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
+      }
+    };
+    auto fetch_x = [&](int c) {
+      umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kX, &tx, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_ld + (c & 1) * 8);
+    };
+    auto store_y = [&](int c) {
+      umma::tma_store_2d(&ty, sm + (c & 1) * M::kStage + M::kX, h * p.P + p0, static_cast<int>(t0) + c * kL);
+      umma::bulk_commit();
+    };
+    auto scores = [&](int c) {
+      const uint64_t st = (c & 1) * (M::kStage >> 4);
+#pragma unroll
+      for (int ks = 0; ks < S_ / 16; ++ks)
+        umma::mma_f16(tmem + (c & 1) * 128, d_c + st + k_step(ks), d_bk + st + k_step(ks), id_s, ks > 0);
+      umma::mma_commit(bar_s);
+    };
+    int loads = 0, n_s = 0, n_yi = 0, n_y = 0, n_dh = 0;  // issued so far
+    if (nch > 0) {
+      if (umma::elect_one()) {
+        fetch_cb(0);
+        fetch_x(0);
+      }
+      __syncwarp();
+      loads = 1;
+      if (wait(bar_ld, 0, kSiteScanLoad)) {
+        if (umma::elect_one()) scores(0);
+        __syncwarp();
+        n_s = 1;
+      }
+    }
+    for (int c = 0; c < nch && mine; ++c) {
+      // h of this chunk is in place, and all work on the chunk before is done
+      if (!wait(bar_h, c & 1, kSiteScanState)) break;
+      umma::fence_after_sync();
+      if (umma::elect_one()) {
+        const uint64_t st = (c & 1) * (M::kStage >> 4);
+        if (c > 0 || seg || ini)
+#pragma unroll
+          for (int ks = 0; ks < S_ / 16; ++ks)
+            umma::mma_f16(tmem + M::kYi, d_c + st + k_step(ks), d_h + mn_step(ks), id_y, ks > 0);
+        umma::mma_commit(bar_yi);
+        if (c > 0) store_y(c - 1);  // a whole chunk
+        if (c + 1 < nch) {
+          fetch_cb(c + 1);
+          umma::bulk_wait_read_all();  // x goes where that y was
+          fetch_x(c + 1);
+        }
+      }
+      __syncwarp();
+      ++n_yi;
+      loads += c + 1 < nch;
+      if (!wait(bar_px, c & 1, kSiteScanScores)) break;
+      umma::fence_after_sync();
+      if (umma::elect_one()) {
+        const uint64_t st = (c & 1) * (M::kStage >> 4);
+#pragma unroll
+        for (int ks = 0; ks < kL / 16; ++ks)
+          umma::mma_f16(tmem + M::kYa, d_p + k_step(ks), d_x + st + mn_step(ks), id_y, ks > 0);
+        umma::mma_commit(bar_y);
+        // With S = 64 rows 64-127 of the accumulator are the product of the
+        // tile after B: never read.
+#pragma unroll
+        for (int ks = 0; ks < kL / 16; ++ks)
+          umma::mma_f16(tmem + M::kDH, d_bm + st + mn_step(ks), d_xs + mn_step(ks), id_h, ks > 0);
+#pragma unroll
+        for (int ks = 0; ks < kL / 16; ++ks)
+          umma::mma_f16(tmem + M::kDH, d_bm + st + mn_step(ks), d_cm + st + mn_step(ks), id_h, 1);
+        if (want_state)
+#pragma unroll
+          for (int ks = 0; ks < kL / 16; ++ks)
+            umma::mma_f16(tmem + M::kDH, d_bm + st + mn_step(ks), d_h + mn_step(ks), id_h, 1);
+        umma::mma_commit(bar_dh);
+      }
+      __syncwarp();
+      ++n_y;
+      ++n_dh;
+      if (c + 1 < nch) {
+        if (!wait(bar_ld + ((c + 1) & 1) * 8, ((c + 1) >> 1) & 1, kSiteScanLoad)) break;
+        if (umma::elect_one()) scores(c + 1);
+        __syncwarp();
+        ++n_s;
+      }
+    }
+    if (mine && nch > 0 && wait(bar_h, nch & 1, kSiteScanState)) {  // the last chunk's y
+      if (umma::elect_one() && length(nch - 1) == kL) store_y(nch - 1);
+    }
+    __syncwarp();
+    if (umma::elect_one()) umma::bulk_wait_all();
+    __syncwarp();
+    if (!mine) {
+      // copies and products that were issued may be in flight: wait (bounded)
+      // for the last of each before memory is released
+      const long long drain = 20000000LL;
+      if (loads > 1) umma::mbar_wait(bar_ld + (loads & 1) * 8, ((loads - 2) >> 1) & 1, drain);
+      if (loads > 0) umma::mbar_wait(bar_ld + ((loads - 1) & 1) * 8, ((loads - 1) >> 1) & 1, drain);
+      if (n_s) umma::mbar_wait(bar_s, (n_s - 1) & 1, drain);
+      if (n_yi) umma::mbar_wait(bar_yi, (n_yi - 1) & 1, drain);
+      if (n_y) umma::mbar_wait(bar_y, (n_y - 1) & 1, drain);
+      if (n_dh) umma::mbar_wait(bar_dh, (n_dh - 1) & 1, drain);
+    }
+  } else {
+    // ---- everything between the products ----
+    const int quad = warp & 3, cq = warp >> 2;  // TMEM lane quadrant; quarter of the columns
+    const int row = quad * 32 + lane;           // token of the chunk, or state column s
+    const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const Pieces piece(row, cq);
+    const uint32_t cf = sbase + M::kCf + warp * 128;
+    const int64_t prow = static_cast<int64_t>(h) * p.total + t0;
+    const int64_t col = static_cast<int64_t>(h) * p.P + p0 + cq * 16;
+    const int64_t at_seq = ((n * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
+    const int64_t at_seg = ((id * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
+    const float D = p.D ? p.D[h] : 0.f;
+    TokenScalars sc;
+    float kj = 0.f;  // k of token 32 cq + lane
+    if (nch > 0) {
+      sc = load_scalars(prep, prow, length(0), row);
+      if (cq * 32 + lane < length(0)) kj = ld_now(prep.k + prow + cq * 32 + lane);
+    }
+    float2 hr[8];  // h[s = row][16 columns of P]
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
       float v = 0.f;
       if (row < S_) {
         if (seg) v = p.seg_state[at_seg + static_cast<int64_t>(j) * S_];
@@ -287,209 +452,134 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       if (j & 1) hr[j / 2].y = v;
       else hr[j / 2].x = v;
     }
-  }
-  auto store_h = [&]() {
-    if (row < S_)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) *tile16(sm + M::kH, row, half * 4 + q) = pack8(hr + q * 4);
-  };
-  if (has_h) store_h();
-  constexpr uint32_t id_s = umma::idesc_f16(128, 128, true, false, false);
-  constexpr uint32_t id_y = umma::idesc_f16(128, 64, true, false, true);
-  constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
-  // operand descriptors: x's and the parts' rows are tokens (K) with 64 columns
-  // (N), B is read both ways; a k-step of 16 advances 32 bytes within a
-  // K-major atom of 64 columns and 2048 bytes over MN-major rows
-  const uint64_t d_c = umma::smem_desc_sw128(sbase + M::kC, 16, 1024), d_bk = umma::smem_desc_sw128(sbase + M::kB, 16, 1024);
-  const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_x = umma::smem_desc_sw128(sbase + M::kX, kTile, 1024);
-  const uint64_t d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024), d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024);
-
-  bool mine = true;
-  int commits_s = 0, commits_dh = 0, commits_y = 0, loads_cb = nch > 0, loads_x = nch > 0;  // so far (leader)
-  auto wait = [&](uint32_t bar, uint32_t parity, int site) {
-    // one answer per warp: what follows holds warp-wide instructions
-    const bool got = __all_sync(0xffffffffu, mine && (umma::mbar_test(bar, parity) || umma::mbar_wait(bar, parity, kWaitLimit)));
-    if (mine && !got) record_device_error(p.err, kErrWaitTimeout, site, static_cast<int>(blockIdx.x), tid);
-    mine = got;
-  };
-  uint32_t par_dh = 0, tmem = 0, tl = 0;
-  // dH (+)= B^T part.  With S = 64 rows 64-127 of the accumulator are the
-  // product of the tile after B: never read.
-  auto mma_dh = [&](uint64_t d_part, bool first) {
-#pragma unroll
-    for (int ks = 0; ks < kL / 16; ++ks)
-      umma::mma_f16(tmem + M::kDH, d_bm + mn_step(ks), d_part + mn_step(ks), id_h, !first || ks > 0);
-  };
-  bool ok = true;
-  for (int c = 0; c < nch; ++c) {
-    const int64_t tc0 = t0 + static_cast<int64_t>(c) * kL;
-    const int len = length(c);
-    if (half == 0) reinterpret_cast<float*>(sm + M::kCf)[row] = sc.k;
-    const float ai = sc.a, all = sc.end[3], own_end = pick4(sc.end, quad);
-    const float wj = sc.k * ex2(all - own_end);
-    // ---- S = C B^T, Yi = C h ----
-    umma::fence_proxy_async();  // h's tile, and the reads of the tiles that are loaded next
-    umma::fence_before_sync();
-    if (__syncthreads_or(!mine)) { ok = false; break; }
-    umma::fence_after_sync();
-    if (c == 0) {
-      tmem = __shfl_sync(0xffffffffu, *tslot, 0);
-      tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    }
-    if (warp == kLead) {
-      if (c > 0 && umma::elect_one()) {  // y of the last chunk (a whole one) leaves from x's tile
-        umma::tma_store_2d(&ty, sm + M::kX, h * p.P + p0, static_cast<int>(tc0 - kL));
-        umma::bulk_commit();
+    auto store_h = [&]() {
+      if (row < S_) {
+        sts16(sbase + M::kH + piece.at[0], pack8(hr));
+        sts16(sbase + M::kH + piece.at[1], pack8(hr + 4));
       }
-      wait(bar_cb, c & 1, kSiteScanLoad);
-      if (mine && umma::elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < S_ / 16; ++ks) umma::mma_f16(tmem, d_c + k_step(ks), d_bk + k_step(ks), id_s, ks > 0);
-        if (has_h)
-#pragma unroll
-          for (int ks = 0; ks < S_ / 16; ++ks)
-            umma::mma_f16(tmem + M::kYi, d_c + k_step(ks), d_h + mn_step(ks), id_y, ks > 0);
-        umma::mma_commit(bar_s);
-        ++commits_s;
-        if (c > 0) {  // x goes where y was
-          umma::bulk_wait_read_all();
-          fetch_x(c);
-          ++loads_x;
-        }
+    };
+    store_h();
+    publish(bar_h);
+    for (int c = 0; c < nch; ++c) {
+      const int len = length(c);
+      const uint32_t st = sbase + (c & 1) * M::kStage;
+      const float ai = sc.a, all = sc.end[3];
+      const float wj = sc.k * ex2(all - pick4(sc.end, quad));
+      uint4 zr[2];
+      if (p.z && row < len) {
+        const __nv_bfloat16* zp = static_cast<const __nv_bfloat16*>(p.z) + (t0 + static_cast<int64_t>(c) * kL + row) * p.sz + col;
+        zr[0] = ld_now16(zp);
+        zr[1] = ld_now16(zp + 8);
       }
-      __syncwarp();
-    }
-    uint4 zr[4];
-    const int64_t col = static_cast<int64_t>(h) * p.P + p0 + half * 32;
-    if (p.z && row < len) {
-      const uint4* zp = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.z) + (tc0 + row) * p.sz + col);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) zr[q] = __ldg(zp + q);
-    }
-    // ---- P from the scores ----
-    wait(bar_s, c & 1, kSiteScanScores);
-    umma::fence_after_sync();
-#pragma unroll
-    for (int jb = 0; jb < 2; ++jb) {
-      const int J = half * 2 + jb;
-      uint4 out[4];
-      if (J <= quad) {
+      // ---- P from the scores: block of columns J = cq ----
+      const uint32_t prow_at = sbase + M::kP + (cq >> 1) * kTile + row * 128;
+      if (!wait(bar_s, c & 1, kSiteScanScores)) break;
+      umma::fence_after_sync();
+      if (cq <= quad) {
+        const float far = ai - pick4(sc.end, cq);
+        const bool diag = cq == quad;
         float v[32];
-        umma::tmem_ld32(tl + J * 32, v);
-        const float far = ai - (jb == 0 ? (half == 0 ? sc.end[0] : sc.end[2]) : (half == 0 ? sc.end[1] : sc.end[3]));
-        const bool diag = J == quad;
+        umma::tmem_ld32(tl + (c & 1) * 128 + cq * 32, v);
         // far is largest in the block's first row: one answer per warp
         if (!diag || __shfl_sync(0xffffffffu, far, 0) < 100.f) {
+          asm volatile("st.shared.f32 [%0], %1;" :: "r"(cf + lane * 4), "f"(kj) : "memory");
+          __syncwarp();
           const float f = ex2(far);
           const float2 f2 = make_float2(f, f);
-          const float4* cf = reinterpret_cast<const float4*>(sm + M::kCf) + J * 8;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float4 k0 = cf[q * 2], k1 = cf[q * 2 + 1];
-            float2 w[4] = {make_float2(v[q * 8], v[q * 8 + 1]), make_float2(v[q * 8 + 2], v[q * 8 + 3]),
-                           make_float2(v[q * 8 + 4], v[q * 8 + 5]), make_float2(v[q * 8 + 6], v[q * 8 + 7])};
-            w[0] = __fmul2_rn(w[0], __fmul2_rn(f2, make_float2(k0.x, k0.y)));
-            w[1] = __fmul2_rn(w[1], __fmul2_rn(f2, make_float2(k0.z, k0.w)));
-            w[2] = __fmul2_rn(w[2], __fmul2_rn(f2, make_float2(k1.x, k1.y)));
-            w[3] = __fmul2_rn(w[3], __fmul2_rn(f2, make_float2(k1.z, k1.w)));
-            if (diag)
+            const uint4 k0 = lds16(cf + q * 32), k1 = lds16(cf + q * 32 + 16);
+            const uint32_t kk[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+            float2 w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e) {
+              const float2 k2 = make_float2(__uint_as_float(kk[e * 2]), __uint_as_float(kk[e * 2 + 1]));
+              w[e] = __fmul2_rn(make_float2(v[q * 8 + e * 2], v[q * 8 + e * 2 + 1]), __fmul2_rn(f2, k2));
+              if (diag) {
                 if (q * 8 + e * 2 > lane) w[e].x = 0.f;
                 if (q * 8 + e * 2 + 1 > lane) w[e].y = 0.f;
               }
-            out[q] = pack8(w);
+            }
+            sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), pack8(w));
           }
+          __syncwarp();
         } else {
-          const float dt = row < len ? __ldg(prep.dt + prow + tc0 + row) : 0.f;
+          const float dt = row < len ? __ldg(prep.dt + prow + c * kL + row) : 0.f;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const float aj = __shfl_sync(0xffffffffu, ai, j), dj = __shfl_sync(0xffffffffu, dt, j);
             v[j] = j <= lane ? v[j] * (ex2(ai - aj) * dj) : 0.f;
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) out[q] = tc::pack8<__nv_bfloat16>(v + q * 8);
+          for (int q = 0; q < 4; ++q)
+            sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), tc::pack8<__nv_bfloat16>(v + q * 8));
         }
-      } else {
+      } else if (c == 0) {  // nothing else is written there
 #pragma unroll
-        for (int q = 0; q < 4; ++q) out[q] = make_uint4(0u, 0u, 0u, 0u);
+        for (int q = 0; q < 4; ++q) sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
       }
+      // ---- w x in parts (x has been there since the scores were issued) ----
+      if (!wait(bar_ld + (c & 1) * 8, (c >> 1) & 1, kSiteScanLoad)) break;
+      uint4 part[2], low[2];
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) *tile16(sm + M::kC + half * kTile, row, jb * 4 + q) = out[q];
-    }
-    // ---- w x in parts ----
-    wait(bar_x, c & 1, kSiteScanLoad);
-    uint4 low[4];
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      for (int q = 0; q < 2; ++q) {
+        uint4 u = lds16(st + M::kX + piece.at[q]);
+        if (row >= len) {  // another sequence's rows: zero operands, whatever they hold
+          u = zero;
+          sts16(st + M::kX + piece.at[q], zero);
+        }
+        float2 v[4];
+        unpack8(u, v);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4* xp = tile16(sm + M::kX, row, half * 4 + q);
-      uint4 u = *xp;
-      if (row >= len) *xp = u = zero;  // another sequence's rows: zero operands, whatever they hold
-      float2 v[4];
-      unpack8(u, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(wj, wj));
-      *tile16(sm + M::kXs, row, half * 4 + q) = take_part(v);
-      if (want_state) {
-        *tile16(sm + M::kH, row, half * 4 + q) = take_part(v);
-        low[q] = pack8(v);
-      } else {
-        *tile16(sm + M::kH, row, half * 4 + q) = pack8(v);
-      }
-    }
-    if (row >= len) {
-#pragma unroll
-      for (int q = 0; q < S_ / 16; ++q) {
-        const int piece = half * (S_ / 16) + q;  // of S_ / 8
-        *tile16(sm + M::kB + (piece >> 3) * kTile, row, piece & 7) = zero;
-      }
-    }
-    if (c + 1 < nch) sc = load_scalars(prep, prow, tc0 + kL, length(c + 1), row);
-    umma::fence_proxy_async();
-    umma::fence_before_sync();
-    if (__syncthreads_or(!mine)) { ok = false; break; }
-    umma::fence_after_sync();
-    if (warp == kLead && umma::elect_one()) {
-#pragma unroll
-      for (int ks = 0; ks < kL / 16; ++ks)
-        umma::mma_f16(tmem + M::kYa, d_c + k_step(ks), d_x + mn_step(ks), id_y, ks > 0);
-      umma::mma_commit(bar_y);
-      ++commits_y;
-      mma_dh(d_xs, true);
-      mma_dh(d_h, false);
-      umma::mma_commit(bar_dh);
-      ++commits_dh;
-    }
-    __syncwarp();
-    // ---- outputs ----
-    wait(bar_y, c & 1, kSiteScanOut);
-    umma::fence_after_sync();
-    if (leader && mine && c + 1 < nch) {
-      fetch_c(c + 1);
-      ++loads_cb;
-    }
-    __syncwarp();
-    if (mine) {
-      const float g1 = ex2(ai);
-      const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
-      __nv_bfloat16* yp = static_cast<__nv_bfloat16*>(p.y) + (tc0 + row) * p.H * p.P + col;
-#pragma unroll
-      for (int q2 = 0; q2 < 2; ++q2) {
-        float yi[16], ya[16];
-        if (has_h) {
-          umma::tmem_ld16x2(tl + M::kYi + half * 32 + q2 * 16, tl + M::kYa + half * 32 + q2 * 16, yi, ya);
+        for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(wj, wj));
+        sts16(sbase + M::kXs + piece.at[q], take_part(v));
+        if (want_state) {
+          part[q] = take_part(v);
+          low[q] = pack8(v);
         } else {
-          umma::tmem_ld16(tl + M::kYa + half * 32 + q2 * 16, ya);
+          part[q] = pack8(v);
+        }
+      }
+      if (row >= len)
+#pragma unroll
+        for (int q = 0; q < S_ / 32; ++q) {
+          const int at = cq * (S_ / 32) + q;  // of S_ / 8 pieces
+          sts16(st + M::kB + (at >> 3) * kTile + row * 128 + (((at & 7) ^ (row & 7)) << 4), zero);
+        }
+      if (!wait(bar_yi, c & 1, kSiteScanScores)) break;  // C and h are read
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        sts16(st + M::kC + piece.at[q], part[q]);
+        if (want_state) sts16(sbase + M::kH + piece.at[q], low[q]);
+      }
+      publish(bar_px);
+      if (c + 1 < nch) {
+        const int ln = length(c + 1);
+        sc = load_scalars(prep, prow + (c + 1) * kL, ln, row);
+        kj = 0.f;
+        if (cq * 32 + lane < ln) kj = ld_now(prep.k + prow + (c + 1) * kL + cq * 32 + lane);
+      }
+      // ---- outputs ----
+      if (!wait(bar_y, c & 1, kSiteScanOut)) break;
+      umma::fence_after_sync();
+      {
+        const float g1 = ex2(ai);
+        const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
+        float yi[16], ya[16];
+        if (c > 0 || seg || ini) {
+          umma::tmem_ld16x2(tl + M::kYi + cq * 16, tl + M::kYa + cq * 16, yi, ya);
+        } else {
+          umma::tmem_ld16(tl + M::kYa + cq * 16, ya);
 #pragma unroll
           for (int e = 0; e < 16; ++e) yi[e] = 0.f;
         }
+        __nv_bfloat16* yp = static_cast<__nv_bfloat16*>(p.y) + (t0 + static_cast<int64_t>(c) * kL + row) * p.H * p.P + col;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          uint4* xp = tile16(sm + M::kX, row, half * 4 + q2 * 2 + q);
           float2 xv[4], zv[4], o[4];
-          unpack8(*xp, xv);
-          if (p.z) unpack8(zr[q2 * 2 + q], zv);
+          unpack8(lds16(st + M::kX + piece.at[q]), xv);
+          if (p.z) unpack8(zr[q], zv);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = q * 8 + e * 2;
@@ -502,79 +592,37 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
             }
           }
           const uint4 u = pack8(o);
-          if (len == kL) *xp = u;
-          else if (row < len) *reinterpret_cast<uint4*>(yp + q2 * 16 + q * 8) = u;
+          if (len == kL) sts16(st + M::kX + piece.at[q], u);
+          else if (row < len) *reinterpret_cast<uint4*>(yp + q * 8) = u;
         }
       }
-    }
-    // ---- state ----
-    wait(bar_dh, par_dh, kSiteScanState);
-    par_dh ^= 1;
-    if (want_state) {  // the third part, in the first one's tile
-#pragma unroll
-      for (int q = 0; q < 4; ++q) *tile16(sm + M::kXs, row, half * 4 + q) = low[q];
-      umma::fence_proxy_async();
-      umma::fence_before_sync();
-      if (__syncthreads_or(!mine)) { ok = false; break; }
+      // ---- state ----
+      if (!wait(bar_dh, c & 1, kSiteScanState)) break;
       umma::fence_after_sync();
-      if (warp == kLead && umma::elect_one()) {
-        mma_dh(d_xs, false);
-        umma::mma_commit(bar_dh);
-        ++commits_dh;
+      const float decay = ex2(all);
+      {
+        float d[16];
+        umma::tmem_ld16(tl + M::kDH + cq * 16, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          hr[j] = __ffma2_rn(make_float2(decay, decay), hr[j], make_float2(d[j * 2], d[j * 2 + 1]));
       }
-      __syncwarp();
-      wait(bar_dh, par_dh, kSiteScanState);
-      par_dh ^= 1;
+      store_h();
+      publish(bar_h);
     }
-    umma::fence_after_sync();
-    if (leader && mine && c + 1 < nch) fetch_b(c + 1);
-    __syncwarp();
-    const float decay = ex2(all);
-    {
-      float d[32];
-      umma::tmem_ld32(tl + M::kDH + half * 32, d);
+    if (mine && row < S_ && want_state)
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        hr[j] = __ffma2_rn(make_float2(decay, decay), hr[j], make_float2(d[j * 2], d[j * 2 + 1]));
-    }
-    if (c + 1 < nch) store_h();
-    has_h = true;
-  }
-  if (nch > 0) {  // the last chunk's y
-    umma::fence_proxy_async();
-    umma::fence_before_sync();
-    if (ok) ok = !__syncthreads_or(!mine);
-    if (ok && leader) {
-      if (length(nch - 1) == kL) {
-        umma::tma_store_2d(&ty, sm + M::kX, h * p.P + p0, static_cast<int>(t1) - kL);
-        umma::bulk_commit();
-      }
-    }
-    __syncwarp();
-  }
-  if (ok && row < S_ && want_state)
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      st_any(p.final_state, p.final_dtype, at_seq + static_cast<int64_t>(j) * S_, j & 1 ? hr[j / 2].y : hr[j / 2].x);
-  if (leader) umma::bulk_wait_all();
-  if (!ok && leader) {
-    // copies and products that this CTA issued may be in flight: wait
-    // (bounded) for the last of each before memory is released
-    const long long drain = 20000000LL;
-    if (loads_cb) umma::mbar_wait(bar_cb, (loads_cb - 1) & 1, drain);
-    if (loads_x) umma::mbar_wait(bar_x, (loads_x - 1) & 1, drain);
-    if (commits_s) umma::mbar_wait(bar_s, (commits_s - 1) & 1, drain);
-    if (commits_y) umma::mbar_wait(bar_y, (commits_y - 1) & 1, drain);
-    if (commits_dh) umma::mbar_wait(bar_dh, (commits_dh - 1) & 1, drain);
+        st_any(p.final_state, p.final_dtype, at_seq + static_cast<int64_t>(j) * S_, j & 1 ? hr[j / 2].y : hr[j / 2].x);
   }
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  if (warp == kLead) umma::tmem_dealloc(*tslot, M::kCols);
+  if (warp == kLead) umma::tmem_dealloc(tmem, M::kCols);
 }
 
 template <int S_>
-__global__ void __launch_bounds__(kTcThreads, 2)
+__global__ void __launch_bounds__(kTcThreads, 1)
 scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, const __grid_constant__ CUtensorMap tx,
                      const __grid_constant__ CUtensorMap tb) {
   using M = StateSmem<S_>;
@@ -582,11 +630,8 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::kBar);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + M::kTmem);
   const uint32_t sbase = umma::smem_u32(sm);
-  const uint32_t bar_ld = umma::smem_u32(bars), bar_dh = bar_ld + 8;
+  const uint32_t bar_ld = umma::smem_u32(bars), bar_xs = bar_ld + 16, bar_dh = bar_ld + 32;  // [2] each
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
-  // the thread that issues every copy and product (elect.sync picks the same lane each time)
-  const bool leader = warp == 0 && umma::elect_one();
   if (!base_ok(p, sbase)) return;
   const int units = p.H * slices;
   const int64_t id = blockIdx.x / units;
@@ -596,96 +641,114 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   bool last = false;
   if (!find_segment(p, id, n, ls, t0, t1, last) || last) return;
   const int nch = static_cast<int>((t1 - t0) / kL);  // a segment that is not the last is whole chunks
-  const int64_t prow = static_cast<int64_t>(h) * p.total;
-  auto fetch = [&](int c) {
-    const int t = static_cast<int>(t0) + c * kL;
-    umma::mbar_arrive_expect_tx(bar_ld, M::kTx);
+  if (warp == kLead) {
+    if (umma::elect_one()) {
 #pragma unroll
-    for (int q = 0; q < S_ / 64; ++q) umma::tma_load_2d(sm + M::kB + q * kTile, &tb, g * S_ + q * 64, t, bar_ld);
-    umma::tma_load_2d(sm + M::kX, &tx, h * p.P + p0, t, bar_ld);
-  };
-  if (leader) {
-    umma::mbar_init(bars, 1);
-    umma::mbar_init(bars + 1, 1);
-    umma::mbar_fence_init();
-    fetch(nch - 1);
-  }
-  if (warp == 0) {
+      for (int i = 0; i < 6; ++i) umma::mbar_init(bars + i, i == 2 || i == 3 ? kLead : 1);
+      umma::mbar_fence_init();
+    }
+    __syncwarp();
     umma::tmem_alloc(tslot, M::kCols);
     umma::fence_before_sync();
   }
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tslot, 0);
-  constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
-  const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
-  bool ok = true, mine = true;
-  int loads = 1, commits = 0;
+  bool mine = true;
   auto wait = [&](uint32_t bar, uint32_t parity, int site) {
     const bool got = __all_sync(0xffffffffu, mine && (umma::mbar_test(bar, parity) || umma::mbar_wait(bar, parity, kWaitLimit)));
     if (mine && !got) record_device_error(p.err, kErrWaitTimeout, site, static_cast<int>(blockIdx.x), tid);
     mine = got;
+    return got;
   };
-  float later = 0.f;  // log2 decay from the chunk's end to the segment's
-  TokenScalars sc = load_scalars(prep, prow, t0 + static_cast<int64_t>(nch - 1) * kL, kL, row);
-  for (int i = 0; i < nch; ++i) {
-    const int c = nch - 1 - i;
-    const float wj = sc.k * ex2(sc.end[3] - pick4(sc.end, quad)) * ex2(later);
-    later += sc.end[3];
-    if (c > 0) sc = load_scalars(prep, prow, t0 + static_cast<int64_t>(c - 1) * kL, kL, row);
-    wait(bar_ld, i & 1, kSiteScanLoad);
+  // step i works on chunk nch - 1 - i in stage i & 1
+  if (warp == kLead) {
+    constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
+    const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
+    auto fetch = [&](int i) {
+      const int t = static_cast<int>(t0) + (nch - 1 - i) * kL;
+      const uint32_t bar = bar_ld + (i & 1) * 8;
+      uint8_t* st = sm + (i & 1) * M::kStage;
+      umma::mbar_arrive_expect_tx(bar, M::kTx);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float2 v[4];
-      unpack8(*tile16(sm + M::kX, row, half * 4 + q), v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(wj, wj));
-      *tile16(sm + M::kXs, row, half * 4 + q) = take_part(v);
-      *tile16(sm + M::kXs + kTile, row, half * 4 + q) = take_part(v);
-      *tile16(sm + M::kXs + 2 * kTile, row, half * 4 + q) = pack8(v);
-    }
-    umma::fence_proxy_async();
-    umma::fence_before_sync();
-    if (__syncthreads_or(!mine)) { ok = false; break; }
-    umma::fence_after_sync();
-    if (warp == 0 && umma::elect_one()) {
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int ks = 0; ks < kL / 16; ++ks)
-          umma::mma_f16(tmem, d_bm + mn_step(ks), d_xs + ((part * kTile) >> 4) + mn_step(ks), id_h, i > 0 || part > 0 || ks > 0);
-      umma::mma_commit(bar_dh);
-      ++commits;
+      for (int q = 0; q < S_ / 64; ++q) umma::tma_load_2d(st + M::kB + q * kTile, &tb, g * S_ + q * 64, t, bar);
+      umma::tma_load_2d(st + M::kX, &tx, h * p.P + p0, t, bar);
+    };
+    if (umma::elect_one()) {
+      fetch(0);
+      if (nch > 1) fetch(1);
     }
     __syncwarp();
-    wait(bar_dh, i & 1, kSiteScanState);
-    umma::fence_after_sync();
-    if (leader && mine && c > 0) {
-      fetch(c - 1);
-      ++loads;
-    }
-    __syncwarp();
-  }
-  if (ok) ok = !__syncthreads_or(!mine);
-  if (ok) {
-    float d[32];
-    umma::tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 32, d);
-    if (row < S_) {
-      float* out = p.seg_state + ((id * p.H + h) * p.P + p0 + half * 32) * S_ + row;
+    int loads = min(nch, 2), done = 0;
+    for (int i = 0; i < nch; ++i) {
+      if (!wait(bar_xs + (i & 1) * 8, (i >> 1) & 1, kSiteScanScores)) break;
+      if (i >= 1 && i + 1 < nch) {  // step i + 1 goes where step i - 1 was
+        if (!wait(bar_dh + ((i - 1) & 1) * 8, ((i - 1) >> 1) & 1, kSiteScanState)) break;
+        if (umma::elect_one()) fetch(i + 1);
+        __syncwarp();
+        ++loads;
+      }
+      umma::fence_after_sync();
+      if (umma::elect_one()) {
+        const uint64_t st = (i & 1) * (M::kStage >> 4);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) out[j * S_] = d[j];
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int ks = 0; ks < kL / 16; ++ks)
+            umma::mma_f16(tmem, d_bm + st + mn_step(ks), d_xs + st + ((part * kTile) >> 4) + mn_step(ks), id_h,
+                          i > 0 || part > 0 || ks > 0);
+        umma::mma_commit(bar_dh + (i & 1) * 8);
+      }
+      __syncwarp();
+      ++done;
     }
-    if (tid == 0 && p0 == 0) p.seg_decay[id * p.H + h] = later * 0.6931471805599453f;
-  }
-  if (!ok && leader) {
-    const long long drain = 20000000LL;
-    umma::mbar_wait(bar_ld, (loads - 1) & 1, drain);
-    if (commits) umma::mbar_wait(bar_dh, (commits - 1) & 1, drain);
+    if (!mine) {
+      const long long drain = 20000000LL;
+      for (int i = max(0, loads - 2); i < loads; ++i) umma::mbar_wait(bar_ld + (i & 1) * 8, (i >> 1) & 1, drain);
+      for (int i = max(0, done - 2); i < done; ++i) umma::mbar_wait(bar_dh + (i & 1) * 8, (i >> 1) & 1, drain);
+    }
+  } else {
+    const int quad = warp & 3, cq = warp >> 2, row = quad * 32 + lane;
+    const Pieces piece(row, cq);
+    const int64_t prow = static_cast<int64_t>(h) * p.total + t0;
+    float later = 0.f;  // log2 decay from the chunk's end to the segment's
+    TokenScalars sc = load_scalars(prep, prow + (nch - 1) * kL, kL, row);
+    for (int i = 0; i < nch; ++i) {
+      const uint32_t st = sbase + (i & 1) * M::kStage;
+      const float wj = sc.k * ex2(sc.end[3] - pick4(sc.end, quad)) * ex2(later);
+      later += sc.end[3];
+      if (i + 1 < nch) sc = load_scalars(prep, prow + (nch - 2 - i) * kL, kL, row);
+      // the stage's products of two steps ago are done: its loads came after them
+      if (!wait(bar_ld + (i & 1) * 8, (i >> 1) & 1, kSiteScanLoad)) break;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float2 v[4];
+        unpack8(lds16(st + M::kX + piece.at[q]), v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(wj, wj));
+        sts16(st + M::kXs + piece.at[q], take_part(v));
+        sts16(st + M::kXs + kTile + piece.at[q], take_part(v));
+        sts16(st + M::kXs + 2 * kTile + piece.at[q], pack8(v));
+      }
+      publish(bar_xs + (i & 1) * 8);
+    }
+    const int i = nch - 1;  // the last step's products come after all others
+    if (mine && wait(bar_dh + (i & 1) * 8, (i >> 1) & 1, kSiteScanState)) {
+      umma::fence_after_sync();
+      float d[16];
+      umma::tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + cq * 16, d);
+      if (row < S_) {
+        float* out = p.seg_state + ((id * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[j * S_] = d[j];
+      }
+      if (tid == 0 && p0 == 0) p.seg_decay[id * p.H + h] = later * 0.6931471805599453f;
+    }
   }
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  if (warp == 0) umma::tmem_dealloc(tmem, M::kCols);
+  if (warp == kLead) umma::tmem_dealloc(tmem, M::kCols);
 }
 
 bool tc_shape(const gdn_scan_args& a) {
