@@ -61,16 +61,17 @@ struct PrepOut {
 template <int S_>
 struct Smem {
   // two stages of operands
-  static constexpr int kC = 0;                              // C, then the second part of w x
-  static constexpr int kB = S_ / 64 * kTile;
-  static constexpr int kX = 2 * kB;                         // x, then y
+  static constexpr int kC = 0;                              // C, then the second part of w x, and z
+  static constexpr int kZ = kC + kTile;
+  static constexpr int kB = kC + 2 * kTile;
+  static constexpr int kX = kB + S_ / 64 * kTile;           // x, then y
   static constexpr int kStage = kX + kTile;
   static constexpr int kXs = 2 * kStage;                    // first part of w x
   static constexpr int kH = kXs + kTile;                    // h, then the third part of w x
   static constexpr int kP = kH + kTile;
   static constexpr int kCf = kP + 2 * kTile;                // k of one block of 32 tokens per warp
-  static constexpr int kBar = kCf + kWork / 32 * 32 * 4;    // loads[2], S, Yi, Ya, dH, h ready, P and w x ready
-  static constexpr int kBars = 8;
+  static constexpr int kBar = kCf + kWork / 32 * 32 * 4;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
+  static constexpr int kBars = 9;
   static constexpr int kTmem = kBar + kBars * 8;
   static constexpr int kBytes = kTmem + 8;
   static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile;
@@ -184,11 +185,6 @@ __device__ __forceinline__ float ld_now(const float* p) {
   asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint4 ld_now16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 
 // What a thread (token `row` of a chunk) needs of a and k.
 struct TokenScalars {
@@ -251,18 +247,36 @@ __device__ __forceinline__ bool base_ok(const ScanParams& p, uint32_t sbase) {
   return false;
 }
 
+// A diagonal block of P under decays past 2^100 within it: the difference of
+// each pair.  Out of line: its registers would push the common path's out.
+__device__ __noinline__ void diag_by_difference(uint32_t ts, uint32_t prow_at, int piece0, int row, float ai, float dt) {
+  const int lane = row & 31;
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    float v[8];
+    umma::tmem_ld8(ts + q * 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = q * 8 + e;
+      const float aj = __shfl_sync(0xffffffffu, ai, j), dj = __shfl_sync(0xffffffffu, dt, j);
+      v[e] = j <= lane ? v[e] * (ex2(ai - aj) * dj) : 0.f;
+    }
+    sts16(prow_at + (((piece0 + q) ^ (row & 7)) << 4), tc::pack8<__nv_bfloat16>(v));
+  }
+}
+
 template <int S_>
 __global__ void __launch_bounds__(kTcThreads, 1)
 scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const __grid_constant__ CUtensorMap tx,
                const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tcm,
-               const __grid_constant__ CUtensorMap ty) {
+               const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tz) {
   using M = Smem<S_>;
   extern __shared__ __align__(1024) uint8_t sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::kBar);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + M::kTmem);
   const uint32_t sbase = umma::smem_u32(sm);
   const uint32_t bar_ld = umma::smem_u32(bars), bar_s = bar_ld + 16, bar_yi = bar_ld + 24, bar_y = bar_ld + 32,
-                 bar_dh = bar_ld + 40, bar_h = bar_ld + 48, bar_px = bar_ld + 56;
+                 bar_dh = bar_ld + 40, bar_z = bar_ld + 48, bar_h = bar_ld + 56, bar_px = bar_ld + 64;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (!base_ok(p, sbase)) return;
   // Block = segment * units + unit: the CTAs that read the same B and C are
@@ -283,7 +297,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   if (warp == kLead) {
     if (umma::elect_one()) {
 #pragma unroll
-      for (int i = 0; i < M::kBars; ++i) umma::mbar_init(bars + i, i < 6 ? 1 : kLead);
+      for (int i = 0; i < M::kBars; ++i) umma::mbar_init(bars + i, i < 7 ? 1 : kLead);
       umma::mbar_fence_init();
     }
     __syncwarp();
@@ -339,7 +353,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         umma::mma_f16(tmem + (c & 1) * 128, d_c + st + k_step(ks), d_bk + st + k_step(ks), id_s, ks > 0);
       umma::mma_commit(bar_s);
     };
-    int loads = 0, n_s = 0, n_yi = 0, n_y = 0, n_dh = 0;  // issued so far
+    int loads = 0, n_s = 0, n_yi = 0, n_y = 0, n_dh = 0, n_z = 0;  // issued so far
     if (nch > 0) {
       if (umma::elect_one()) {
         fetch_cb(0);
@@ -374,6 +388,15 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       __syncwarp();
       ++n_yi;
       loads += c + 1 < nch;
+      if (p.z) {  // beside what C's tile takes next, once Yi has read it
+        if (!wait(bar_yi, c & 1, kSiteScanScores)) break;
+        if (umma::elect_one()) {
+          umma::mbar_arrive_expect_tx(bar_z, kTile);
+          umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kZ, &tz, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_z);
+        }
+        __syncwarp();
+        ++n_z;
+      }
       if (!wait(bar_px, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
       if (umma::elect_one()) {
@@ -418,6 +441,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       const long long drain = 20000000LL;
       if (loads > 1) umma::mbar_wait(bar_ld + (loads & 1) * 8, ((loads - 2) >> 1) & 1, drain);
       if (loads > 0) umma::mbar_wait(bar_ld + ((loads - 1) & 1) * 8, ((loads - 1) >> 1) & 1, drain);
+      if (n_z) umma::mbar_wait(bar_z, (n_z - 1) & 1, drain);
       if (n_s) umma::mbar_wait(bar_s, (n_s - 1) & 1, drain);
       if (n_yi) umma::mbar_wait(bar_yi, (n_yi - 1) & 1, drain);
       if (n_y) umma::mbar_wait(bar_y, (n_y - 1) & 1, drain);
@@ -432,8 +456,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     const uint32_t cf = sbase + M::kCf + warp * 128;
     const int64_t prow = static_cast<int64_t>(h) * p.total + t0;
     const int64_t col = static_cast<int64_t>(h) * p.P + p0 + cq * 16;
-    const int64_t at_seq = ((n * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
-    const int64_t at_seg = ((id * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
+    auto state_at = [&](int64_t i) { return ((i * p.H + h) * p.P + p0 + cq * 16) * S_ + row; };
     const float D = p.D ? p.D[h] : 0.f;
     TokenScalars sc;
     float kj = 0.f;  // k of token 32 cq + lane
@@ -446,8 +469,8 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     for (int j = 0; j < 16; ++j) {
       float v = 0.f;
       if (row < S_) {
-        if (seg) v = p.seg_state[at_seg + static_cast<int64_t>(j) * S_];
-        else if (ini) v = ld_any(p.init, p.init_dtype, at_seq + static_cast<int64_t>(j) * S_);
+        if (seg) v = p.seg_state[state_at(id) + j * S_];
+        else if (ini) v = ld_any(p.init, p.init_dtype, state_at(n) + j * S_);
       }
       if (j & 1) hr[j / 2].y = v;
       else hr[j / 2].x = v;
@@ -465,12 +488,6 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       const uint32_t st = sbase + (c & 1) * M::kStage;
       const float ai = sc.a, all = sc.end[3];
       const float wj = sc.k * ex2(all - pick4(sc.end, quad));
-      uint4 zr[2];
-      if (p.z && row < len) {
-        const __nv_bfloat16* zp = static_cast<const __nv_bfloat16*>(p.z) + (t0 + static_cast<int64_t>(c) * kL + row) * p.sz + col;
-        zr[0] = ld_now16(zp);
-        zr[1] = ld_now16(zp + 8);
-      }
       // ---- P from the scores: block of columns J = cq ----
       const uint32_t prow_at = sbase + M::kP + (cq >> 1) * kTile + row * 128;
       if (!wait(bar_s, c & 1, kSiteScanScores)) break;
@@ -478,8 +495,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       if (cq <= quad) {
         const float far = ai - pick4(sc.end, cq);
         const bool diag = cq == quad;
-        float v[32];
-        umma::tmem_ld32(tl + (c & 1) * 128 + cq * 32, v);
+        const uint32_t ts = tl + (c & 1) * 128 + cq * 32;
         // far is largest in the block's first row: one answer per warp
         if (!diag || __shfl_sync(0xffffffffu, far, 0) < 100.f) {
           asm volatile("st.shared.f32 [%0], %1;" :: "r"(cf + lane * 4), "f"(kj) : "memory");
@@ -487,32 +503,30 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
           const float f = ex2(far);
           const float2 f2 = make_float2(f, f);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint4 k0 = lds16(cf + q * 32), k1 = lds16(cf + q * 32 + 16);
-            const uint32_t kk[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-            float2 w[4];
+          for (int hf = 0; hf < 2; ++hf) {  // 16 columns at a time: registers
+            float v[16];
+            umma::tmem_ld16(ts + hf * 16, v);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 k2 = make_float2(__uint_as_float(kk[e * 2]), __uint_as_float(kk[e * 2 + 1]));
-              w[e] = __fmul2_rn(make_float2(v[q * 8 + e * 2], v[q * 8 + e * 2 + 1]), __fmul2_rn(f2, k2));
-              if (diag) {
-                if (q * 8 + e * 2 > lane) w[e].x = 0.f;
-                if (q * 8 + e * 2 + 1 > lane) w[e].y = 0.f;
+            for (int q = 0; q < 2; ++q) {
+              const uint4 k0 = lds16(cf + hf * 64 + q * 32), k1 = lds16(cf + hf * 64 + q * 32 + 16);
+              const uint32_t kk[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+              float2 w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = hf * 16 + q * 8 + e * 2;
+                const float2 k2 = make_float2(__uint_as_float(kk[e * 2]), __uint_as_float(kk[e * 2 + 1]));
+                w[e] = __fmul2_rn(make_float2(v[q * 8 + e * 2], v[q * 8 + e * 2 + 1]), __fmul2_rn(f2, k2));
+                if (diag) {
+                  if (j > lane) w[e].x = 0.f;
+                  if (j + 1 > lane) w[e].y = 0.f;
+                }
               }
+              sts16(prow_at + ((((cq & 1) * 4 + hf * 2 + q) ^ (row & 7)) << 4), pack8(w));
             }
-            sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), pack8(w));
           }
           __syncwarp();
         } else {
-          const float dt = row < len ? __ldg(prep.dt + prow + c * kL + row) : 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float aj = __shfl_sync(0xffffffffu, ai, j), dj = __shfl_sync(0xffffffffu, dt, j);
-            v[j] = j <= lane ? v[j] * (ex2(ai - aj) * dj) : 0.f;
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), tc::pack8<__nv_bfloat16>(v + q * 8));
+          diag_by_difference(ts, prow_at, (cq & 1) * 4, row, ai, row < len ? __ldg(prep.dt + prow + c * kL + row) : 0.f);
         }
       } else if (c == 0) {  // nothing else is written there
 #pragma unroll
@@ -561,29 +575,25 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         if (cq * 32 + lane < ln) kj = ld_now(prep.k + prow + (c + 1) * kL + cq * 32 + lane);
       }
       // ---- outputs ----
+      if (p.z && !wait(bar_z, c & 1, kSiteScanLoad)) break;
       if (!wait(bar_y, c & 1, kSiteScanOut)) break;
       umma::fence_after_sync();
       {
         const float g1 = ex2(ai);
         const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
-        float yi[16], ya[16];
-        if (c > 0 || seg || ini) {
-          umma::tmem_ld16x2(tl + M::kYi + cq * 16, tl + M::kYa + cq * 16, yi, ya);
-        } else {
-          umma::tmem_ld16(tl + M::kYa + cq * 16, ya);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) yi[e] = 0.f;
-        }
-        __nv_bfloat16* yp = static_cast<__nv_bfloat16*>(p.y) + (t0 + static_cast<int64_t>(c) * kL + row) * p.H * p.P + col;
+        const bool has_yi = c > 0 || seg || ini;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
+          float yi[8], ya[8];
+          umma::tmem_ld8x2(tl + M::kYi + cq * 16 + q * 8, tl + M::kYa + cq * 16 + q * 8, yi, ya);
           float2 xv[4], zv[4], o[4];
           unpack8(lds16(st + M::kX + piece.at[q]), xv);
-          if (p.z) unpack8(zr[q], zv);
+          if (p.z) unpack8(lds16(st + M::kZ + piece.at[q]), zv);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = q * 8 + e * 2;
-            o[e] = __ffma2_rn(g2, make_float2(yi[i], yi[i + 1]), make_float2(ya[i], ya[i + 1]));
+            const float2 a2 = make_float2(ya[e * 2], ya[e * 2 + 1]);
+            // without a state Yi was not computed: its columns hold anything
+            o[e] = has_yi ? __ffma2_rn(g2, make_float2(yi[e * 2], yi[e * 2 + 1]), a2) : a2;
             o[e] = __ffma2_rn(D2, xv[e], o[e]);
             if (p.z) {
               float zz[2] = {zv[e].x, zv[e].y};
@@ -592,8 +602,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
             }
           }
           const uint4 u = pack8(o);
-          if (len == kL) sts16(st + M::kX + piece.at[q], u);
-          else if (row < len) *reinterpret_cast<uint4*>(yp + q * 8) = u;
+          if (len == kL) {
+            sts16(st + M::kX + piece.at[q], u);
+          } else if (row < len) {
+            __nv_bfloat16* yp = static_cast<__nv_bfloat16*>(p.y) + (t0 + static_cast<int64_t>(c) * kL + row) * p.H * p.P + col;
+            *reinterpret_cast<uint4*>(yp + q * 8) = u;
+          }
         }
       }
       // ---- state ----
@@ -613,7 +627,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     if (mine && row < S_ && want_state)
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        st_any(p.final_state, p.final_dtype, at_seq + static_cast<int64_t>(j) * S_, j & 1 ? hr[j / 2].y : hr[j / 2].x);
+        st_any(p.final_state, p.final_dtype, state_at(n) + j * S_, j & 1 ? hr[j / 2].y : hr[j / 2].x);
   }
   umma::fence_before_sync();
   __syncthreads();
@@ -781,13 +795,14 @@ static cudaError_t make_rows_map(CUtensorMap* m, const void* ptr, int64_t cols, 
 
 template <int S_>
 static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, cudaStream_t s) {
-  CUtensorMap tx, tb, tcm, ty;
+  CUtensorMap tx, tb, tcm, ty, tz;
   cudaError_t e;
   const int64_t total = a.B * a.T, gs = static_cast<int64_t>(a.G) * a.S, hp = static_cast<int64_t>(a.H) * a.P;
   if ((e = make_rows_map(&tx, a.x, hp, total, a.stride_x)) != cudaSuccess) return e;
   if ((e = make_rows_map(&tb, a.b, gs, total, a.stride_b)) != cudaSuccess) return e;
   if ((e = make_rows_map(&tcm, a.c, gs, total, a.stride_c)) != cudaSuccess) return e;
   if ((e = make_rows_map(&ty, a.y, hp, total, hp)) != cudaSuccess) return e;
+  if ((e = make_rows_map(&tz, a.z ? a.z : a.y, hp, total, a.z ? a.stride_z : hp)) != cudaSuccess) return e;
   const int slices = a.P / 64;
   const PrepOut prep{scratch, scratch + total * a.H, scratch + 2 * total * a.H};
   ScanParams q = p;
@@ -808,7 +823,7 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
   if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<S_>::kBytes)) != cudaSuccess)
     return e;
   note_launch();
-  kern<<<grid, kTcThreads, Smem<S_>::kBytes, s>>>(p, prep, slices, tx, tb, tcm, ty);
+  kern<<<grid, kTcThreads, Smem<S_>::kBytes, s>>>(p, prep, slices, tx, tb, tcm, ty, tz);
   return cudaGetLastError();
 }
 
