@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgdn_b200.so")
@@ -215,6 +216,26 @@ class ScanUpdateArgs(ctypes.Structure):
     ]
 
 
+class Packed:
+    """Packs the fields of an argument struct, in order, into bytes that a C
+    entry point takes in the struct's place: building a ctypes structure of
+    forty fields costs about 10 us of host time, which a call on a few tokens
+    would be bound by.  Pointers are integers (0 for null)."""
+
+    _CODES = {_vp: "P", _i64: "q", _i32: "i", ctypes.c_size_t: "N", ctypes.c_float: "f"}
+
+    def __init__(self, cls):
+        self.fields = [name for name, _ in cls._fields_]
+        layout = struct.Struct("@" + "".join(self._CODES[t] for _, t in cls._fields_) + "0q")
+        assert layout.size == ctypes.sizeof(cls), cls
+        self.pack = layout.pack
+
+
+pack_conv1d_bwd = Packed(Conv1dBwdArgs).pack
+pack_norm = Packed(NormArgs).pack
+pack_scan = Packed(ScanArgs).pack
+pack_scan_update = Packed(ScanUpdateArgs).pack
+
 _lib = None
 
 
@@ -266,16 +287,13 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.gdn_conv_chunk_workspace_size.restype = ctypes.c_size_t
     lib.gdn_conv_chunk_fwd.argtypes = [ctypes.POINTER(ChunkArgs), ctypes.POINTER(Conv1dFnArgs), _vp]
     lib.gdn_conv_chunk_fwd.restype = ctypes.c_int
-    for name, args in (("gdn_causal_conv1d_bwd", Conv1dBwdArgs), ("gdn_norm_fwd", NormArgs),
-                       ("gdn_norm_bwd", NormArgs), ("gdn_scan_fwd", ScanArgs),
-                       ("gdn_scan_update", ScanUpdateArgs)):
+    for name in ("gdn_causal_conv1d_bwd", "gdn_norm_fwd", "gdn_norm_bwd", "gdn_scan_fwd", "gdn_scan_update"):
         fn = getattr(lib, name)
-        fn.argtypes = [ctypes.POINTER(args), _vp]
+        fn.argtypes = [_vp, _vp]  # packed bytes (see Packed) or byref(struct)
         fn.restype = ctypes.c_int
-    for name, args in (("gdn_causal_conv1d_bwd_workspace_size", Conv1dBwdArgs),
-                       ("gdn_norm_bwd_workspace_size", NormArgs), ("gdn_scan_workspace_size", ScanArgs)):
+    for name in ("gdn_causal_conv1d_bwd_workspace_size", "gdn_norm_bwd_workspace_size", "gdn_scan_workspace_size"):
         fn = getattr(lib, name)
-        fn.argtypes = [ctypes.POINTER(args)]
+        fn.argtypes = [_vp]
         fn.restype = ctypes.c_size_t
     lib.gdn_last_error.argtypes = []
     lib.gdn_last_error.restype = ctypes.c_char_p

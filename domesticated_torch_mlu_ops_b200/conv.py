@@ -28,12 +28,13 @@ Differences from the reference, all supersets or stricter checks:
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .gdn import _DT, _IDT, _call, _cuda, _ptr, _stream
+from .gdn import _DT, _IDT, _addr, _cuda, _launch, _plain, _ptr, _stream
 
 
 def _act(activation):
@@ -111,6 +112,18 @@ def _fn_args(x, weight, bias, conv_states, query_start_loc, cache_indices, has_i
     return args, (w, b, qsl, ci, hi, blocks)
 
 
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace(B, T, N, D, W, x_dtype):
+    """Bytes of gdn_causal_conv1d_bwd's workspace: they depend on the shapes alone."""
+    args = _lib.Conv1dBwdArgs(B=B, T=T, N=N, D=D, stride_x_token=D, stride_dy_token=D, W=W, x_dtype=x_dtype)
+    if N != B:
+        args.cu_seqlens, args.cu_dtype = ctypes.c_void_p(16), _lib.GDN_I64  # packed: only whether it is there counts
+    n = _lib.load().gdn_causal_conv1d_bwd_workspace_size(ctypes.byref(args))
+    if n == 0:
+        _lib.check(_lib.GDN_ERR_INVALID)
+    return n
+
+
 def _conv1d_bwd_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], dy: torch.Tensor,
                      initial_state: Optional[torch.Tensor], activation: int,
                      cu_seqlens: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor,
@@ -133,22 +146,16 @@ def _conv1d_bwd_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     db = torch.empty(0 if bias is None else D, dtype=weight.dtype, device=dev)
     dh = torch.empty((0,) if initial_state is None else initial_state.shape,
                      dtype=x.dtype if initial_state is None else initial_state.dtype, device=dev)
-    args = _lib.Conv1dBwdArgs(
-        x=_ptr(x), weight=_ptr(weight), bias=_ptr(bias), initial_state=_ptr(initial_state), dy=_ptr(dy), dx=_ptr(dx),
-        dweight=_ptr(dw), dbias=None if bias is None else _ptr(db),
-        dinitial_state=None if initial_state is None else _ptr(dh), cu_seqlens=_ptr(cu_seqlens), B=B, T=T, N=N, D=D,
-        stride_x_token=sx, stride_dy_token=sdy, W=W, x_dtype=_fdt(x, "x"), w_dtype=_fdt(weight, "weight"),
-        state_dtype=_fdt(initial_state, "initial_state") if initial_state is not None else _lib.GDN_F32,
-        cu_dtype=_IDT[cu_seqlens.dtype] if cu_seqlens is not None else _lib.GDN_I64, activation=activation)
-    lib = _lib.load()
-    nbytes = lib.gdn_causal_conv1d_bwd_workspace_size(args)
-    if nbytes == 0:
-        # nothing to do is no error; everything else that has no size is
-        _lib.check(_lib.GDN_ERR_INVALID)
+    cu_dt = _lib.GDN_I64 if cu_seqlens is None else _IDT[cu_seqlens.dtype]
+    xt, wt = _DT[x.dtype], _DT[weight.dtype]
+    nbytes = _bwd_workspace(B, T, N, D, W, xt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ctypes.c_void_p(ws.data_ptr()), nbytes
-    with torch.cuda.device(dev):
-        _lib.check(lib.gdn_causal_conv1d_bwd(args, _stream(dev)))
+    packed = _lib.pack_conv1d_bwd(
+        x.data_ptr(), weight.data_ptr(), _addr(bias), _addr(initial_state), dy.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+        0 if bias is None else db.data_ptr(), 0 if initial_state is None else dh.data_ptr(), _addr(cu_seqlens),
+        ws.data_ptr(), nbytes, B, T, N, D, sx, sdy, W, xt, wt,
+        _lib.GDN_F32 if initial_state is None else _DT[initial_state.dtype], cu_dt, activation)
+    _launch(_lib.load().gdn_causal_conv1d_bwd, packed, dev)
     return dx, dw, db, dh
 
 
@@ -198,10 +205,9 @@ def causal_conv1d_bwd(
     if initial_state is not None and tuple(initial_state.shape) != (N, D, W):
         raise ValueError(f"[CausalConv1d] initial_state {tuple(initial_state.shape)} must be [N, D, W] = {(N, D, W)}")
     b_dtype = None if bias is None else bias.dtype
-    dx, dw, db, dh = _call(
-        torch.ops.gdn_b200.causal_conv1d_bwd, _conv1d_bwd_impl, x, weight.contiguous(),
-        None if bias is None else bias.to(weight.dtype).contiguous(), dy,
-        None if initial_state is None else initial_state.contiguous(), act, cu)
+    op = _conv1d_bwd_impl if _plain(x, weight, bias, dy, initial_state, cu) else torch.ops.gdn_b200.causal_conv1d_bwd
+    dx, dw, db, dh = op(x, weight.contiguous(), None if bias is None else bias.to(weight.dtype).contiguous(), dy,
+                        None if initial_state is None else initial_state.contiguous(), act, cu)
     return dx, dw, None if bias is None else db.to(b_dtype), None if initial_state is None else dh
 
 

@@ -148,6 +148,31 @@ def _call(op, impl, *args):
     return impl(*args)
 
 
+def _plain(*tensors):
+    """Whether a call on these tensors (or None) runs eagerly on plain ones:
+    then it may skip the dispatcher, see :func:`_call`."""
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return not torch.compiler.is_compiling()
+
+
+def _addr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(fn, packed, dev):
+    """Calls ``fn(packed args, current stream)`` on the tensors' device."""
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
+
+
 # ---------------------------------------------------------------------------
 # torch.library custom ops (CUDA implementations call the C ABI)
 # ---------------------------------------------------------------------------

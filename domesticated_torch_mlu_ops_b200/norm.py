@@ -9,12 +9,13 @@ ABI); there is no CPU path.  The ops are the ``torch.library`` custom ops
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .gdn import _DT, _call, _cuda, _ptr, _stream
+from .gdn import _DT, _addr, _cuda, _launch, _plain
 
 Tensor = torch.Tensor
 _GATE = {"silu": _lib.GDN_GATE_SILU, "swish": _lib.GDN_GATE_SILU, "sigmoid": _lib.GDN_GATE_SIGMOID}
@@ -45,6 +46,9 @@ def _row_strides(t):
 
 def _two_strides(x, z):
     """Row strides of x and z over one split of the rows into tokens x heads."""
+    if x.is_contiguous() and (z is None or z.is_contiguous()):
+        D = x.shape[-1]
+        return x, z, 1, D, D, D, D
     x, hx, sxt, sxh = _row_strides(x)
     if z is None:
         return x, None, hx, sxt, sxh, 0, 0
@@ -61,16 +65,6 @@ def _two_strides(x, z):
     return x, z, hx, sxt, sxh, szt, szh
 
 
-def _base_args(x, weight, z, eps, group_size, norm_before_gate, zero_centered, residual_scale, activation):
-    D = x.shape[-1]
-    x, z, heads, sxt, sxh, szt, szh = _two_strides(x, z)
-    return x, z, dict(
-        x=_ptr(x), z=_ptr(z), weight=_ptr(weight), rows=x.numel() // D, heads=heads, D=D,
-        stride_x_token=sxt, stride_x_head=sxh, stride_z_token=szt, stride_z_head=szh, group=group_size,
-        x_dtype=_DT[x.dtype], w_dtype=_DT[weight.dtype], gate_before=int(not norm_before_gate),
-        zero_centered=int(zero_centered), activation=activation, eps=eps, residual_scale=residual_scale)
-
-
 def _empty(dev, dtype):
     return torch.empty(0, dtype=dtype, device=dev)
 
@@ -79,16 +73,20 @@ def _norm_fwd_impl(x: Tensor, weight: Tensor, z: Optional[Tensor], residual: Opt
                    group_size: int, norm_before_gate: bool, zero_centered: bool, residual_scale: float,
                    activation: int) -> tuple[Tensor, Tensor]:
     """Returns ``(y, sum)``; sum is empty without a residual."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = _empty(x.device, x.dtype) if residual is None else torch.empty_like(residual)
+    dev = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    total = _empty(dev, x.dtype) if residual is None else torch.empty_like(residual)
     if x.numel() == 0:
         return y, total
-    x, z, base = _base_args(x, weight, z, eps, group_size, norm_before_gate, zero_centered, residual_scale, activation)
-    args = _lib.NormArgs(
-        y=_ptr(y), residual=_ptr(residual), sum=None if residual is None else _ptr(total), dtype=base["x_dtype"],
-        res_dtype=base["x_dtype"] if residual is None else _DT[residual.dtype], **base)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().gdn_norm_fwd(args, _stream(x.device)))
+    D = x.shape[-1]
+    x, z, heads, sxt, sxh, szt, szh = _two_strides(x, z)
+    dt = _DT[x.dtype]
+    packed = _lib.pack_norm(
+        x.data_ptr(), _addr(z), _addr(residual), weight.data_ptr(), y.data_ptr(),
+        0 if residual is None else total.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, x.numel() // D, heads, D, sxt, sxh, szt, szh,
+        group_size, dt, dt, dt if residual is None else _DT[residual.dtype], _DT[weight.dtype], not norm_before_gate,
+        zero_centered, activation, eps, residual_scale)
+    _launch(_lib.load().gdn_norm_fwd, packed, dev)
     return y, total
 
 
@@ -100,31 +98,39 @@ def _(x, weight, z, residual, eps, group_size, norm_before_gate, zero_centered, 
     return x.new_empty(x.shape), x.new_empty((0,)) if residual is None else residual.new_empty(residual.shape)
 
 
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace(rows, D, group, dtype, x_dtype):
+    """Bytes of gdn_norm_bwd's workspace: they depend on the shapes alone."""
+    args = _lib.NormArgs(rows=rows, heads=1, D=D, group=group, dtype=dtype, x_dtype=x_dtype, res_dtype=x_dtype)
+    n = _lib.load().gdn_norm_bwd_workspace_size(ctypes.byref(args))
+    if n == 0:
+        _lib.check(_lib.GDN_ERR_INVALID)
+    return n
+
+
 def _norm_bwd_impl(dy: Tensor, x: Tensor, weight: Tensor, z: Optional[Tensor], dsum: Optional[Tensor],
                    want_dresidual: bool, eps: float, group_size: int, norm_before_gate: bool, zero_centered: bool,
                    residual_scale: float, activation: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """Returns ``(dx, dweight, dz, dresidual)``; the last two are empty when
     there is no z or dresidual is not wanted."""
     dev = dy.device
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-    dz = _empty(dev, dy.dtype) if z is None else torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-    dres = torch.empty(dy.shape, dtype=x.dtype, device=dev) if want_dresidual else _empty(dev, x.dtype)
+    dx = torch.empty_like(dy)  # dy is contiguous
+    dz = _empty(dev, dy.dtype) if z is None else torch.empty_like(dy)
+    dres = torch.empty_like(dy, dtype=x.dtype) if want_dresidual else _empty(dev, x.dtype)
     if x.numel() == 0:
         return dx, torch.zeros_like(weight), dz, dres
     dw = torch.empty_like(weight)
-    x, z, base = _base_args(x, weight, z, eps, group_size, norm_before_gate, zero_centered, residual_scale, activation)
-    args = _lib.NormArgs(
-        dy=_ptr(dy), dsum=_ptr(dsum), dx=_ptr(dx), dz=None if z is None else _ptr(dz),
-        dresidual=_ptr(dres) if want_dresidual else None, dweight=_ptr(dw), dtype=_DT[dy.dtype],
-        res_dtype=base["x_dtype"], **base)
-    lib = _lib.load()
-    nbytes = lib.gdn_norm_bwd_workspace_size(args)
-    if nbytes == 0:
-        _lib.check(_lib.GDN_ERR_INVALID)
+    D = x.shape[-1]
+    x, z, heads, sxt, sxh, szt, szh = _two_strides(x, z)
+    dt, xt, rows = _DT[dy.dtype], _DT[x.dtype], x.numel() // D
+    nbytes = _bwd_workspace(rows, D, group_size, dt, xt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ctypes.c_void_p(ws.data_ptr()), nbytes
-    with torch.cuda.device(dev):
-        _lib.check(lib.gdn_norm_bwd(args, _stream(dev)))
+    packed = _lib.pack_norm(
+        x.data_ptr(), _addr(z), 0, weight.data_ptr(), 0, 0, dy.data_ptr(), _addr(dsum), dx.data_ptr(),
+        0 if z is None else dz.data_ptr(), dres.data_ptr() if want_dresidual else 0, dw.data_ptr(), ws.data_ptr(), nbytes,
+        rows, heads, D, sxt, sxh, szt, szh, group_size, dt, xt, xt, _DT[weight.dtype], not norm_before_gate,
+        zero_centered, activation, eps, residual_scale)
+    _launch(_lib.load().gdn_norm_bwd, packed, dev)
     return dx, dw, dz, dres
 
 
@@ -136,6 +142,18 @@ def _(dy, x, weight, z, dsum, want_dresidual, eps, group_size, norm_before_gate,
       activation):
     return (dy.new_empty(dy.shape), weight.new_empty(weight.shape), dy.new_empty((0,) if z is None else dy.shape),
             x.new_empty(dy.shape if want_dresidual else (0,)))
+
+
+def _fwd(x, weight, z, residual, meta):
+    if _plain(x, weight, z, residual):
+        return _norm_fwd_impl(x, weight, z, residual, *meta)
+    return torch.ops.gdn_b200.norm_fwd(x, weight, z, residual, *meta)
+
+
+def _bwd(dy, x, weight, z, dsum, want_dresidual, meta):
+    if _plain(dy, x, weight, z, dsum):
+        return _norm_bwd_impl(dy, x, weight, z, dsum, want_dresidual, *meta)
+    return torch.ops.gdn_b200.norm_bwd(dy, x, weight, z, dsum, want_dresidual, *meta)
 
 
 def _check(name, x, weight, z, residual, group_size, activation):
@@ -169,7 +187,7 @@ class GatedRMSNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, z, residual, meta):
-        y, total = _call(torch.ops.gdn_b200.norm_fwd, _norm_fwd_impl, x, weight, z, residual, *meta)
+        y, total = _fwd(x, weight, z, residual, meta)
         ctx.save_for_backward(x if residual is None else total, weight, z)
         ctx.meta, ctx.has_residual = meta, residual is not None
         return (y, total) if residual is not None else y
@@ -180,8 +198,7 @@ class GatedRMSNormFunction(torch.autograd.Function):
         dtype = z.dtype if z is not None else dy.dtype
         dy = dy.to(dtype).contiguous()
         dsum = None if dsum is None else dsum.contiguous()
-        dx, dw, dz, dres = _call(torch.ops.gdn_b200.norm_bwd, _norm_bwd_impl, dy, x, weight, z, dsum,
-                                 ctx.has_residual, *ctx.meta)
+        dx, dw, dz, dres = _bwd(dy, x, weight, z, dsum, ctx.has_residual, ctx.meta)
         return dx, dw, None if z is None else dz, dres if ctx.has_residual else None, None
 
 
@@ -224,7 +241,7 @@ def gated_rms_norm(
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (z is not None and z.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return GatedRMSNormFunction.apply(x, weight, z, residual, meta)
-    y, total = _call(torch.ops.gdn_b200.norm_fwd, _norm_fwd_impl, x, weight, z, residual, *meta)
+    y, total = _fwd(x, weight, z, residual, meta)
     return y if residual is None else (y, total)
 
 
@@ -258,8 +275,7 @@ def gated_rms_norm_bwd(
         if not has_residual or dresidual.shape != x.shape or dresidual.dtype != x.dtype:
             raise ValueError("gated_rms_norm_bwd: dresidual needs has_residual and must match x in shape and dtype")
         dresidual = dresidual.contiguous()
-    dx, dw, dz, dres = _call(
-        torch.ops.gdn_b200.norm_bwd, _norm_bwd_impl, dy.contiguous(), x, weight.contiguous(), z, dresidual,
-        bool(has_residual), float(eps), group, bool(norm_before_gate), bool(zero_centered),
-        float(residual_scale) if has_residual else 1.0, act)
+    meta = (float(eps), group, bool(norm_before_gate), bool(zero_centered),
+            float(residual_scale) if has_residual else 1.0, act)
+    dx, dw, dz, dres = _bwd(dy.contiguous(), x, weight.contiguous(), z, dresidual, bool(has_residual), meta)
     return dx, dw, None if z is None else dz, dres if has_residual else None

@@ -16,37 +16,39 @@ the cache as mutated).
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .gdn import _DT, _IDT, _call, _cuda, _err_word, _f32, _idx, _ptr, _raise_err_word, _stream
+from .gdn import _DT, _IDT, _addr, _cuda, _err_word, _idx, _launch, _plain, _raise_err_word
 
 Tensor = torch.Tensor
 _INF = float("inf")
 
 
+def _f32(t):
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
+
+
 def _packed_rows(t, tail):
-    """(tensor, distance between token rows) of ``t`` whose last ``tail``
-    dimensions are one packed row: in place when only the token rows are
+    """(tensor, distance between token rows) of ``t`` whose last ``tail`` (1 or
+    2) dimensions are one packed row: in place when only the token rows are
     strided (views of one projection), else a packed copy."""
-    width = 1
-    for n in t.shape[t.dim() - tail:]:
-        width *= n
-    if t.is_contiguous():
-        return t, width
-    want, ok = 1, True
-    for n, st in zip(reversed(t.shape[t.dim() - tail:]), reversed(t.stride()[t.dim() - tail:])):
-        ok = ok and (n == 1 or st == want)
-        want *= n
-    lead = [(n, st) for n, st in zip(t.shape[:t.dim() - tail], t.stride()) if n != 1]
-    if len(lead) == 2 and lead[0][1] == lead[1][0] * lead[1][1]:
-        lead = lead[1:]
-    if ok and not lead:
-        return t, width
-    if ok and len(lead) == 1 and lead[0][1] >= width:
-        return t, lead[0][1]
+    shape, st = t.shape, t.stride()
+    width = shape[-1] if tail == 1 else shape[-1] * shape[-2]
+    # the usual views: one token dimension, or a leading one of size 1
+    if st[-1] == 1 and (tail == 1 or st[-2] == shape[-1]):
+        lead = len(shape) - tail
+        if lead == 1 or shape[0] == 1:
+            row = st[lead - 1]
+            if row >= width:
+                return t, row
+        elif st[0] == shape[1] * st[1] and st[1] >= width:
+            return t, st[1]
     return t.contiguous(), width
 
 
@@ -56,11 +58,21 @@ def _aligned_rows(t, tail):
     the recurrent kernel."""
     t, st = _packed_rows(t, tail)
     if t.data_ptr() % 16 or st * t.element_size() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        st = 1
-        for n in t.shape[t.dim() - tail:]:
-            st *= n
+        t, st = _packed_rows(t.clone(memory_format=torch.contiguous_format), tail)
     return t, st
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(B, T, N, H, P, G, S, dtype, force_generic):
+    """Bytes of gdn_scan_fwd's workspace: they depend on the shapes alone."""
+    args = _lib.ScanArgs(B=B, T=T, N=N, H=H, P=P, G=G, S=S, dtype=dtype, dt_dtype=dtype, stride_x=H * P, stride_z=H * P,
+                         stride_b=G * S, stride_c=G * S, stride_dt=H, force_generic=force_generic)
+    if N != B:
+        args.cu_seqlens, args.cu_dtype = ctypes.c_void_p(16), _lib.GDN_I64  # packed: only whether it is there counts
+    n = _lib.load().gdn_scan_workspace_size(ctypes.byref(args))
+    if n == 0:
+        _lib.check(_lib.GDN_ERR_INVALID)
+    return n
 
 
 def _scan_fwd_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor], z: Optional[Tensor],
@@ -77,25 +89,19 @@ def _scan_fwd_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Op
     z, sz = (None, 0) if z is None else rows(z, 2)
     y = torch.empty((Bt, T, H, P), dtype=x.dtype, device=dev)
     fin = torch.empty((N, H, P, S) if output_final_state else (0,), dtype=state_dtype, device=dev)
-    args = _lib.ScanArgs(
-        x=_ptr(x), dt=_ptr(dt), A=_ptr(A), b=_ptr(B), c=_ptr(C), D=_ptr(D), z=_ptr(z), dt_bias=_ptr(dt_bias),
-        initial_state=_ptr(initial_state), y=_ptr(y), final_state=_ptr(fin) if output_final_state else None,
-        cu_seqlens=_ptr(cu_seqlens), B=Bt, T=T, N=N, stride_x=sx, stride_dt=sdt, stride_b=sb, stride_c=sc, stride_z=sz,
-        H=H, P=P, G=G, S=S, dtype=_DT[x.dtype], dt_dtype=_DT[dt.dtype],
-        init_dtype=_DT[initial_state.dtype] if initial_state is not None else _lib.GDN_F32,
-        final_dtype=_DT[state_dtype], cu_dtype=_IDT[cu_seqlens.dtype] if cu_seqlens is not None else _lib.GDN_I64,
-        dt_softplus=int(dt_softplus), force_generic=int(force_generic), dt_min=dt_min, dt_max=dt_max)
-    lib = _lib.load()
-    nbytes = lib.gdn_scan_workspace_size(args)
-    if nbytes == 0:
-        _lib.check(_lib.GDN_ERR_INVALID)
+    dtype, dt_dtype = _DT[x.dtype], _DT[dt.dtype]
+    nbytes = _workspace(Bt, T, N, H, P, G, S, dtype, force_generic)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ctypes.c_void_p(ws.data_ptr()), nbytes
-    with torch.cuda.device(dev):
-        stream = _stream(dev)
-        _lib.check(lib.gdn_scan_fwd(args, stream))
-        if check_errors:
-            _lib.check(lib.gdn_chunk_check_device_error(args.workspace, stream))
+    packed = _lib.pack_scan(
+        x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _addr(D), _addr(z), _addr(dt_bias),
+        _addr(initial_state), y.data_ptr(), fin.data_ptr() if output_final_state else 0, _addr(cu_seqlens), ws.data_ptr(),
+        nbytes, Bt, T, N, sx, sdt, sb, sc, sz, H, P, G, S, dtype, dt_dtype,
+        _lib.GDN_F32 if initial_state is None else _DT[initial_state.dtype], _DT[state_dtype],
+        _lib.GDN_I64 if cu_seqlens is None else _IDT[cu_seqlens.dtype], dt_softplus, force_generic, dt_min, dt_max)
+    lib = _lib.load()
+    _launch(lib.gdn_scan_fwd, packed, dev)
+    if check_errors:
+        _launch(lib.gdn_chunk_check_device_error, ws.data_ptr(), dev)
     return y, fin
 
 
@@ -123,18 +129,15 @@ def _scan_update_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
     if N == 0:
         return y
     err = _err_word(dev)
-    args = _lib.ScanUpdateArgs(
-        x=_ptr(x), dt=_ptr(dt), A=_ptr(A), b=_ptr(B), c=_ptr(C), D=_ptr(D), z=_ptr(z), dt_bias=_ptr(dt_bias),
-        state=_ptr(state), y=_ptr(y), ssm_state_indices=_ptr(ssm_state_indices), err=_ptr(err),
-        N=N, num_slots=state.shape[0], stride_slot=state.stride(0) if state.shape[0] > 1 else H * P * S,
-        stride_x=sx, stride_dt=sdt, stride_b=sb, stride_c=sc, stride_z=sz, H=H, P=P, G=G, S=S, dtype=_DT[x.dtype],
-        dt_dtype=_DT[dt.dtype], state_dtype=_DT[state.dtype],
-        idx_dtype=_IDT[ssm_state_indices.dtype] if ssm_state_indices is not None else _lib.GDN_I64,
-        dt_softplus=int(dt_softplus), dt_min=dt_min, dt_max=dt_max)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().gdn_scan_update(args, _stream(dev)))
-        if check_errors:
-            _raise_err_word(err)
+    packed = _lib.pack_scan_update(
+        x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _addr(D), _addr(z), _addr(dt_bias),
+        state.data_ptr(), y.data_ptr(), _addr(ssm_state_indices), err.data_ptr(), N, state.shape[0],
+        state.stride(0) if state.shape[0] > 1 else H * P * S, sx, sdt, sb, sc, sz, H, P, G, S, _DT[x.dtype], _DT[dt.dtype],
+        _DT[state.dtype], _lib.GDN_I64 if ssm_state_indices is None else _IDT[ssm_state_indices.dtype], dt_softplus,
+        dt_min, dt_max)
+    _launch(_lib.load().gdn_scan_update, packed, dev)
+    if check_errors:
+        _raise_err_word(err)
     return y
 
 
@@ -148,21 +151,22 @@ def _(x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, state, ssm_sta
 
 
 def _check(name, lead, x, dt, A, B, C, D, z, dt_bias, dt_limit):
-    H, P = x.shape[-2:]
-    if x.dtype not in _DT:
-        raise ValueError(f"{name}: x dtype {x.dtype} must be float32, bfloat16 or float16")
-    if B.dim() != x.dim() or B.shape != C.shape or B.shape[:-2] != x.shape[:-2]:
+    shape, dtype = x.shape, x.dtype
+    H = shape[-2]
+    if dtype not in _DT:
+        raise ValueError(f"{name}: x dtype {dtype} must be float32, bfloat16 or float16")
+    if B.dim() != x.dim() or B.shape != C.shape or B.shape[:-2] != shape[:-2]:
         raise ValueError(f"{name}: B {tuple(B.shape)} and C {tuple(C.shape)} must be [{lead}, G, S]")
     if B.shape[-2] == 0 or H % B.shape[-2] != 0:
         raise ValueError(f"{name}: {H} heads are no multiple of {B.shape[-2]} groups")
-    if B.dtype != x.dtype or C.dtype != x.dtype or (z is not None and z.dtype != x.dtype):
+    if B.dtype is not dtype or C.dtype is not dtype or (z is not None and z.dtype is not dtype):
         raise ValueError(f"{name}: x, B, C and z must share a dtype")
-    if z is not None and z.shape != x.shape:
-        raise ValueError(f"{name}: z {tuple(z.shape)} must match x {tuple(x.shape)}")
-    if dt.shape != x.shape[:-1] or dt.dtype not in _DT:
-        raise ValueError(f"{name}: dt {tuple(dt.shape)} {dt.dtype} must be {tuple(x.shape[:-1])} of a float type")
+    if z is not None and z.shape != shape:
+        raise ValueError(f"{name}: z {tuple(z.shape)} must match x {tuple(shape)}")
+    if dt.shape != shape[:-1] or dt.dtype not in _DT:
+        raise ValueError(f"{name}: dt {tuple(dt.shape)} {dt.dtype} must be {tuple(shape[:-1])} of a float type")
     for what, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-        if t is not None and tuple(t.shape) != (H,):
+        if t is not None and (t.dim() != 1 or t.shape[0] != H):
             raise ValueError(f"{name}: {what} {tuple(t.shape)} must be ({H},), one value per head")
     lo, hi = float(dt_limit[0]), float(dt_limit[1])
     if not lo <= hi:
@@ -227,9 +231,9 @@ def chunk_selective_scan(
             raise ValueError(f"initial_state must be {shape} of a float type, got {tuple(initial_state.shape)} "
                              f"{initial_state.dtype}")
         initial_state = initial_state.contiguous()
-    y, fin = _call(torch.ops.gdn_b200.scan_fwd, _scan_fwd_impl, x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias),
-                   bool(dt_softplus), lo, hi, initial_state, bool(output_final_state), state_dtype, cu,
-                   bool(force_generic), bool(check_errors))
+    op = (_scan_fwd_impl if _plain(x, dt, A, B, C, D, z, dt_bias, initial_state, cu) else torch.ops.gdn_b200.scan_fwd)
+    y, fin = op(x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias), bool(dt_softplus), lo, hi, initial_state,
+                bool(output_final_state), state_dtype, cu, bool(force_generic), bool(check_errors))
     return y, (fin if output_final_state else None)
 
 
@@ -286,6 +290,6 @@ def selective_scan_update(
         if tuple(idx.shape) != (N,):
             raise ValueError(f"selective_scan_update: ssm_state_indices {tuple(idx.shape)} must be ({N},)")
         idx = _idx(idx)[0].contiguous()
-    y = _call(torch.ops.gdn_b200.scan_update, _scan_update_impl, x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias),
-              bool(dt_softplus), lo, hi, state, idx, bool(check_errors))
+    op = _scan_update_impl if _plain(x, dt, A, B, C, D, z, dt_bias, state, idx) else torch.ops.gdn_b200.scan_update
+    y = op(x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias), bool(dt_softplus), lo, hi, state, idx, bool(check_errors))
     return y, state
