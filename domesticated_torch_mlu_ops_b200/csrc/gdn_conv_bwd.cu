@@ -17,6 +17,7 @@
 #include "conv_math.cuh"
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
+#include "packed2.cuh"
 
 #include <algorithm>
 
@@ -27,6 +28,13 @@ using namespace conv;
 
 constexpr int kMinRun = 64;  // tokens per run, at least
 constexpr int kThreads = 128;
+// A thread's vector in bytes, CTAs per SM, and tokens whose loads are in
+// flight together at W = 4.  Measured at 8192 tokens x 8192 bf16 channels
+// (403 MB): 89 us, 4.5 TB/s, 69 % of a plain copy's rate.  The fp32 pipe and
+// the two special functions per element set the pace, not the loads: copying
+// the blocks through shared memory (cp.async, 15 tokens ahead) took 90 us,
+// 16-byte vectors 91 us, five CTAs per SM 113 us, 4-byte vectors 154 us.
+constexpr int kVecBytes = 8, kResident = 4, kBlock4 = 6;
 constexpr int kMaxW = 16;
 
 struct BwdParams {
@@ -45,20 +53,15 @@ struct BwdParams {
   int W, w_dtype, init_dtype, cu_dtype, act;
 };
 
-// dpre from pre and dy, with the hardware exponential and divide (a few fp32
-// ulp: dw and db may be fp32 sums of these).
-__device__ __forceinline__ float silu_grad(float p, float dy) {
-  const float s = __fdividef(1.f, 1.f + __expf(-p));
-  return dy * s * fmaf(p, 1.f - s, 1.f);
-}
-
-template <typename T, int VEC, int KW>
+template <int VEC, int KW, typename T>
 struct GradLane {
+  using V = pk::Vec<VEC>;
   static constexpr int WM = KW > 0 ? KW : kMaxW;
-  float w[WM][VEC], bias[VEC];
-  float win[WM][VEC];   // win[j] = input at token t - (W-1) + j, j < W-1
-  float pend[WM][VEC];  // pend[j] = dx so far of token t - (W-1) + j, j < W-1
-  float dw[WM][VEC], db[VEC];
+  static constexpr int WP = WM > 1 ? WM - 1 : 1;
+  V w[WM], bias;
+  V win[WP];   // win[j] = input at token t - (W-1) + j, j < W-1
+  V pend[WP];  // pend[j] = dx so far of token t - (W-1) + j, j < W-1
+  V dw[WM], db;
   int w_rt;
   int64_t c;
 
@@ -69,93 +72,73 @@ struct GradLane {
     c = c_;
     const int W = width();
 #pragma unroll
-    for (int i = 0; i < WM; ++i)
+    for (int i = 0; i < WM; ++i) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        w[i][e] = i < W ? ld_any(p.weight, p.w_dtype, (c + e) * W + i) : 0.f;
-        dw[i][e] = 0.f;
-      }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      bias[e] = p.bias ? ld_any(p.bias, p.w_dtype, c + e) : 0.f;
-      db[e] = 0.f;
+      for (int e = 0; e < VEC; ++e) pk::set(w[i], e, i < W ? ld_any(p.weight, p.w_dtype, (c + e) * W + i) : 0.f);
+      dw[i] = pk::splat<VEC>(0.f);
     }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) pk::set(bias, e, p.bias ? ld_any(p.bias, p.w_dtype, c + e) : 0.f);
+    db = pk::splat<VEC>(0.f);
   }
 
   // The window before token t of sequence n = [bos, ...), nothing pending.
   __device__ __forceinline__ void enter(const BwdParams& p, int64_t t, int64_t n, int64_t bos) {
     const int W = width();
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j) {
-      if (j >= W - 1) break;
+    for (int j = 0; j < WP; ++j) {
+      pend[j] = pk::splat<VEC>(0.f);
+      win[j] = pk::splat<VEC>(0.f);
+      if (j >= W - 1) continue;
       const int64_t u = t - (W - 1) + j;
       if (u >= bos) {
-        ldv<T, VEC>(static_cast<const T*>(p.x) + u * p.sx + c, win[j]);
-      } else {
+        pk::Raw<T, VEC> r;
+        pk::load(r, static_cast<const T*>(p.x) + u * p.sx + c);
+        win[j] = pk::widen<T, VEC>(r);
+      } else if (p.init) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          win[j][e] = p.init ? ld_any(p.init, p.init_dtype, (n * p.D + c + e) * W + (u - bos) + W) : 0.f;
+          pk::set(win[j], e, ld_any(p.init, p.init_dtype, (n * p.D + c + e) * W + (u - bos) + W));
       }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) pend[j][e] = 0.f;
     }
   }
 
-  // One token: dpre, its share of dw and db (when `count`), and of the W
-  // gradients it reaches; leaves the finished one (token t - (W-1)) in `out`.
-  __device__ __forceinline__ void step(const BwdParams& p, const float* xv, const float* dyv, bool count, float* out) {
+  // One token: dpre = dy s (1 + pre (1 - s)) with s = sigmoid(pre), its share
+  // of dw and db (when `count`), and of the W gradients it reaches; returns
+  // the finished one (token t - (W-1)).
+  __device__ __forceinline__ V step(const BwdParams& p, const V& xv, const V& dyv, bool count) {
     const int W = width();
-    float d[VEC];
+    V d = dyv;
     if (p.act == GDN_ACT_SILU) {
-      float pre[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) pre[e] = bias[e];
+      V pre = bias;
 #pragma unroll
       for (int j = 0; j < WM - 1; ++j)
-        if (j < W - 1) fma_vec<VEC>(pre, w[j], win[j]);
-      fma_vec<VEC>(pre, w[W - 1], xv);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) d[e] = silu_grad(pre[e], dyv[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) d[e] = dyv[e];
+        if (j < W - 1) pre = pk::fma(w[j], win[j], pre);
+      pre = pk::fma(w[W - 1], xv, pre);
+      const V s = pk::sigmoid(pre), one = pk::splat<VEC>(1.f);
+      const V r = pk::fma(s, pk::splat<VEC>(-1.f), one);
+      d = pk::mul(pk::mul(dyv, s), pk::fma(pre, r, one));
     }
     if (count) {
 #pragma unroll
       for (int j = 0; j < WM - 1; ++j)
-        if (j < W - 1) fma_vec<VEC>(dw[j], d, win[j]);
-      fma_vec<VEC>(dw[W - 1], d, xv);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) db[e] += d[e];
+        if (j < W - 1) dw[j] = pk::fma(d, win[j], dw[j]);
+      dw[W - 1] = pk::fma(d, xv, dw[W - 1]);
+      db = pk::add(db, d);
     }
+    V last = pk::mul(w[W - 1], d), out = last;
+    if (W >= 2) {
+      out = pk::fma(w[0], d, pend[0]);
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j)
-      if (j < W - 1) fma_vec<VEC>(pend[j], w[j], d);
-    float last[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      last[e] = w[W - 1][e] * d[e];
-      out[e] = W >= 2 ? pend[0][e] : last[e];
-    }
-    shift(last, xv);
-  }
-
-  __device__ __forceinline__ void shift(const float* last, const float* xv) {
-    const int W = width();
-#pragma unroll
-    for (int j = 0; j + 1 < WM - 1; ++j)
-      if (j + 1 < W - 1)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          win[j][e] = win[j + 1][e];
-          pend[j][e] = pend[j + 1][e];
+      for (int j = 0; j + 1 < WM - 1; ++j)
+        if (j + 1 < W - 1) {
+          pend[j] = pk::fma(w[j + 1], d, pend[j + 1]);
+          win[j] = win[j + 1];
         }
-    if (W >= 2)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        win[W - 2][e] = xv[e];
-        pend[W - 2][e] = last[e];
-      }
+      win[W - 2] = xv;
+      pend[W - 2] = last;
+    }
+    return out;
   }
 };
 
@@ -163,25 +146,29 @@ struct GradLane {
 // sequence start, and the start in this run) a column of dinit.
 template <typename T, int VEC>
 __device__ __forceinline__ void emit(const BwdParams& p, int64_t s, int64_t t0, int64_t t1, int64_t n, int64_t bos,
-                                     int64_t c, int W, const float* v) {
+                                     int64_t c, int W, const pk::Vec<VEC>& v) {
   if (s >= bos) {
-    if (s >= t0 && s < t1) stv<T, VEC>(static_cast<T*>(p.dx) + s * p.D + c, v);
+    if (s >= t0 && s < t1) pk::store<T, VEC>(static_cast<T*>(p.dx) + s * p.D + c, v);
   } else if (bos >= t0 && p.dinit) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) st_any(p.dinit, p.init_dtype, (n * p.D + c + e) * W + (s - bos) + W, v[e]);
+    for (int e = 0; e < VEC; ++e) st_any(p.dinit, p.init_dtype, (n * p.D + c + e) * W + (s - bos) + W, pk::get(v, e));
   }
 }
 
+// U tokens per block, a multiple of W-1 where W is known: the window and the
+// pending gradients rotate through their registers and are back in place at a
+// block's end, without moves.
 template <typename T, int VEC, int KW>
-__global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const BwdParams p) {
-  constexpr int U = 4;  // tokens whose loads are in flight together
+__global__ void __launch_bounds__(kThreads, VEC > 1 && KW > 0 ? kResident : 1) conv_bwd_kernel(const BwdParams p) {
+  constexpr int U = KW == 4 ? kBlock4 : 4;
+  using V = pk::Vec<VEC>;
   const int64_t cb = blockIdx.x % p.nblk, share = blockIdx.x / p.nblk;
   const int64_t t0 = share * p.run, t1 = min64(p.total, t0 + p.run);
   const int64_t c = (cb * kThreads + threadIdx.x) * VEC;
   if (c >= p.D) return;
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.dy);
-  GradLane<T, VEC, KW> L;
+  GradLane<VEC, KW, T> L;
   L.init(p, c);
   const int W = L.width();
   int64_t n, bos, eos;
@@ -207,59 +194,65 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const BwdParams p) {
       eos = p.cu ? min64(load_index(p.cu, p.cu_dtype, n + 1), p.total) : bos + p.T;
     }
     if (t < bos || t >= eos) {  // a token outside every sequence reaches no output
-      const float zero[VEC] = {};
-      stv<T, VEC>(static_cast<T*>(p.dx) + t * p.D + c, zero);
+      pk::store<T, VEC>(static_cast<T*>(p.dx) + t * p.D + c, pk::splat<VEC>(0.f));
       ++t;
       continue;
     }
     L.enter(p, t, n, bos);
     const int64_t from = t, stop = min64(eos, t1 + W - 1);
-    float xv[VEC], dv[VEC], out[VEC];
+    // a block's loads are issued before the block ahead of it is computed
+    pk::Raw<T, VEC> rx[U], rd[U];
+    auto load = [&](int64_t at) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int64_t u = min64(at + k, stop - 1);
+        pk::load(rx[k], x + u * p.sx + c);
+        pk::load(rd[k], dy + u * p.sdy + c);
+      }
+    };
+    load(t);
     while (t < stop) {
+      pk::Raw<T, VEC> cx[U], cd[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        cx[k] = rx[k];
+        cd[k] = rd[k];
+      }
+      if (t + U < stop) load(t + U);
       if (t + U <= min64(stop, t1) && t - (W - 1) >= from) {
         // inside the run: every finished gradient is this run's own
-        using Raw = typename std::conditional<VEC * sizeof(T) == 16, uint4,
-                    typename std::conditional<VEC * sizeof(T) == 8, uint2,
-                    typename std::conditional<VEC * sizeof(T) == 4, uint32_t, uint16_t>::type>::type>::type;
-        Raw rx[U], rd[U];
+        T* out = static_cast<T*>(p.dx) + (t - (W - 1)) * p.D + c;
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-          rx[k] = __ldg(reinterpret_cast<const Raw*>(x + (t + k) * p.sx + c));
-          rd[k] = __ldg(reinterpret_cast<const Raw*>(dy + (t + k) * p.sdy + c));
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            xv[e] = to_f<T>(reinterpret_cast<const T*>(&rx[k])[e]);
-            dv[e] = to_f<T>(reinterpret_cast<const T*>(&rd[k])[e]);
-          }
-          L.step(p, xv, dv, true, out);
-          stv<T, VEC>(static_cast<T*>(p.dx) + (t + k - (W - 1)) * p.D + c, out);
+          pk::store<T, VEC>(out, L.step(p, pk::widen<T, VEC>(cx[k]), pk::widen<T, VEC>(cd[k]), true));
+          out += p.D;
         }
         t += U;
       } else {
-        ldv<T, VEC>(x + t * p.sx + c, xv);
-        ldv<T, VEC>(dy + t * p.sdy + c, dv);
-        L.step(p, xv, dv, t < t1, out);
-        emit<T, VEC>(p, t - (W - 1), t0, t1, n, bos, c, W, out);
-        ++t;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (t < stop) {
+            const V out = L.step(p, pk::widen<T, VEC>(cx[k]), pk::widen<T, VEC>(cd[k]), t < t1);
+            emit<T, VEC>(p, t - (W - 1), t0, t1, n, bos, c, W, out);
+            ++t;
+          }
+        }
       }
     }
     if (stop == eos) {  // the sequence's last W-1 gradients have no later terms
 #pragma unroll
-      for (int j = 0; j < GradLane<T, VEC, KW>::WM - 1; ++j)
+      for (int j = 0; j < GradLane<VEC, KW, T>::WP; ++j)
         if (j < W - 1) emit<T, VEC>(p, eos - (W - 1) + j, t0, t1, n, bos, c, W, L.pend[j]);
     }
   }
   float* out = p.partial + share * (W + 1) * p.D + c;
 #pragma unroll
-  for (int i = 0; i < GradLane<T, VEC, KW>::WM; ++i)
+  for (int i = 0; i < GradLane<VEC, KW, T>::WM; ++i)
     if (i < W)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) out[i * p.D + e] = L.dw[i][e];
+      for (int e = 0; e < VEC; ++e) out[i * p.D + e] = pk::get(L.dw[i], e);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) out[W * p.D + e] = L.db[e];
+  for (int e = 0; e < VEC; ++e) out[W * p.D + e] = pk::get(L.db, e);
 }
 
 // dw[c][i], db[c] = sum over the runs, in order: eight lanes of runs per
@@ -289,21 +282,21 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 // it, else one.  Wider vectors need more registers for the window, the
 // pending gradients and dw than they save in loads.
 int vec_of(const gdn_conv1d_bwd_args& a) {
-  const int es = a.x_dtype == GDN_F32 ? 4 : 2, v = 8 / es;
-  const bool ok = a.D % v == 0 && a.stride_x_token % v == 0 && a.stride_dy_token % v == 0 && aligned(a.x, 8) &&
-                  aligned(a.dy, 8) && aligned(a.dx, 8);
+  const int es = a.x_dtype == GDN_F32 ? 4 : 2, v = kVecBytes / es;
+  const bool ok = a.D % v == 0 && a.stride_x_token % v == 0 && a.stride_dy_token % v == 0 && aligned(a.x, kVecBytes) &&
+                  aligned(a.dy, kVecBytes) && aligned(a.dx, kVecBytes);
   return ok ? v : 1;
 }
 
 struct Split {
   int64_t nblk, run, shares;
 };
-// Equal runs of at least kMinRun tokens, about six CTAs per SM (888 on 148):
+// Equal runs of at least kMinRun tokens, kResident CTAs per SM of 148:
 // the same on every device, so the sums' order is too.
 Split split_of(int64_t total, int64_t D, int vec) {
   Split s;
   s.nblk = (D + vec * kThreads - 1) / (vec * kThreads);
-  s.shares = std::max<int64_t>(1, std::min<int64_t>(888 / s.nblk, (total + kMinRun - 1) / kMinRun));
+  s.shares = std::max<int64_t>(1, std::min<int64_t>(148 * kResident / s.nblk, (total + kMinRun - 1) / kMinRun));
   s.run = std::max<int64_t>(1, (total + s.shares - 1) / s.shares);
   s.shares = std::max<int64_t>(1, (total + s.run - 1) / s.run);
   return s;
@@ -350,7 +343,7 @@ void launch_w(const BwdParams& p, cudaStream_t s) {
 
 template <typename T>
 void launch(const BwdParams& p, int vec, cudaStream_t s) {
-  if (vec > 1) launch_w<T, 8 / sizeof(T)>(p, s);
+  if (vec > 1) launch_w<T, kVecBytes / sizeof(T)>(p, s);
   else launch_w<T, 1>(p, s);
 }
 
@@ -365,7 +358,7 @@ extern "C" GDN_API size_t gdn_causal_conv1d_bwd_workspace_size(const gdn_conv1d_
   if (convb::check(a)) return 0;
   const int es = a->x_dtype == GDN_F32 ? 4 : 2;
   const int64_t total = a->B * a->T;
-  const int64_t shares = std::max(convb::split_of(total, a->D, 8 / es).shares, convb::split_of(total, a->D, 1).shares);
+  const int64_t shares = std::max(convb::split_of(total, a->D, convb::kVecBytes / es).shares, convb::split_of(total, a->D, 1).shares);
   return static_cast<size_t>(shares) * (a->W + 1) * a->D * sizeof(float);
 }
 

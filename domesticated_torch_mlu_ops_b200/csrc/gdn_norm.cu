@@ -20,6 +20,7 @@
 #include "conv_math.cuh"
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
+#include "packed2.cuh"
 
 #include <algorithm>
 
@@ -27,9 +28,7 @@ namespace gdn {
 namespace norm {
 
 using conv::ld_any;
-using conv::ldv;
 using conv::st_any;
-using conv::stv;
 
 struct Params {
   const void* x;  // forward: T; backward: X
@@ -41,79 +40,45 @@ struct Params {
   const void *dy, *dsum;
   void *dx, *dz, *dresidual;
   float* partial;  // [gridDim.x][D]
-  int64_t rows, heads, D;
+  int64_t D;
   int64_t sx_tok, sx_head, sz_tok, sz_head;  // row (t, h) of x and z, in elements
+  int rows, heads;
   int group;
   int w_dtype, res_f32, gate_before, sigmoid_gate;
   float eps, alpha, w_off;
 };
 
-// act(z) and act'(z), with the hardware exponential and divide.
-__device__ __forceinline__ float gate(float z, int sigmoid_gate) {
-  const float s = __fdividef(1.f, 1.f + __expf(-z));
-  return sigmoid_gate ? s : z * s;
+// act(z) from z and sigmoid(z), and act'(z).
+template <int VEC>
+__device__ __forceinline__ pk::Vec<VEC> gate(const pk::Vec<VEC>& z, const pk::Vec<VEC>& s, int sigmoid_gate) {
+  return sigmoid_gate ? s : pk::mul(z, s);
 }
-__device__ __forceinline__ void gate_grad(float z, int sigmoid_gate, float& a, float& da) {
-  const float s = __fdividef(1.f, 1.f + __expf(-z));
-  a = sigmoid_gate ? s : z * s;
-  da = sigmoid_gate ? s * (1.f - s) : s * fmaf(z, 1.f - s, 1.f);
+template <int VEC>
+__device__ __forceinline__ pk::Vec<VEC> gate_grad(const pk::Vec<VEC>& s, const pk::Vec<VEC>& a, int sigmoid_gate) {
+  // silu: s + a (1 - s);  sigmoid: s (1 - s)
+  const pk::Vec<VEC> r = pk::fma(s, pk::splat<VEC>(-1.f), pk::splat<VEC>(1.f));
+  return sigmoid_gate ? pk::mul(s, r) : pk::fma(a, r, s);
 }
 
-// VEC values as floats from T or fp32 rows (fp32 vectors of 8 as two 16-byte loads).
 template <int VEC>
-__device__ __forceinline__ void ldf(const float* p, float* v) {
-  if constexpr (VEC % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
-      v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = __ldg(p + i);
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void stf(float* p, const float* v) {
-  if constexpr (VEC % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) p[i] = v[i];
-  }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void ld_res(const void* p, int f32, int64_t i, float* v) {
-  if (f32) ldf<VEC>(static_cast<const float*>(p) + i, v);
-  else ldv<T, VEC>(static_cast<const T*>(p) + i, v);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void st_res(void* p, int f32, int64_t i, const float* v) {
-  if (f32) stf<VEC>(static_cast<float*>(p) + i, v);
-  else stv<T, VEC>(static_cast<T*>(p) + i, v);
-}
-template <int VEC>
-__device__ __forceinline__ void ld_weight(const Params& p, int64_t i, float* w) {
+__device__ __forceinline__ pk::Vec<VEC> ld_weight(const Params& p, int64_t i) {
+  pk::Vec<VEC> w;
   if (VEC > 1 && p.w_dtype == GDN_F32) {
-    ldf<VEC>(static_cast<const float*>(p.weight) + i, w);
+    pk::Raw<float, VEC> r;
+    pk::load(r, static_cast<const float*>(p.weight) + i);
+    w = pk::widen<float, VEC>(r);
   } else if (VEC > 1 && p.w_dtype == GDN_BF16) {
-#pragma unroll
-    for (int e = 0; e < VEC; e += 4) {
-      const float4 f = load4(static_cast<const __nv_bfloat16*>(p.weight) + i + e);
-      w[e] = f.x; w[e + 1] = f.y; w[e + 2] = f.z; w[e + 3] = f.w;
-    }
+    pk::Raw<__nv_bfloat16, VEC> r;
+    pk::load(r, static_cast<const __nv_bfloat16*>(p.weight) + i);
+    w = pk::widen<__nv_bfloat16, VEC>(r);
   } else if (VEC > 1) {
-#pragma unroll
-    for (int e = 0; e < VEC; e += 4) {
-      const float4 f = load4(static_cast<const __half*>(p.weight) + i + e);
-      w[e] = f.x; w[e + 1] = f.y; w[e + 2] = f.z; w[e + 3] = f.w;
-    }
+    pk::Raw<__half, VEC> r;
+    pk::load(r, static_cast<const __half*>(p.weight) + i);
+    w = pk::widen<__half, VEC>(r);
   } else {
-    w[0] = ld_any(p.weight, p.w_dtype, i);
+    pk::set(w, 0, ld_any(p.weight, p.w_dtype, i));
   }
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) w[e] += p.w_off;
+  return pk::add(w, pk::splat<VEC>(p.w_off));
 }
 
 // Sum over the team: TS lanes of a warp, or (TS = 0) the CTA; `buf` holds
@@ -140,194 +105,225 @@ __device__ __forceinline__ void team_sum(float* v, float (*buf)[32]) {
   }
 }
 
-// One team per (row, group).  TS = 0: the CTA.
-template <typename T, int VEC, int ITER, int TS, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const Params p) {
-  __shared__ float buf[1][32];
-  const int ts = TS ? TS : blockDim.x;
-  const int lane = TS ? threadIdx.x % TS : threadIdx.x;
-  const int64_t teams = blockDim.x / ts;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * teams + (TS ? threadIdx.x / TS : 0);
-  const int64_t g0 = static_cast<int64_t>(blockIdx.y) * p.group;
-  const bool live = row < p.rows;  // every lane stays for the shuffles
-  const int64_t tok = live ? row / p.heads : 0, head = live ? row - tok * p.heads : 0;
-  const T* x = static_cast<const T*>(p.x) + tok * p.sx_tok + head * p.sx_head + g0;
-  const T* z = p.z ? static_cast<const T*>(p.z) + tok * p.sz_tok + head * p.sz_head + g0 : nullptr;
-  float u[ITER][VEC], a[ITER][VEC];
-  float ss[1] = {0.f};
-#pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const int i = (k * ts + lane) * VEC;
-    const bool in = live && i < p.group;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      u[k][e] = 0.f;
-      a[k][e] = 0.f;
-    }
-    if (in) {
-      ldv<T, VEC>(x + i, u[k]);
-      if (z) ldv<T, VEC>(z + i, a[k]);
-      if (p.residual) {
-        float r[VEC];
-        ld_res<T, VEC>(p.residual, p.res_f32, row * p.D + g0 + i, r);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) u[k][e] = fmaf(p.alpha, u[k][e], r[e]);
-      }
-    }
+// A thread's place in its team, and where its vectors are in a row's group.
+// Vectors past the group's end are loaded from its first one and count as 0.
+template <int VEC, int ITER, int TS>
+struct Team {
+  int ts, lane, team, teams, group;
+  bool full;  // every vector of every lane lies in the group
+  __device__ __forceinline__ explicit Team(int group_) : group(group_) {
+    ts = TS ? TS : blockDim.x;
+    lane = TS ? threadIdx.x % (TS ? TS : 1) : threadIdx.x;
+    team = TS ? threadIdx.x / (TS ? TS : 1) : 0;
+    teams = TS ? blockDim.x / (TS ? TS : 1) : 1;
+    full = group == ts * ITER * VEC;
   }
-#pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const int i = (k * ts + lane) * VEC;
-    if (p.sum && live && i < p.group) st_res<T, VEC>(p.sum, p.res_f32, row * p.D + g0 + i, u[k]);
-    if (z)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        a[k][e] = gate(a[k][e], p.sigmoid_gate);
-        if (p.gate_before) u[k][e] = i < p.group ? u[k][e] * a[k][e] : 0.f;
-      }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) ss[0] = fmaf(u[k][e], u[k][e], ss[0]);
-  }
-  team_sum<TS, 1>(ss, buf);
-  const float rstd = rsqrtf(ss[0] / static_cast<float>(p.group) + p.eps);
-  if (!live) return;
-  const bool after = z && !p.gate_before;
-#pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const int i = (k * ts + lane) * VEC;
-    if (i >= p.group) break;
-    float w[VEC];
-    ld_weight<VEC>(p, g0 + i, w);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      u[k][e] = u[k][e] * rstd * w[e];
-      if (after) u[k][e] *= a[k][e];
-    }
-    stv<T, VEC>(static_cast<T*>(p.y) + row * p.D + g0 + i, u[k]);
+  __device__ __forceinline__ int col(int k) const { return (k * ts + lane) * VEC; }
+  __device__ __forceinline__ bool in(int k) const { return full || col(k) < group; }
+  __device__ __forceinline__ int at(int k) const { return in(k) ? col(k) : 0; }
+};
+
+__device__ __forceinline__ void row_of(const Params& p, int row, int64_t& x_at, int64_t& z_at) {
+  if (p.heads == 1) {
+    x_at = row * p.sx_tok;
+    z_at = row * p.sz_tok;
+  } else {
+    const unsigned t = static_cast<unsigned>(row) / static_cast<unsigned>(p.heads);
+    const int64_t h = row - static_cast<int>(t * p.heads);
+    x_at = t * p.sx_tok + h * p.sx_head;
+    z_at = t * p.sz_tok + h * p.sz_head;
   }
 }
 
-// X: the type of x (the residual's when the forward summed one).  A team
-// walks rows blockIdx.x * teams + team, + gridDim.x * teams, ...
-template <typename T, typename X, int VEC, int ITER, int TS, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const Params p) {
-  extern __shared__ float dws[];  // [teams][group] when teams > 1
-  __shared__ float buf[2][2][32];
-  const int ts = TS ? TS : blockDim.x;
-  const int lane = TS ? threadIdx.x % TS : threadIdx.x;
-  const int team = TS ? threadIdx.x / TS : 0;
-  const int64_t teams = blockDim.x / ts;
+// Rows blockIdx.x * teams + team, + gridDim.x * teams, ...: the next row's
+// loads are issued before this one is computed.  R: the residual's type, or
+// void without one.
+template <typename T, typename R, int VEC, int ITER, int TS, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const Params p) {
+  using V = pk::Vec<VEC>;
+  constexpr bool kAhead = MAXT <= 256;  // larger CTAs have no registers for the next row
+  constexpr bool kRes = !std::is_void<R>::value;
+  using RT = typename std::conditional<kRes, R, T>::type;
+  __shared__ float buf[2][1][32];
+  const Team<VEC, ITER, TS> tm(p.group);
   const int64_t g0 = static_cast<int64_t>(blockIdx.y) * p.group;
   const float inv = 1.f / static_cast<float>(p.group);
-  float w[ITER][VEC], dw[ITER][VEC];
+  const int step = gridDim.x * tm.teams;
+  V w[ITER];
 #pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const int i = (k * ts + lane) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[k][e] = 0.f;
-      dw[k][e] = 0.f;
-    }
-    if (i < p.group) ld_weight<VEC>(p, g0 + i, w[k]);
-  }
-  int par = 0;
-  // the CTA's teams walk together (shuffles and barriers are for all of them)
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * teams; row0 < p.rows; row0 += gridDim.x * teams) {
-    const int64_t row = row0 + team;
-    const bool live = row < p.rows;
-    const int64_t tok = live ? row / p.heads : 0, head = live ? row - tok * p.heads : 0;
-    const X* x = static_cast<const X*>(p.x) + tok * p.sx_tok + head * p.sx_head + g0;
-    const T* z = p.z ? static_cast<const T*>(p.z) + tok * p.sz_tok + head * p.sz_head + g0 : nullptr;
-    const int64_t at = row * p.D + g0;
-    float r[ITER][VEC], d[ITER][VEC], zz[ITER][VEC];
+  for (int k = 0; k < ITER; ++k) w[k] = ld_weight<VEC>(p, g0 + tm.at(k));
+  pk::Raw<T, VEC> rx[ITER], rz[ITER];
+  pk::Raw<RT, VEC> rr[ITER];
+  auto load = [&](int row) {
+    int64_t xa, za;
+    row_of(p, min(row, p.rows - 1), xa, za);
+    const int64_t at = static_cast<int64_t>(min(row, p.rows - 1)) * p.D + g0;
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
-      const int i = (k * ts + lane) * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        r[k][e] = 0.f;
-        d[k][e] = 0.f;
-        zz[k][e] = 0.f;
-      }
-      if (live && i < p.group) {
-        if constexpr (sizeof(X) == 4) ldf<VEC>(x + i, r[k]);
-        else ldv<X, VEC>(x + i, r[k]);
-        ldv<T, VEC>(static_cast<const T*>(p.dy) + at + i, d[k]);
-        if (z) ldv<T, VEC>(z + i, zz[k]);
-      }
+      pk::load(rx[k], static_cast<const T*>(p.x) + xa + g0 + tm.at(k));
+      if (p.z) pk::load(rz[k], static_cast<const T*>(p.z) + za + g0 + tm.at(k));
+      if constexpr (kRes) pk::load(rr[k], static_cast<const RT*>(p.residual) + at + tm.at(k));
     }
-    float s[2] = {0.f, 0.f};  // sum u^2, sum dn u
+  };
+  int row0 = blockIdx.x * tm.teams, par = 0;
+  if (kAhead && row0 < p.rows) load(row0 + tm.team);
+  // the CTA's teams walk together (shuffles and barriers are for all of them)
+  for (; row0 < p.rows; row0 += step) {
+    const int row = row0 + tm.team;
+    if (!kAhead) load(row);
+    V u[ITER], a[ITER];
 #pragma unroll
-    for (int k = 0; k < ITER; ++k)
+    for (int k = 0; k < ITER; ++k) {
+      u[k] = pk::widen<T, VEC>(rx[k]);
+      if (p.z) a[k] = pk::widen<T, VEC>(rz[k]);
+      if constexpr (kRes) u[k] = pk::fma(pk::splat<VEC>(p.alpha), u[k], pk::widen<RT, VEC>(rr[k]));
+    }
+    if (kAhead && row0 + step < p.rows) load(row + step);
+    const bool live = row < p.rows;
+    const int64_t at = static_cast<int64_t>(row) * p.D + g0;
+    V sq = pk::splat<VEC>(0.f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float u = r[k][e], g = d[k][e];
-        if (z) {
-          const float a = gate(zz[k][e], p.sigmoid_gate);
-          if (p.gate_before) u *= a;
-          else g *= a;
-        }
-        s[0] = fmaf(u, u, s[0]);
-        s[1] = fmaf(g * w[k][e], u, s[1]);
+    for (int k = 0; k < ITER; ++k) {
+      if constexpr (kRes)
+        if (live && tm.in(k)) pk::store<RT, VEC>(static_cast<RT*>(p.sum) + at + tm.col(k), u[k]);
+      if (p.z) {
+        a[k] = gate(a[k], pk::sigmoid(a[k]), p.sigmoid_gate);
+        if (p.gate_before) u[k] = pk::mul(u[k], a[k]);
       }
-    team_sum<TS, 2>(s, buf[par]);
+      if (tm.in(k)) sq = pk::fma(u[k], u[k], sq);
+    }
+    float ss[1] = {pk::sum(sq)};
+    team_sum<TS, 1>(ss, buf[par]);
     par ^= 1;
-    const float rstd = rsqrtf(s[0] * inv + p.eps);
-    const float c = s[1] * rstd * inv;  // mean(dn n)
+    const V rstd = pk::splat<VEC>(rsqrtf(fmaf(ss[0], inv, p.eps)));
     if (!live) continue;
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
-      const int i = (k * ts + lane) * VEC;
-      if (i >= p.group) break;
-      float dr[VEC], dz[VEC];
+      V y = pk::mul(pk::mul(u[k], rstd), w[k]);
+      if (p.z && !p.gate_before) y = pk::mul(y, a[k]);
+      if (tm.in(k)) pk::store<T, VEC>(static_cast<T*>(p.y) + at + tm.col(k), y);
+    }
+  }
+}
+
+// X: the type of x (the residual's when the forward summed one).
+template <typename T, typename X, int VEC, int ITER, int TS, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const Params p) {
+  using V = pk::Vec<VEC>;
+  extern __shared__ float dws[];  // [teams][group] when teams > 1
+  __shared__ float buf[2][2][32];
+  const Team<VEC, ITER, TS> tm(p.group);
+  const int64_t g0 = static_cast<int64_t>(blockIdx.y) * p.group;
+  const float inv = 1.f / static_cast<float>(p.group);
+  const int step = gridDim.x * tm.teams;
+  constexpr bool kAhead = MAXT <= 256;  // larger CTAs have no registers for the next row
+  V w[ITER], dw[ITER];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float a = 1.f, da = 0.f;
-        if (z) gate_grad(zz[k][e], p.sigmoid_gate, a, da);
-        const float u = p.gate_before ? r[k][e] * a : r[k][e];
-        const float n = u * rstd;
-        const float g = p.gate_before ? d[k][e] : d[k][e] * a;
-        dw[k][e] = fmaf(g, n, dw[k][e]);
-        const float du = rstd * fmaf(-n, c, g * w[k][e]);
-        dz[e] = (p.gate_before ? du * r[k][e] : d[k][e] * n * w[k][e]) * da;
-        dr[e] = p.gate_before ? du * a : du;
+  for (int k = 0; k < ITER; ++k) {
+    w[k] = ld_weight<VEC>(p, g0 + tm.at(k));
+    dw[k] = pk::splat<VEC>(0.f);
+  }
+  pk::Raw<X, VEC> nx[ITER], rs[ITER];
+  pk::Raw<T, VEC> nd[ITER], nz[ITER];
+  auto load = [&](int row) {
+    int64_t xa, za;
+    row_of(p, min(row, p.rows - 1), xa, za);
+    const int64_t at = static_cast<int64_t>(min(row, p.rows - 1)) * p.D + g0;
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      pk::load(nx[k], static_cast<const X*>(p.x) + xa + g0 + tm.at(k));
+      pk::load(nd[k], static_cast<const T*>(p.dy) + at + tm.at(k));
+      if (p.z) pk::load(nz[k], static_cast<const T*>(p.z) + za + g0 + tm.at(k));
+    }
+  };
+  int row0 = blockIdx.x * tm.teams, par = 0;
+  if (kAhead && row0 < p.rows) load(row0 + tm.team);
+  for (; row0 < p.rows; row0 += step) {
+    const int row = row0 + tm.team;
+    if (!kAhead) load(row);
+    const bool live = row < p.rows;
+    const int64_t at = static_cast<int64_t>(row) * p.D + g0;
+    pk::Raw<X, VEC> rx[ITER];
+    pk::Raw<T, VEC> rd[ITER], rz[ITER];
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      rx[k] = nx[k];
+      rd[k] = nd[k];
+      if (p.z) rz[k] = nz[k];
+      if (p.dsum && live) pk::load(rs[k], static_cast<const X*>(p.dsum) + at + tm.at(k));
+    }
+    if (kAhead && row0 + step < p.rows) load(row + step);
+    V s[ITER], squ = pk::splat<VEC>(0.f), sgu = pk::splat<VEC>(0.f);
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) {
+      V u = pk::widen<X, VEC>(rx[k]), g = pk::mul(pk::widen<T, VEC>(rd[k]), w[k]);
+      if (p.z) {
+        const V z = pk::widen<T, VEC>(rz[k]);
+        s[k] = pk::sigmoid(z);
+        const V a = gate(z, s[k], p.sigmoid_gate);
+        if (p.gate_before) u = pk::mul(u, a);
+        else g = pk::mul(g, a);
       }
-      if (z) stv<T, VEC>(static_cast<T*>(p.dz) + at + i, dz);
-      if (p.dsum) {
-        float ds[VEC];
-        ld_res<T, VEC>(p.dsum, p.res_f32, at + i, ds);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) dr[e] += ds[e];
+      if (tm.in(k)) {
+        squ = pk::fma(u, u, squ);
+        sgu = pk::fma(g, u, sgu);
       }
-      if (p.dresidual) st_res<T, VEC>(p.dresidual, p.res_f32, at + i, dr);
+    }
+    float sums[2] = {pk::sum(squ), pk::sum(sgu)};
+    team_sum<TS, 2>(sums, buf[par]);
+    par ^= 1;
+    const float rstd = rsqrtf(fmaf(sums[0], inv, p.eps));
+    const V rs2 = pk::splat<VEC>(rstd), nc = pk::splat<VEC>(-sums[1] * rstd * inv);  // -mean(dn n)
+    if (!live) continue;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) dr[e] *= p.alpha;
-      stv<T, VEC>(static_cast<T*>(p.dx) + at + i, dr);
+    for (int k = 0; k < ITER; ++k) {
+      if (!tm.in(k)) break;
+      const V r = pk::widen<X, VEC>(rx[k]), dy = pk::widen<T, VEC>(rd[k]);
+      V dr;
+      if (!p.z) {
+        const V n = pk::mul(r, rs2);
+        dw[k] = pk::fma(dy, n, dw[k]);
+        dr = pk::mul(rs2, pk::fma(n, nc, pk::mul(dy, w[k])));
+      } else {
+        const V a = gate(pk::widen<T, VEC>(rz[k]), s[k], p.sigmoid_gate), da = gate_grad(s[k], a, p.sigmoid_gate);
+        V dz;
+        if (p.gate_before) {
+          const V n = pk::mul(pk::mul(r, a), rs2);
+          dw[k] = pk::fma(dy, n, dw[k]);
+          const V du = pk::mul(rs2, pk::fma(n, nc, pk::mul(dy, w[k])));
+          dz = pk::mul(pk::mul(du, r), da);
+          dr = pk::mul(du, a);
+        } else {
+          const V n = pk::mul(r, rs2), g = pk::mul(dy, a), nw = pk::mul(n, w[k]);
+          dw[k] = pk::fma(g, n, dw[k]);
+          dr = pk::mul(rs2, pk::fma(n, nc, pk::mul(g, w[k])));
+          dz = pk::mul(pk::mul(dy, nw), da);
+        }
+        pk::store<T, VEC>(static_cast<T*>(p.dz) + at + tm.col(k), dz);
+      }
+      if (p.dsum) dr = pk::add(dr, pk::widen<X, VEC>(rs[k]));
+      if (p.dresidual) pk::store<X, VEC>(static_cast<X*>(p.dresidual) + at + tm.col(k), dr);
+      pk::store<T, VEC>(static_cast<T*>(p.dx) + at + tm.col(k), pk::mul(dr, pk::splat<VEC>(p.alpha)));
     }
   }
   float* out = p.partial + static_cast<int64_t>(blockIdx.x) * p.D + g0;
   if (TS == 0) {
 #pragma unroll
-    for (int k = 0; k < ITER; ++k) {
-      const int i = (k * ts + lane) * VEC;
-      if (i < p.group) stf<1>(out + i, dw[k]);
+    for (int k = 0; k < ITER; ++k)
+      if (tm.in(k))
 #pragma unroll
-      for (int e = 1; e < VEC; ++e)
-        if (i < p.group) out[i + e] = dw[k][e];
-    }
+        for (int e = 0; e < VEC; ++e) out[tm.col(k) + e] = pk::get(dw[k], e);
     return;
   }
 #pragma unroll
-  for (int k = 0; k < ITER; ++k) {
-    const int i = (k * ts + lane) * VEC;
+  for (int k = 0; k < ITER; ++k)
+    if (tm.in(k))
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (i < p.group) dws[team * p.group + i + e] = dw[k][e];
-  }
+      for (int e = 0; e < VEC; ++e) dws[tm.team * p.group + tm.col(k) + e] = pk::get(dw[k], e);
   __syncthreads();
   for (int i = threadIdx.x; i < p.group; i += blockDim.x) {
     float a = 0.f;
-    for (int t = 0; t < teams; ++t) a += dws[t * p.group + i];
+    for (int t = 0; t < tm.teams; ++t) a += dws[t * p.group + i];
     out[i] = a;
   }
 }
@@ -357,6 +353,7 @@ bool fdtype_ok(int d) { return d == GDN_F32 || d == GDN_BF16 || d == GDN_F16; }
 int esize(int d) { return d == GDN_F32 ? 4 : 2; }
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+constexpr int kFwdThreads = 1024, kBwdThreads = 512;  // per SM
 constexpr int kMaxScalar = 16 * 1024, kMaxVector = 4 * 1024;  // elements / vectors a CTA can hold
 
 // 16-byte vectors when the group, the strides and every pointer allow them.
@@ -369,30 +366,40 @@ int vec_of(const gdn_norm_args& a) {
   return ok ? v : 1;
 }
 
+template <int I>
+using Int = std::integral_constant<int, I>;
+
 struct Shape {
   int ts, iter, threads;  // ts = 0: the CTA is the team
 };
-// Lanes for n vectors (or scalars) per group.  Few lanes per row keep the
-// reductions inside a warp; more than four vectors per lane would spill.
-Shape shape_of(int n, bool vec) {
-  if (!vec) {
-    if (n <= 128) return {32, 4, 256};
-    if (n <= 4096) return {0, 4, ((n + 3) / 4 + 31) / 32 * 32};
-    return {0, 16, 1024};
+
+// How a row's group of n vectors (or scalars) is held, as f(vectors per
+// thread, lanes per team or 0 for the CTA, largest CTA) and the Shape: one
+// vector per thread as far as a CTA reaches.  (Two vectors on half the lanes
+// measured the same in the forward, 36 us for 262144 rows of 128 with a gate,
+// and cost the backward half its resident threads.)
+template <int VEC, typename F>
+void pick(int n, F&& f) {
+  auto cta = [](int lanes) { return std::max(32, (lanes + 31) / 32 * 32); };
+  if constexpr (VEC == 1) {
+    if (n <= 128) f(Int<4>{}, Int<32>{}, Int<128>{}, Shape{32, 4, 128});
+    else if (n <= 4096) f(Int<4>{}, Int<0>{}, Int<1024>{}, Shape{0, 4, cta((n + 3) / 4)});
+    else f(Int<16>{}, Int<0>{}, Int<1024>{}, Shape{0, 16, 1024});
+  } else {
+    if (n <= 8) f(Int<1>{}, Int<8>{}, Int<128>{}, Shape{8, 1, 128});
+    else if (n <= 16) f(Int<1>{}, Int<16>{}, Int<128>{}, Shape{16, 1, 128});
+    else if (n <= 32) f(Int<1>{}, Int<32>{}, Int<128>{}, Shape{32, 1, 128});
+    else if (n <= 256) f(Int<1>{}, Int<0>{}, Int<256>{}, Shape{0, 1, cta(n)});
+    else if (n <= 1024) f(Int<1>{}, Int<0>{}, Int<1024>{}, Shape{0, 1, cta(n)});
+    else f(Int<4>{}, Int<0>{}, Int<1024>{}, Shape{0, 4, 1024});
   }
-  if (n <= 8) return {8, 1, 128};
-  if (n <= 16) return {16, 1, 128};
-  if (n <= 32) return {32, 1, 128};
-  if (n <= 64) return {32, 2, 128};
-  if (n <= 128) return {32, 4, 128};
-  if (n <= 512) return {0, 2, ((n + 1) / 2 + 31) / 32 * 32};
-  if (n <= 1024) return {0, 1, (n + 31) / 32 * 32};
-  return {0, 4, 1024};
 }
-// CTAs per group of the backward: about four per SM over all groups.
+
+// CTAs per group of the backward, over all groups: as many as reside.
 int64_t parts_of(const gdn_norm_args& a, const Shape& sh) {
   const int64_t teams = sh.ts ? sh.threads / sh.ts : 1, groups = a.D / a.group;
-  return std::max<int64_t>(1, std::min((a.rows + teams - 1) / teams, std::max<int64_t>(1, 592 / groups)));
+  const int64_t most = 148 * std::max(1, kBwdThreads / sh.threads);
+  return std::max<int64_t>(1, std::min((a.rows + teams - 1) / teams, std::max<int64_t>(1, most / groups)));
 }
 
 int check(const gdn_norm_args* a, bool bwd) {
@@ -407,6 +414,8 @@ int check(const gdn_norm_args* a, bool bwd) {
   if (a->group > kMaxScalar && fdtype_ok(a->dtype) && vec_of(v) == 1)
     return set_last_error(GDN_ERR_UNSUPPORTED, "group=%d above %d (or above %d vectors of 16 bytes)", a->group, kMaxScalar,
                           kMaxVector);
+  if (a->rows > 0x7fffffffLL || a->heads > 0x7fffffffLL)
+    return set_last_error(GDN_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   if (a->D / a->group > 65535) return set_last_error(GDN_ERR_UNSUPPORTED, "more than 65535 groups per row");
   if (!fdtype_ok(a->dtype) || !fdtype_ok(a->w_dtype) || !fdtype_ok(a->x_dtype) || !fdtype_ok(a->res_dtype))
     return set_last_error(GDN_ERR_INVALID, "dtypes must be F32, BF16 or F16");
@@ -426,66 +435,52 @@ Params params(const gdn_norm_args& a) {
   p.x = a.x; p.z = a.z; p.residual = a.residual; p.weight = a.weight; p.y = a.y; p.sum = a.sum;
   p.dy = a.dy; p.dsum = a.dsum; p.dx = a.dx; p.dz = a.dz; p.dresidual = a.dresidual;
   p.partial = static_cast<float*>(a.workspace);
-  p.rows = a.rows; p.heads = a.heads; p.D = a.D;
+  p.rows = static_cast<int>(a.rows); p.heads = static_cast<int>(a.heads); p.D = a.D;
   p.sx_tok = a.stride_x_token; p.sx_head = a.stride_x_head; p.sz_tok = a.stride_z_token; p.sz_head = a.stride_z_head;
   p.group = a.group; p.w_dtype = a.w_dtype; p.res_f32 = a.res_dtype == GDN_F32;
   p.gate_before = a.z && a.gate_before; p.sigmoid_gate = a.activation == GDN_GATE_SIGMOID;
   p.eps = a.eps; p.alpha = a.residual_scale; p.w_off = a.zero_centered ? 1.f : 0.f;
+  if (p.sx_tok == p.heads * p.sx_head && (!a.z || p.sz_tok == p.heads * p.sz_head)) {  // rows in one run
+    p.heads = 1;
+    p.sx_tok = p.sx_head;
+    p.sz_tok = p.sz_head;
+  }
   return p;
 }
 
-template <int I>
-using Int = std::integral_constant<int, I>;
-
-// Calls f(vectors per thread, lanes per team, largest CTA) of the shape.
-template <typename F>
-void pick(const Shape& sh, bool vec, F&& f) {
-  if (!vec) {
-    if (sh.ts == 32) f(Int<4>{}, Int<32>{}, Int<256>{});
-    else if (sh.iter == 4) f(Int<4>{}, Int<0>{}, Int<1024>{});
-    else f(Int<16>{}, Int<0>{}, Int<1024>{});
-    return;
-  }
-  if (sh.ts == 8) f(Int<1>{}, Int<8>{}, Int<128>{});
-  else if (sh.ts == 16) f(Int<1>{}, Int<16>{}, Int<128>{});
-  else if (sh.ts == 32 && sh.iter == 1) f(Int<1>{}, Int<32>{}, Int<128>{});
-  else if (sh.ts == 32 && sh.iter == 2) f(Int<2>{}, Int<32>{}, Int<128>{});
-  else if (sh.ts == 32) f(Int<4>{}, Int<32>{}, Int<128>{});
-  else if (sh.iter == 2) f(Int<2>{}, Int<0>{}, Int<256>{});
-  else if (sh.iter == 1) f(Int<1>{}, Int<0>{}, Int<1024>{});
-  else f(Int<4>{}, Int<0>{}, Int<1024>{});
-}
-
-template <typename T, int VEC>
+// CTAs per group of the forward: as many as reside, about 1024 threads per SM.
+template <typename T, typename R, int VEC>
 void fwd(const gdn_norm_args& a, const Params& p, cudaStream_t s) {
-  const Shape sh = shape_of(a.group / VEC, VEC > 1);
-  const int64_t teams = sh.ts ? sh.threads / sh.ts : 1;
-  const dim3 grid(static_cast<unsigned>((a.rows + teams - 1) / teams), static_cast<unsigned>(a.D / a.group));
-  pick(sh, VEC > 1, [&](auto iter, auto ts, auto most) {
-    norm_fwd_kernel<T, VEC, decltype(iter)::value, decltype(ts)::value,
-                    decltype(most)::value><<<grid, sh.threads, 0, s>>>(p);
+  pick<VEC>(a.group / VEC, [&](auto iter, auto ts, auto max_threads, Shape sh) {
+    const int64_t teams = sh.ts ? sh.threads / sh.ts : 1, groups = a.D / a.group;
+    const int64_t most = std::max<int64_t>(1, 148 * std::max(1, kFwdThreads / sh.threads) / groups);
+    const dim3 grid(static_cast<unsigned>(std::min((a.rows + teams - 1) / teams, most)), static_cast<unsigned>(groups));
+    norm_fwd_kernel<T, R, VEC, decltype(iter)::value, decltype(ts)::value, decltype(max_threads)::value>
+        <<<grid, sh.threads, 0, s>>>(p);
   });
 }
 
 template <typename T, typename X, int VEC>
 void bwd(const gdn_norm_args& a, const Params& p, cudaStream_t s) {
-  const Shape sh = shape_of(a.group / VEC, VEC > 1);
-  const int64_t parts = parts_of(a, sh);
-  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(a.D / a.group));
-  const size_t smem = sh.ts ? static_cast<size_t>(sh.threads / sh.ts) * a.group * sizeof(float) : 0;
-  pick(sh, VEC > 1, [&](auto iter, auto ts, auto most) {
-    norm_bwd_kernel<T, X, VEC, decltype(iter)::value, decltype(ts)::value,
-                    decltype(most)::value><<<grid, sh.threads, smem, s>>>(p);
+  pick<VEC>(a.group / VEC, [&](auto iter, auto ts, auto max_threads, Shape sh) {
+    const int64_t parts = parts_of(a, sh);
+    const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(a.D / a.group));
+    const size_t smem = sh.ts ? static_cast<size_t>(sh.threads / sh.ts) * a.group * sizeof(float) : 0;
+    norm_bwd_kernel<T, X, VEC, decltype(iter)::value, decltype(ts)::value, decltype(max_threads)::value>
+        <<<grid, sh.threads, smem, s>>>(p);
+    note_launch();
+    norm_dw_kernel<<<static_cast<unsigned>((a.D + 31) / 32), 1024, 0, s>>>(p.partial, parts, a.D,
+                                                                         const_cast<void*>(a.dweight), a.w_dtype);
   });
-  note_launch();
-  norm_dw_kernel<<<static_cast<unsigned>((a.D + 31) / 32), 1024, 0, s>>>(p.partial, parts, a.D, const_cast<void*>(a.dweight),
-                                                                       a.w_dtype);
 }
 
 template <typename T>
 void fwd_t(const gdn_norm_args& a, const Params& p, cudaStream_t s) {
-  if (vec_of(a) > 1) fwd<T, 16 / sizeof(T)>(a, p, s);
-  else fwd<T, 1>(a, p, s);
+  const bool vec = vec_of(a) > 1;
+  constexpr int kV = 16 / sizeof(T);
+  if (!a.residual) vec ? fwd<T, void, kV>(a, p, s) : fwd<T, void, 1>(a, p, s);
+  else if (p.res_f32) vec ? fwd<T, float, kV>(a, p, s) : fwd<T, float, 1>(a, p, s);
+  else vec ? fwd<T, T, kV>(a, p, s) : fwd<T, T, 1>(a, p, s);
 }
 // Vectors follow the activations' type: eight 16-bit values (and eight fp32
 // ones of the residual beside them).
@@ -508,7 +503,6 @@ extern "C" GDN_API int gdn_norm_fwd(const gdn_norm_args* a, void* stream) {
   if (a->rows == 0) return GDN_OK;
   if (!a->x || !a->weight || !a->y) return set_last_error(GDN_ERR_INVALID, "x, weight and y must be non-null");
   if ((a->residual != nullptr) != (a->sum != nullptr)) return set_last_error(GDN_ERR_INVALID, "sum goes with residual");
-  if (a->rows > 0x7fffffffLL) return set_last_error(GDN_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   const norm::Params p = norm::params(*a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   note_launch();
@@ -520,10 +514,10 @@ extern "C" GDN_API int gdn_norm_fwd(const gdn_norm_args* a, void* stream) {
   return GDN_OK;
 }
 
-// At most 592 CTAs' parts of a row (see parts_of), whatever the alignment.
+// The parts of parts_of at its most (CTAs of 64 threads), whatever the alignment.
 extern "C" GDN_API size_t gdn_norm_bwd_workspace_size(const gdn_norm_args* a) {
   if (norm::check(a, true)) return 0;
-  return static_cast<size_t>(std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(a->rows, 1), 592))) * a->D * sizeof(float);
+  return static_cast<size_t>(std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(a->rows, 1), 148 * (norm::kBwdThreads / 32)))) * a->D * sizeof(float);
 }
 
 extern "C" GDN_API int gdn_norm_bwd(const gdn_norm_args* a, void* stream) {
