@@ -10,6 +10,7 @@
 // state).  With one segment per sequence the second pass is the only one.
 
 #include "gdn_scan.h"
+#include "packed2.cuh"
 #include "scan_common.cuh"
 
 #include <algorithm>
@@ -140,8 +141,10 @@ __global__ void __launch_bounds__(256) scan_rec_kernel(const ScanParams p) {
 }
 
 // States between segments: for each sequence, head and state element, in
-// order, seg_state[i] <- h and h <- exp(log decay of i) h + seg_state[i].
-// One thread per four elements; a stream over the segments' states.
+// order of its segments, the state that the segment starts from (in place of
+// its first piece's) and h <- exp(log decay) h + state over its pieces.  A
+// stream over the pieces' states; VEC elements per thread.
+template <int VEC>
 __global__ void __launch_bounds__(256) scan_pass_kernel(const ScanParams p) {
   __shared__ int64_t first_sh, count_sh;
   const int64_t n = blockIdx.z;
@@ -169,32 +172,33 @@ __global__ void __launch_bounds__(256) scan_pass_kernel(const ScanParams p) {
   }
   __syncthreads();
   const int64_t PS = static_cast<int64_t>(p.P) * p.S;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * VEC;
   if (i >= PS) return;
   const int64_t first = first_sh, count = min64(count_sh, p.segments - first);
-  float cur = p.init ? ld_any(p.init, p.init_dtype, (n * p.H + h) * PS + i) : 0.f;
-  float* st = p.seg_state + (first * p.H + h) * PS + i;
-  const float* ld = p.seg_decay + first * p.H + h;
+  pk::Vec<VEC> cur;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e)
+    pk::set(cur, e, p.init ? ld_any(p.init, p.init_dtype, (n * p.H + h) * PS + i + e) : 0.f);
+  float* st = p.seg_state + (first * p.subs * p.H + h) * PS + i;
+  const float* ld = p.seg_decay + first * p.subs * p.H + h;
   const int64_t step = p.H * PS;
-  int64_t k = 0;
-  for (; k + 4 < count; k += 4) {  // four segments' loads in flight
-    float v[4], d[4];
+  for (int64_t k = 0; k < count; ++k, st += p.subs * step, ld += static_cast<int64_t>(p.subs) * p.H) {
+    const bool more = k + 1 < count;
+    constexpr int kAhead = 4;  // pieces whose loads are in flight together
+    for (int j0 = 0; j0 < (more ? p.subs : 1); j0 += kAhead) {
+      pk::Raw<float, VEC> v[kAhead];
+      float d[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = st[(k + j) * step];
-      d[j] = expf(ld[(k + j) * p.H]);
-    }
+      for (int j = 0; j < kAhead; ++j)
+        if (more && j0 + j < p.subs) {
+          pk::load(v[j], st + (j0 + j) * step);
+          d[j] = expf(ld[(j0 + j) * p.H]);
+        }
+      if (j0 == 0) pk::store<float, VEC>(st, cur);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      st[(k + j) * step] = cur;
-      cur = fmaf(d[j], cur, v[j]);
+      for (int j = 0; j < kAhead; ++j)
+        if (more && j0 + j < p.subs) cur = pk::fma(pk::splat<VEC>(d[j]), cur, pk::widen<float, VEC>(v[j]));
     }
-  }
-  for (; k < count; ++k) {
-    const float v = k + 1 < count ? st[k * step] : 0.f;
-    const float d = k + 1 < count ? expf(ld[k * p.H]) : 1.f;
-    st[k * step] = cur;
-    cur = fmaf(d, cur, v);
   }
 }
 
@@ -322,6 +326,7 @@ int check(const gdn_scan_args* a) {
 
 struct Plan {
   int64_t seg, segments;  // tokens per segment; at most so many segments
+  int64_t sub, subs;      // the first pass's pieces of a segment: tokens, number
   bool split;
   size_t scratch_off, state_off, decay_off, bytes;  // the error word comes first
 };
@@ -346,10 +351,19 @@ Plan plan(const gdn_scan_args& a) {
   pl.segments = pl.split ? total / pl.seg + a.N : a.N;
   pl.scratch_off = 256;
   pl.state_off = pl.bytes = 256 + (tc ? (tc_scratch_bytes(a) + 255) / 256 * 256 : 0);
+  // The first pass has no chain between its chunks: cut its segments (all but
+  // the last of a sequence) further until it fills the GPU too.
+  pl.sub = pl.seg;
+  if (tc && pl.split) {
+    const int64_t cut = std::max<int64_t>(1, want / std::max<int64_t>(1, (pieces - 1) * per_token));
+    pl.sub = std::max<int64_t>(128, (pl.seg / cut + 127) / 128 * 128);
+  }
+  pl.subs = (pl.seg + pl.sub - 1) / pl.sub;
   if (pl.split) {
-    const size_t states = static_cast<size_t>(pl.segments) * a.H * a.P * a.S * sizeof(float);
+    const size_t pieces_all = static_cast<size_t>(pl.segments) * pl.subs;
+    const size_t states = pieces_all * a.H * a.P * a.S * sizeof(float);
     pl.decay_off = pl.state_off + (states + 255) / 256 * 256;
-    pl.bytes = pl.decay_off + static_cast<size_t>(pl.segments) * a.H * sizeof(float);
+    pl.bytes = pl.decay_off + pieces_all * a.H * sizeof(float);
   }
   return pl;
 }
@@ -380,9 +394,11 @@ void launch_t(const ScanParams& p, const Plan& pl, cudaStream_t s) {
 
 void launch_pass(const ScanParams& p, cudaStream_t s) {
   const int64_t PS = static_cast<int64_t>(p.P) * p.S;
+  const int vec = PS % 4 == 0 ? 4 : 1;
+  const dim3 grid(static_cast<unsigned>((PS / vec + 255) / 256), static_cast<unsigned>(p.H), static_cast<unsigned>(p.N));
   note_launch();
-  scan_pass_kernel<<<dim3(static_cast<unsigned>((PS + 255) / 256), static_cast<unsigned>(p.H), static_cast<unsigned>(p.N)),
-                     256, 0, s>>>(p);
+  if (vec == 4) scan_pass_kernel<4><<<grid, 256, 0, s>>>(p);
+  else scan_pass_kernel<1><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T, typename CT, int VEC, int LPR, int ITER, int R>
@@ -450,6 +466,7 @@ extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
   p.err = static_cast<int*>(a->workspace);
   p.clear_err = 1;
   p.T = a->T; p.N = a->N; p.total = total; p.seg = pl.seg; p.segments = pl.segments;
+  p.sub = pl.sub; p.subs = static_cast<int>(pl.subs);
   p.sx = a->stride_x; p.sdt = a->stride_dt; p.sb = a->stride_b; p.sc = a->stride_c; p.sz = a->stride_z;
   p.H = a->H; p.P = a->P; p.G = a->G; p.S = a->S;
   p.dt_dtype = a->dt_dtype; p.init_dtype = a->init_dtype; p.final_dtype = a->final_dtype; p.cu_dtype = a->cu_dtype;

@@ -79,18 +79,17 @@ struct Smem {
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
-// First pass: two stages of B and x and, beside each, three parts of w x.
+// First pass: three stages of B (read until its products are done), two of x
+// (read until it is split) and two of its three parts.
 template <int S_>
 struct StateSmem {
-  static constexpr int kB = 0;
-  static constexpr int kX = S_ / 64 * kTile;
-  static constexpr int kXs = kX + kTile;
-  static constexpr int kStage = kXs + 3 * kTile;
-  static constexpr int kBar = 2 * kStage;  // loads[2], parts ready[2], products[2]
-  static constexpr int kTmem = kBar + 6 * 8;
+  static constexpr int kBStage = S_ / 64 * kTile;
+  static constexpr int kX = 3 * kBStage;
+  static constexpr int kXs = kX + 2 * kTile;
+  static constexpr int kBar = kXs + 6 * kTile;  // B[3], x[2], parts ready[2], products[2]
+  static constexpr int kTmem = kBar + 9 * 8;
   static constexpr int kBytes = kTmem + 8;
   static constexpr int kCols = 64;
-  static constexpr uint32_t kTx = (S_ / 64 + 1) * kTile;
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -120,23 +119,34 @@ __device__ __forceinline__ uint4 take_part(float2* v) {
   return u;
 }
 
-// Steps of one chunk of 128 tokens for 32 heads per block: raw steps in
-// through shared memory (rows of heads are what is contiguous), a, k and dt
-// out per head with tokens contiguous.  A warp scans a head's 128 tokens,
-// four per lane.
-__global__ void __launch_bounds__(256) scan_prep_kernel(const ScanParams p, const PrepOut o) {
-  __shared__ float raw[kL][33];
+// Steps of one chunk of 128 tokens for 16 heads per block (a 32-byte sector
+// of 16-bit steps): raw steps in through shared memory (rows of heads are what
+// is contiguous), a, k and dt out per head with tokens contiguous.  A warp
+// scans a head's 128 tokens, four per lane.
+constexpr int kPrepHeads = 16;
+__global__ void __launch_bounds__(kPrepHeads * 32) scan_prep_kernel(const ScanParams p, const PrepOut o) {
+  __shared__ float raw[kL][kPrepHeads + 1];
   clear_error(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = blockIdx.y * 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = blockIdx.y * kPrepHeads;
   int64_t n, ls, t0, t1;
   bool last;
   if (!find_segment(p, blockIdx.x, n, ls, t0, t1, last)) return;  // p.seg is the chunk here
   const int len = static_cast<int>(t1 - t0);
-  for (int i = warp; i < len; i += 8)
-    if (h0 + lane < p.H) raw[i][lane] = ld_any(p.dt, p.dt_dtype, (t0 + i) * p.sdt + h0 + lane);
+  {
+    constexpr int kTurns = kL / (2 * kPrepHeads);  // two tokens per warp and turn, all turns' loads together
+    const int hh = lane % kPrepHeads, i0 = warp * 2 + lane / kPrepHeads;
+    float v[kTurns];
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j) {
+      const int i = i0 + j * 2 * kPrepHeads;
+      v[j] = i < len && h0 + hh < p.H ? ld_any(p.dt, p.dt_dtype, (t0 + i) * p.sdt + h0 + hh) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j) raw[i0 + j * 2 * kPrepHeads][hh] = v[j];
+  }
   __syncthreads();
-  for (int hh = warp; hh < 32 && h0 + hh < p.H; hh += 8) {
-    const int h = h0 + hh;
+  if (h0 + warp < p.H) {
+    const int hh = warp, h = h0 + hh;
     const float A2 = p.A[h] * tc::kLog2e, bias = p.dt_bias ? p.dt_bias[h] : 0.f;
     float d[4], a[4], pre[4], suf[4];
 #pragma unroll
@@ -469,7 +479,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     for (int j = 0; j < 16; ++j) {
       float v = 0.f;
       if (row < S_) {
-        if (seg) v = p.seg_state[state_at(id) + j * S_];
+        if (seg) v = p.seg_state[state_at(id * p.subs) + j * S_];
         else if (ini) v = ld_any(p.init, p.init_dtype, state_at(n) + j * S_);
       }
       if (j & 1) hr[j / 2].y = v;
@@ -635,6 +645,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   if (warp == kLead) umma::tmem_dealloc(tmem, M::kCols);
 }
 
+// Block = (segment * subs + piece of it) * units + unit.
 template <int S_>
 __global__ void __launch_bounds__(kTcThreads, 1)
 scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, const __grid_constant__ CUtensorMap tx,
@@ -644,21 +655,23 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::kBar);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + M::kTmem);
   const uint32_t sbase = umma::smem_u32(sm);
-  const uint32_t bar_ld = umma::smem_u32(bars), bar_xs = bar_ld + 16, bar_dh = bar_ld + 32;  // [2] each
+  const uint32_t bar_b = umma::smem_u32(bars), bar_x = bar_b + 24, bar_xs = bar_b + 40, bar_dh = bar_b + 56;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (!base_ok(p, sbase)) return;
   const int units = p.H * slices;
-  const int64_t id = blockIdx.x / units;
-  const int unit = static_cast<int>(blockIdx.x - id * units), h = unit / slices, p0 = (unit - h * slices) * 64;
+  const int64_t piece_id = blockIdx.x / units, id = piece_id / p.subs;
+  const int unit = static_cast<int>(blockIdx.x - piece_id * units), h = unit / slices, p0 = (unit - h * slices) * 64;
   const int g = h / (p.H / p.G);
   int64_t n = 0, ls = 0, t0 = 0, t1 = 0;
   bool last = false;
   if (!find_segment(p, id, n, ls, t0, t1, last) || last) return;
-  const int nch = static_cast<int>((t1 - t0) / kL);  // a segment that is not the last is whole chunks
+  t0 += (piece_id - id * p.subs) * p.sub;  // a segment that is not the last is whole: pieces of whole chunks
+  t1 = min64(t1, t0 + p.sub);
+  const int nch = static_cast<int>((t1 - t0) / kL);
   if (warp == kLead) {
     if (umma::elect_one()) {
 #pragma unroll
-      for (int i = 0; i < 6; ++i) umma::mbar_init(bars + i, i == 2 || i == 3 ? kLead : 1);
+      for (int i = 0; i < 9; ++i) umma::mbar_init(bars + i, i == 5 || i == 6 ? kLead : 1);
       umma::mbar_fence_init();
     }
     __syncwarp();
@@ -675,41 +688,51 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     mine = got;
     return got;
   };
-  // step i works on chunk nch - 1 - i in stage i & 1
+  // step i works on chunk nch - 1 - i
   if (warp == kLead) {
     constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
-    const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
-    auto fetch = [&](int i) {
-      const int t = static_cast<int>(t0) + (nch - 1 - i) * kL;
-      const uint32_t bar = bar_ld + (i & 1) * 8;
-      uint8_t* st = sm + (i & 1) * M::kStage;
-      umma::mbar_arrive_expect_tx(bar, M::kTx);
+    const uint64_t d_b = umma::smem_desc_sw128(sbase, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
+    auto token = [&](int i) { return static_cast<int>(t0) + (nch - 1 - i) * kL; };
+    auto fetch_b = [&](int i) {
+      umma::mbar_arrive_expect_tx(bar_b + (i % 3) * 8, M::kBStage);
 #pragma unroll
-      for (int q = 0; q < S_ / 64; ++q) umma::tma_load_2d(st + M::kB + q * kTile, &tb, g * S_ + q * 64, t, bar);
-      umma::tma_load_2d(st + M::kX, &tx, h * p.P + p0, t, bar);
+      for (int q = 0; q < S_ / 64; ++q)
+        umma::tma_load_2d(sm + (i % 3) * M::kBStage + q * kTile, &tb, g * S_ + q * 64, token(i), bar_b + (i % 3) * 8);
+    };
+    auto fetch_x = [&](int i) {
+      umma::mbar_arrive_expect_tx(bar_x + (i & 1) * 8, kTile);
+      umma::tma_load_2d(sm + M::kX + (i & 1) * kTile, &tx, h * p.P + p0, token(i), bar_x + (i & 1) * 8);
     };
     if (umma::elect_one()) {
-      fetch(0);
-      if (nch > 1) fetch(1);
+      fetch_x(0);
+      fetch_b(0);
+      if (nch > 1) {
+        fetch_x(1);
+        fetch_b(1);
+      }
     }
     __syncwarp();
-    int loads = min(nch, 2), done = 0;
+    int loads_b = min(nch, 2), loads_x = min(nch, 2), done = 0;
     for (int i = 0; i < nch; ++i) {
       if (!wait(bar_xs + (i & 1) * 8, (i >> 1) & 1, kSiteScanScores)) break;
-      if (i >= 1 && i + 1 < nch) {  // step i + 1 goes where step i - 1 was
-        if (!wait(bar_dh + ((i - 1) & 1) * 8, ((i - 1) >> 1) & 1, kSiteScanState)) break;
-        if (umma::elect_one()) fetch(i + 1);
+      if (i + 2 < nch) {
+        if (umma::elect_one()) fetch_x(i + 2);  // x of step i is split
         __syncwarp();
-        ++loads;
+        ++loads_x;
+        if (i > 0 && !wait(bar_dh + ((i - 1) & 1) * 8, ((i - 1) >> 1) & 1, kSiteScanState)) break;
+        if (umma::elect_one()) fetch_b(i + 2);  // where step i - 1's was
+        __syncwarp();
+        ++loads_b;
       }
+      if (!wait(bar_b + (i % 3) * 8, (i / 3) & 1, kSiteScanLoad)) break;
       umma::fence_after_sync();
       if (umma::elect_one()) {
-        const uint64_t st = (i & 1) * (M::kStage >> 4);
+        const uint64_t db = d_b + (i % 3) * (M::kBStage >> 4), dx = d_xs + (i & 1) * ((3 * kTile) >> 4);
 #pragma unroll
         for (int part = 0; part < 3; ++part)
 #pragma unroll
           for (int ks = 0; ks < kL / 16; ++ks)
-            umma::mma_f16(tmem, d_bm + st + mn_step(ks), d_xs + st + ((part * kTile) >> 4) + mn_step(ks), id_h,
+            umma::mma_f16(tmem, db + mn_step(ks), dx + ((part * kTile) >> 4) + mn_step(ks), id_h,
                           i > 0 || part > 0 || ks > 0);
         umma::mma_commit(bar_dh + (i & 1) * 8);
       }
@@ -718,45 +741,48 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     }
     if (!mine) {
       const long long drain = 20000000LL;
-      for (int i = max(0, loads - 2); i < loads; ++i) umma::mbar_wait(bar_ld + (i & 1) * 8, (i >> 1) & 1, drain);
+      for (int i = max(0, loads_b - 3); i < loads_b; ++i) umma::mbar_wait(bar_b + (i % 3) * 8, (i / 3) & 1, drain);
+      for (int i = max(0, loads_x - 2); i < loads_x; ++i) umma::mbar_wait(bar_x + (i & 1) * 8, (i >> 1) & 1, drain);
       for (int i = max(0, done - 2); i < done; ++i) umma::mbar_wait(bar_dh + (i & 1) * 8, (i >> 1) & 1, drain);
     }
   } else {
     const int quad = warp & 3, cq = warp >> 2, row = quad * 32 + lane;
     const Pieces piece(row, cq);
     const int64_t prow = static_cast<int64_t>(h) * p.total + t0;
-    float later = 0.f;  // log2 decay from the chunk's end to the segment's
+    float later = 0.f;  // log2 decay from the chunk's end to the piece's
     TokenScalars sc = load_scalars(prep, prow + (nch - 1) * kL, kL, row);
     for (int i = 0; i < nch; ++i) {
-      const uint32_t st = sbase + (i & 1) * M::kStage;
+      const uint32_t xt = sbase + M::kX + (i & 1) * kTile, xs = sbase + M::kXs + (i & 1) * 3 * kTile;
       const float wj = sc.k * ex2(sc.end[3] - pick4(sc.end, quad)) * ex2(later);
       later += sc.end[3];
       if (i + 1 < nch) sc = load_scalars(prep, prow + (nch - 2 - i) * kL, kL, row);
-      // the stage's products of two steps ago are done: its loads came after them
-      if (!wait(bar_ld + (i & 1) * 8, (i >> 1) & 1, kSiteScanLoad)) break;
+      if (!wait(bar_x + (i & 1) * 8, (i >> 1) & 1, kSiteScanLoad)) break;
+      if (i >= 2 && !wait(bar_dh + (i & 1) * 8, ((i - 2) >> 1) & 1, kSiteScanState)) break;  // the parts' tiles are read
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float2 v[4];
-        unpack8(lds16(st + M::kX + piece.at[q]), v);
+        unpack8(lds16(xt + piece.at[q]), v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(wj, wj));
-        sts16(st + M::kXs + piece.at[q], take_part(v));
-        sts16(st + M::kXs + kTile + piece.at[q], take_part(v));
-        sts16(st + M::kXs + 2 * kTile + piece.at[q], pack8(v));
+        sts16(xs + piece.at[q], take_part(v));
+        sts16(xs + kTile + piece.at[q], take_part(v));
+        sts16(xs + 2 * kTile + piece.at[q], pack8(v));
       }
       publish(bar_xs + (i & 1) * 8);
     }
-    const int i = nch - 1;  // the last step's products come after all others
+    // the last step's products come after all others; the phase before its own
+    // on that barrier was waited for above
+    const int i = nch - 1;
     if (mine && wait(bar_dh + (i & 1) * 8, (i >> 1) & 1, kSiteScanState)) {
       umma::fence_after_sync();
       float d[16];
       umma::tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + cq * 16, d);
       if (row < S_) {
-        float* out = p.seg_state + ((id * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
+        float* out = p.seg_state + ((piece_id * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
 #pragma unroll
         for (int j = 0; j < 16; ++j) out[j * S_] = d[j];
       }
-      if (tid == 0 && p0 == 0) p.seg_decay[id * p.H + h] = later * 0.6931471805599453f;
+      if (tid == 0 && p0 == 0) p.seg_decay[piece_id * p.H + h] = later * 0.6931471805599453f;
     }
   }
   umma::fence_before_sync();
@@ -808,7 +834,8 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
   ScanParams q = p;
   q.seg = kL;
   note_launch();
-  scan_prep_kernel<<<dim3(static_cast<unsigned>(total / kL + a.N), static_cast<unsigned>((a.H + 31) / 32)), 256, 0, s>>>(
+  scan_prep_kernel<<<dim3(static_cast<unsigned>(total / kL + a.N), static_cast<unsigned>((a.H + kPrepHeads - 1) / kPrepHeads)),
+                     kPrepHeads * 32, 0, s>>>(
       q, prep);
   const unsigned grid = static_cast<unsigned>(p.segments * p.H * slices);
   if (p.seg_state) {
@@ -816,7 +843,7 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, StateSmem<S_>::kBytes)) != cudaSuccess)
       return e;
     note_launch();
-    kern<<<grid, kTcThreads, StateSmem<S_>::kBytes, s>>>(p, prep, slices, tx, tb);
+    kern<<<grid * p.subs, kTcThreads, StateSmem<S_>::kBytes, s>>>(p, prep, slices, tx, tb);
     launch_pass(p, s);
   }
   auto kern = scan_tc_kernel<S_>;
@@ -830,7 +857,7 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
 size_t tc_scratch_bytes(const gdn_scan_args& a) { return static_cast<size_t>(a.B * a.T) * a.H * 3 * sizeof(float); }
 
 cudaError_t launch_tc(const ScanParams& p, const gdn_scan_args& a, float* scratch, cudaStream_t s) {
-  if (p.segments * p.H * (a.P / 64) > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  if (p.segments * p.subs * p.H * (a.P / 64) > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   return a.S == 128 ? run_tc<128>(p, a, scratch, s) : run_tc<64>(p, a, scratch, s);
 }
 

@@ -39,6 +39,9 @@ struct ScanParams {
   int* err;          // int32[4] device error word; zeroed by the call's first kernel
   int clear_err;
   int64_t T, N, total, seg, segments;
+  int64_t sub;  // the first pass works on pieces of a segment, of sub tokens each
+  int subs;     // pieces per segment: seg_state and seg_decay hold that many each
+
   int64_t sx, sdt, sb, sc, sz;  // token strides
   int H, P, G, S;
   int dt_dtype, init_dtype, final_dtype, cu_dtype, softplus;
