@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(256) scan_rec_kernel(const ScanParams p) {
   if (threadIdx.x < 32) {
     int64_t n = 0, ls = 0, t0 = 0, t1 = 0;
     bool last = false;
-    const bool ok = find_segment(p, id, n, ls, t0, t1, last);
+    int64_t chunk0 = 0;
+    const bool ok = find_segment(p, id, n, ls, t0, t1, last, chunk0);
     if (threadIdx.x == 0) {
       seg_n = n; seg_t0 = t0; seg_t1 = t1;
       seg_ok = ok; seg_last = last;

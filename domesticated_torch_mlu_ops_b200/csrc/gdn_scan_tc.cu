@@ -55,7 +55,8 @@ constexpr int kLead = kWork / 32;
 constexpr long long kWaitLimit = 2000000000LL;
 
 struct PrepOut {
-  float *a, *k, *dt;  // [H][tokens]
+  float *a, *k, *dt;  // [H][chunks][128]; past a sequence's end a stays, k and dt are 0
+  int64_t chunks;
 };
 
 template <int S_>
@@ -69,12 +70,12 @@ struct Smem {
   static constexpr int kXs = 2 * kStage;                    // first part of w x
   static constexpr int kH = kXs + kTile;                    // h, then the third part of w x
   static constexpr int kP = kH + kTile;
-  static constexpr int kCf = kP + 2 * kTile;                // k of one block of 32 tokens per warp
-  static constexpr int kBar = kCf + kWork / 32 * 32 * 4;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
+  static constexpr int kSc = kP + 2 * kTile;                // two stages of a and k
+  static constexpr int kBar = kSc + 2 * 2 * kL * 4;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
   static constexpr int kBars = 9;
   static constexpr int kTmem = kBar + kBars * 8;
   static constexpr int kBytes = kTmem + 8;
-  static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile;
+  static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile + 2 * kL * 4;
   static constexpr int kCols = 512, kYi = 256, kYa = 320, kDH = 384;  // TMEM columns: S[2] first
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
@@ -86,7 +87,8 @@ struct StateSmem {
   static constexpr int kBStage = S_ / 64 * kTile;
   static constexpr int kX = 3 * kBStage;
   static constexpr int kXs = kX + 2 * kTile;
-  static constexpr int kBar = kXs + 6 * kTile;  // B[3], x[2], parts ready[2], products[2]
+  static constexpr int kSc = kXs + 6 * kTile;   // two stages of a and k, with x
+  static constexpr int kBar = kSc + 2 * 2 * kL * 4;  // B[3], x[2], parts ready[2], products[2]
   static constexpr int kTmem = kBar + 9 * 8;
   static constexpr int kBytes = kTmem + 8;
   static constexpr int kCols = 64;
@@ -130,7 +132,8 @@ __global__ void __launch_bounds__(kPrepHeads * 32) scan_prep_kernel(const ScanPa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = blockIdx.y * kPrepHeads;
   int64_t n, ls, t0, t1;
   bool last;
-  if (!find_segment(p, blockIdx.x, n, ls, t0, t1, last)) return;  // p.seg is the chunk here
+  int64_t chunk0;
+  if (!find_segment(p, blockIdx.x, n, ls, t0, t1, last, chunk0)) return;  // p.seg is the chunk here
   const int len = static_cast<int>(t1 - t0);
   {
     constexpr int kTurns = kL / (2 * kPrepHeads);  // two tokens per warp and turn, all turns' loads together
@@ -176,43 +179,45 @@ __global__ void __launch_bounds__(kPrepHeads * 32) scan_prep_kernel(const ScanPa
     }
     dn = __shfl_down_sync(0xffffffffu, dn, 1, 8);
     if ((lane & 7) == 7) dn = 0.f;
-    const int64_t at = static_cast<int64_t>(h) * p.total + t0 + lane * 4;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane * 4 + e < len) {
-        o.a[at + e] = up + pre[e];
-        o.k[at + e] = exp2f(suf[e] + dn) * d[e];
-        o.dt[at + e] = d[e];
-      }
+    const int64_t at = (h * o.chunks + blockIdx.x) * kL + lane * 4;
+    float4 oa, ok;
+    oa = make_float4(up + pre[0], up + pre[1], up + pre[2], up + pre[3]);
+    if (len > 0 && len < kL) {
+      // past the end a is the last token's to the bit: the decay between the
+      // two is exactly 1, whatever the size of a (another lane's sum of the
+      // same terms may round otherwise)
+      const int e = (len - 1) & 3;
+      const float mine = e < 2 ? (e == 0 ? oa.x : oa.y) : (e == 2 ? oa.z : oa.w);
+      const float end = __shfl_sync(0xffffffffu, mine, (len - 1) >> 2);
+      if (lane * 4 >= len) oa.x = end;
+      if (lane * 4 + 1 >= len) oa.y = end;
+      if (lane * 4 + 2 >= len) oa.z = end;
+      if (lane * 4 + 3 >= len) oa.w = end;
+    }
+    ok = make_float4(ex2(suf[0] + dn) * d[0], ex2(suf[1] + dn) * d[1], ex2(suf[2] + dn) * d[2], ex2(suf[3] + dn) * d[3]);
+    *reinterpret_cast<float4*>(o.a + at) = oa;
+    *reinterpret_cast<float4*>(o.k + at) = ok;
+    *reinterpret_cast<float4*>(o.dt + at) = make_float4(d[0], d[1], d[2], d[3]);
   }
 }
 
-// Loads that stay where they are written, a chunk ahead of their use: the
-// compiler otherwise moves plain ones down to it and the full latency shows
-// (measured: 1-2 K cycles per chunk).
-__device__ __forceinline__ float ld_now(const float* p) {
+__device__ __forceinline__ float lds4(uint32_t a) {
   float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
   return v;
 }
 
-// What a thread (token `row` of a chunk) needs of a and k.
+// What a thread (token `row` of a chunk) needs of a and k, from their stage.
 struct TokenScalars {
-  float a, k;    // its own (0 past the end)
-  float end[4];  // a at the end of each block of 32 (of the chunk, past its end)
-};
-__device__ __forceinline__ TokenScalars load_scalars(const PrepOut& o, int64_t at, int len, int row) {
-  TokenScalars s;
-  const float *a = o.a + at, *k = o.k + at;
-  s.a = s.k = 0.f;
-  if (row < len) {
-    s.a = ld_now(a + row);
-    s.k = ld_now(k + row);
-  }
+  float a, k;    // its own
+  float end[4];  // a at the end of each block of 32
+  __device__ __forceinline__ void load(uint32_t at, int row) {
+    a = lds4(at + row * 4);
+    k = lds4(at + (kL + row) * 4);
 #pragma unroll
-  for (int b = 0; b < 4; ++b) s.end[b] = ld_now(a + min(b * 32 + 31, len - 1));
-  return s;
-}
+    for (int b = 0; b < 4; ++b) end[b] = lds4(at + (b * 32 + 31) * 4);
+  }
+};
 __device__ __forceinline__ float pick4(const float* v, int q) {
   return q < 2 ? (q == 0 ? v[0] : v[1]) : (q == 2 ? v[2] : v[3]);
 }
@@ -297,8 +302,11 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   const int g = h / (p.H / p.G);
   int64_t n = 0, ls = 0, t0 = 0, t1 = 0;
   bool last = false;
-  if (!find_segment(p, id, n, ls, t0, t1, last)) return;  // every warp finds the same
+  int64_t chunk0 = 0;
+  if (!find_segment(p, id, n, ls, t0, t1, last, chunk0)) return;  // every warp finds the same
+  const int64_t prow = (h * prep.chunks + chunk0) * kL;  // a, k, dt of the segment's first token
   const int nch = static_cast<int>((t1 - t0 + kL - 1) / kL);
+  if (chunk0 + nch > prep.chunks) return;  // sequences that overlap: more chunks than tokens
   const bool want_state = last && p.final_state;
   // an all-zero state needs no product
   const bool seg = p.seg_state != nullptr, ini = !seg && p.init;
@@ -343,6 +351,8 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       const uint32_t bar = bar_ld + (c & 1) * 8;
       uint8_t* st = sm + (c & 1) * M::kStage;
       umma::mbar_arrive_expect_tx(bar, M::kTx);
+      umma::bulk_g2s(sm + M::kSc + (c & 1) * 2 * kL * 4, prep.a + prow + c * kL, kL * 4, bar);
+      umma::bulk_g2s(sm + M::kSc + (c & 1) * 2 * kL * 4 + kL * 4, prep.k + prow + c * kL, kL * 4, bar);
 #pragma unroll
       for (int q = 0; q < S_ / 64; ++q) {
         umma::tma_load_2d(st + M::kC + q * kTile, &tcm, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
@@ -463,17 +473,10 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     const int row = quad * 32 + lane;           // token of the chunk, or state column s
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const Pieces piece(row, cq);
-    const uint32_t cf = sbase + M::kCf + warp * 128;
-    const int64_t prow = static_cast<int64_t>(h) * p.total + t0;
     const int64_t col = static_cast<int64_t>(h) * p.P + p0 + cq * 16;
     auto state_at = [&](int64_t i) { return ((i * p.H + h) * p.P + p0 + cq * 16) * S_ + row; };
     const float D = p.D ? p.D[h] : 0.f;
     TokenScalars sc;
-    float kj = 0.f;  // k of token 32 cq + lane
-    if (nch > 0) {
-      sc = load_scalars(prep, prow, length(0), row);
-      if (cq * 32 + lane < length(0)) kj = ld_now(prep.k + prow + cq * 32 + lane);
-    }
     float2 hr[8];  // h[s = row][16 columns of P]
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -496,6 +499,9 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     for (int c = 0; c < nch; ++c) {
       const int len = length(c);
       const uint32_t st = sbase + (c & 1) * M::kStage;
+      const uint32_t sc_at = sbase + M::kSc + (c & 1) * 2 * kL * 4;
+      if (!wait(bar_ld + (c & 1) * 8, (c >> 1) & 1, kSiteScanLoad)) break;
+      sc.load(sc_at, row);
       const float ai = sc.a, all = sc.end[3];
       const float wj = sc.k * ex2(all - pick4(sc.end, quad));
       // ---- P from the scores: block of columns J = cq ----
@@ -508,8 +514,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         const uint32_t ts = tl + (c & 1) * 128 + cq * 32;
         // far is largest in the block's first row: one answer per warp
         if (!diag || __shfl_sync(0xffffffffu, far, 0) < 100.f) {
-          asm volatile("st.shared.f32 [%0], %1;" :: "r"(cf + lane * 4), "f"(kj) : "memory");
-          __syncwarp();
+          const uint32_t cf = sc_at + (kL + cq * 32) * 4;
           const float f = ex2(far);
           const float2 f2 = make_float2(f, f);
 #pragma unroll
@@ -534,16 +539,14 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
               sts16(prow_at + ((((cq & 1) * 4 + hf * 2 + q) ^ (row & 7)) << 4), pack8(w));
             }
           }
-          __syncwarp();
         } else {
-          diag_by_difference(ts, prow_at, (cq & 1) * 4, row, ai, row < len ? __ldg(prep.dt + prow + c * kL + row) : 0.f);
+          diag_by_difference(ts, prow_at, (cq & 1) * 4, row, ai, __ldg(prep.dt + prow + c * kL + row));
         }
       } else if (c == 0) {  // nothing else is written there
 #pragma unroll
         for (int q = 0; q < 4; ++q) sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
       }
       // ---- w x in parts (x has been there since the scores were issued) ----
-      if (!wait(bar_ld + (c & 1) * 8, (c >> 1) & 1, kSiteScanLoad)) break;
       uint4 part[2], low[2];
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
@@ -578,12 +581,6 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         if (want_state) sts16(sbase + M::kH + piece.at[q], low[q]);
       }
       publish(bar_px);
-      if (c + 1 < nch) {
-        const int ln = length(c + 1);
-        sc = load_scalars(prep, prow + (c + 1) * kL, ln, row);
-        kj = 0.f;
-        if (cq * 32 + lane < ln) kj = ld_now(prep.k + prow + (c + 1) * kL + cq * 32 + lane);
-      }
       // ---- outputs ----
       if (p.z && !wait(bar_z, c & 1, kSiteScanLoad)) break;
       if (!wait(bar_y, c & 1, kSiteScanOut)) break;
@@ -664,10 +661,13 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   const int g = h / (p.H / p.G);
   int64_t n = 0, ls = 0, t0 = 0, t1 = 0;
   bool last = false;
-  if (!find_segment(p, id, n, ls, t0, t1, last) || last) return;
+  int64_t chunk0 = 0;
+  if (!find_segment(p, id, n, ls, t0, t1, last, chunk0) || last) return;
+  const int64_t prow = (h * prep.chunks + chunk0) * kL + (piece_id - id * p.subs) * p.sub;
   t0 += (piece_id - id * p.subs) * p.sub;  // a segment that is not the last is whole: pieces of whole chunks
   t1 = min64(t1, t0 + p.sub);
   const int nch = static_cast<int>((t1 - t0) / kL);
+  if (prow / kL + nch > (h + 1) * prep.chunks) return;  // sequences that overlap: more chunks than tokens
   if (warp == kLead) {
     if (umma::elect_one()) {
 #pragma unroll
@@ -700,8 +700,12 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
         umma::tma_load_2d(sm + (i % 3) * M::kBStage + q * kTile, &tb, g * S_ + q * 64, token(i), bar_b + (i % 3) * 8);
     };
     auto fetch_x = [&](int i) {
-      umma::mbar_arrive_expect_tx(bar_x + (i & 1) * 8, kTile);
-      umma::tma_load_2d(sm + M::kX + (i & 1) * kTile, &tx, h * p.P + p0, token(i), bar_x + (i & 1) * 8);
+      const uint32_t bar = bar_x + (i & 1) * 8;
+      uint8_t* sc = sm + M::kSc + (i & 1) * 2 * kL * 4;
+      umma::mbar_arrive_expect_tx(bar, kTile + 2 * kL * 4);
+      umma::bulk_g2s(sc, prep.a + prow + (nch - 1 - i) * kL, kL * 4, bar);
+      umma::bulk_g2s(sc + kL * 4, prep.k + prow + (nch - 1 - i) * kL, kL * 4, bar);
+      umma::tma_load_2d(sm + M::kX + (i & 1) * kTile, &tx, h * p.P + p0, token(i), bar);
     };
     if (umma::elect_one()) {
       fetch_x(0);
@@ -748,15 +752,14 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   } else {
     const int quad = warp & 3, cq = warp >> 2, row = quad * 32 + lane;
     const Pieces piece(row, cq);
-    const int64_t prow = static_cast<int64_t>(h) * p.total + t0;
     float later = 0.f;  // log2 decay from the chunk's end to the piece's
-    TokenScalars sc = load_scalars(prep, prow + (nch - 1) * kL, kL, row);
+    TokenScalars sc;
     for (int i = 0; i < nch; ++i) {
       const uint32_t xt = sbase + M::kX + (i & 1) * kTile, xs = sbase + M::kXs + (i & 1) * 3 * kTile;
+      if (!wait(bar_x + (i & 1) * 8, (i >> 1) & 1, kSiteScanLoad)) break;
+      sc.load(sbase + M::kSc + (i & 1) * 2 * kL * 4, row);
       const float wj = sc.k * ex2(sc.end[3] - pick4(sc.end, quad)) * ex2(later);
       later += sc.end[3];
-      if (i + 1 < nch) sc = load_scalars(prep, prow + (nch - 2 - i) * kL, kL, row);
-      if (!wait(bar_x + (i & 1) * 8, (i >> 1) & 1, kSiteScanLoad)) break;
       if (i >= 2 && !wait(bar_dh + (i & 1) * 8, ((i - 2) >> 1) & 1, kSiteScanState)) break;  // the parts' tiles are read
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -819,6 +822,12 @@ static cudaError_t make_rows_map(CUtensorMap* m, const void* ptr, int64_t cols, 
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Chunks of 128 tokens: every sequence has at most ceil(len / 128), and at least one.
+static int64_t prep_chunks(const gdn_scan_args& a) { return a.B * a.T / kL + a.N; }
+size_t tc_scratch_bytes(const gdn_scan_args& a) {
+  return static_cast<size_t>(prep_chunks(a)) * kL * a.H * 3 * sizeof(float);
+}
+
 template <int S_>
 static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, cudaStream_t s) {
   CUtensorMap tx, tb, tcm, ty, tz;
@@ -830,11 +839,12 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
   if ((e = make_rows_map(&ty, a.y, hp, total, hp)) != cudaSuccess) return e;
   if ((e = make_rows_map(&tz, a.z ? a.z : a.y, hp, total, a.z ? a.stride_z : hp)) != cudaSuccess) return e;
   const int slices = a.P / 64;
-  const PrepOut prep{scratch, scratch + total * a.H, scratch + 2 * total * a.H};
+  const int64_t chunks = prep_chunks(a), each = chunks * kL * a.H;
+  const PrepOut prep{scratch, scratch + each, scratch + 2 * each, chunks};
   ScanParams q = p;
   q.seg = kL;
   note_launch();
-  scan_prep_kernel<<<dim3(static_cast<unsigned>(total / kL + a.N), static_cast<unsigned>((a.H + kPrepHeads - 1) / kPrepHeads)),
+  scan_prep_kernel<<<dim3(static_cast<unsigned>(chunks), static_cast<unsigned>((a.H + kPrepHeads - 1) / kPrepHeads)),
                      kPrepHeads * 32, 0, s>>>(
       q, prep);
   const unsigned grid = static_cast<unsigned>(p.segments * p.H * slices);
@@ -854,7 +864,6 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
   return cudaGetLastError();
 }
 
-size_t tc_scratch_bytes(const gdn_scan_args& a) { return static_cast<size_t>(a.B * a.T) * a.H * 3 * sizeof(float); }
 
 cudaError_t launch_tc(const ScanParams& p, const gdn_scan_args& a, float* scratch, cudaStream_t s) {
   if (p.segments * p.subs * p.H * (a.P / 64) > 0x7fffffffLL) return cudaErrorInvalidConfiguration;

@@ -14,11 +14,26 @@ namespace scan {
 using conv::ld_any;
 using conv::st_any;
 
-// The step size: softplus(v) = max(v, 0) + log1p(exp(-|v|)), exact to a few
+// log(1 + e) for 0 <= e <= 1 by the series of the inverse hyperbolic tangent,
+// log(1 + e) = 2 (s + s^3/3 + s^5/5 + ...), s = e / (2 + e) <= 1/3: eight
+// terms leave a relative error under 2^-26.
+__device__ __forceinline__ float log1p_unit(float e) {
+  const float s = __fdividef(e, 2.f + e), q = s * s;
+  float r = 1.f / 15.f;
+  r = fmaf(r, q, 1.f / 13.f);
+  r = fmaf(r, q, 1.f / 11.f);
+  r = fmaf(r, q, 1.f / 9.f);
+  r = fmaf(r, q, 1.f / 7.f);
+  r = fmaf(r, q, 1.f / 5.f);
+  r = fmaf(r, q, 1.f / 3.f);
+  return 2.f * fmaf(s * q, r, s);
+}
+
+// The step size: softplus(v) = max(v, 0) + log(1 + exp(-|v|)), exact to a few
 // fp32 ulp for every v (the state may be compared in fp32).
 __device__ __forceinline__ float step_of(float raw, float bias, int softplus, float lo, float hi) {
   float v = raw + bias;
-  if (softplus) v = fmaxf(v, 0.f) + log1pf(expf(-fabsf(v)));
+  if (softplus) v = fmaxf(v, 0.f) + log1p_unit(expf(-fabsf(v)));
   v = v < lo ? lo : v;  // a NaN stays one
   return v > hi ? hi : v;
 }
@@ -56,40 +71,48 @@ __device__ __forceinline__ void clear_error(const ScanParams& p) {
 
 // Segment `id` of the batch: segment `ls` of sequence n, tokens [t0, t1);
 // `last` when it is the sequence's last.  An empty sequence has one empty
-// segment.  Called by one warp (all lanes); false past the last segment.
+// segment.  `chunk0` is the segment's first 128-token chunk, counted over the
+// batch (an empty sequence counts as one).  Called by whole warps; false past
+// the last segment.
 __device__ __forceinline__ bool find_segment(const ScanParams& p, int64_t id, int64_t& n, int64_t& ls, int64_t& t0,
-                                             int64_t& t1, bool& last) {
+                                             int64_t& t1, bool& last, int64_t& chunk0) {
   const int lane = threadIdx.x & 31;
-  int64_t base = 0;
+  int64_t base = 0, base_ch = 0;
   for (int64_t n0 = 0; n0 < p.N; n0 += 32) {
-    int64_t bos = 0, eos = 0, mine = 0;
+    int64_t bos = 0, eos = 0, mine = 0, mine_ch = 0;
     if (n0 + lane < p.N) {
       seq_bounds(p.cu, p.cu_dtype, n0 + lane, p.T, bos, eos);
       bos = min64(max(bos, static_cast<int64_t>(0)), p.total);
       eos = min64(max(eos, bos), p.total);
       mine = max((eos - bos + p.seg - 1) / p.seg, static_cast<int64_t>(1));
+      mine_ch = max((eos - bos + 127) / 128, static_cast<int64_t>(1));
     }
-    int64_t incl = mine;
+    int64_t incl = mine, incl_ch = mine_ch;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o), w = __shfl_up_sync(0xffffffffu, incl_ch, o);
+      if (lane >= o) {
+        incl += v;
+        incl_ch += w;
+      }
     }
     const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
     if (id < base + total) {
       const unsigned hit = __ballot_sync(0xffffffffu, id < base + incl);
       const int src = __ffs(hit) - 1;
       n = n0 + src;
-      ls = id - base - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src));
+      ls = id - base - __shfl_sync(0xffffffffu, incl - mine, src);
       const int64_t count = __shfl_sync(0xffffffffu, mine, src);
       bos = __shfl_sync(0xffffffffu, bos, src);
       eos = __shfl_sync(0xffffffffu, eos, src);
       t0 = bos + ls * p.seg;
       t1 = min64(eos, t0 + p.seg);
       last = ls + 1 == count;
+      chunk0 = base_ch + __shfl_sync(0xffffffffu, incl_ch - mine_ch, src) + (t0 - bos) / 128;
       return true;
     }
     base += total;
+    base_ch += __shfl_sync(0xffffffffu, incl_ch, 31);
   }
   return false;
 }
