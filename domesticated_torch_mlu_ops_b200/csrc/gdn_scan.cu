@@ -19,6 +19,7 @@ namespace gdn {
 namespace scan {
 
 constexpr int kTok = 16;  // tokens staged together
+constexpr int kUpdWarps = 4;
 
 // One CTA per (segment, head, slice of ROWS state rows).  LPR lanes share a
 // state row; each holds SPT of its columns (columns i*4*LPR + 4*lane + e, so
@@ -222,9 +223,9 @@ struct UpdateParams {
 // columns each, ITER times); a warp moves R rows at a time, all of whose
 // loads are in flight together.
 template <typename T, typename CT, int VEC, int LPR, int ITER, int R>
-__global__ void __launch_bounds__(128) scan_update_kernel(const UpdateParams p) {
+__global__ void __launch_bounds__(kUpdWarps * 32) scan_update_kernel(const UpdateParams p) {
   constexpr int RW = 32 / LPR;  // rows side by side in a warp
-  constexpr int BLK = 4 * RW * R;
+  constexpr int BLK = kUpdWarps * RW * R;
   const int64_t n = blockIdx.z;
   const int h = blockIdx.y, g = h / (p.H / p.G);
   const int lane = threadIdx.x % LPR, sub = (threadIdx.x & 31) / LPR, warp = threadIdx.x >> 5;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(128) scan_update_kernel(const UpdateParams p) 
   if (slot < 0 || slot >= p.slots) {  // padding, or an index out of the cache: no state, output zero
     if (slot >= p.slots && threadIdx.x == 0 && blockIdx.x == 0 && h == 0)
       record_device_error(p.err, kErrSlotRange, kSiteSlotInitial, static_cast<int>(n), static_cast<int>(slot));
-    for (int r = threadIdx.x; r < BLK; r += 128)
+    for (int r = threadIdx.x; r < BLK; r += kUpdWarps * 32)
       if (blockIdx.x * BLK + r < p.P) y[blockIdx.x * BLK + r] = from_f<T>(0.f);
     return;
   }
@@ -334,18 +335,20 @@ struct Plan {
 
 // Segment length: enough (segment, head, row slice) CTAs to fill the GPU (one
 // per SM on the tensor cores, four of the recurrent kernel), but no segment
-// under `least` tokens (below it the passes over states cost more than the
-// tokens).  Without a device query, so the result depends on the shapes alone.
+// under `least` tokens, below which handing states on costs more than it
+// saves: four chunks on the tensor cores, 64 tokens (about 15 us of the
+// recurrence) otherwise.  Without a device query, so the result depends on
+// the shapes alone.
 Plan plan(const gdn_scan_args& a) {
   Plan pl{};
   const bool tc = tc_shape(a);
   const int64_t total = a.B * a.T;
   const int64_t slices = tc ? tc_slices(a) : (a.P + 63) / 64;
-  const int64_t want = 148 * (tc ? 1 : 4), least = 512;
+  const int64_t want = 148 * (tc ? 1 : 4), least = tc ? 512 : 64, unit = tc ? 128 : kTok;
   const int64_t per_token = std::max<int64_t>(1, a.H * slices);
   const int64_t pieces = std::max<int64_t>(1, want / per_token);
   pl.seg = std::max(least, (total + pieces - 1) / pieces);
-  pl.seg = (pl.seg + 127) / 128 * 128;
+  pl.seg = (pl.seg + unit - 1) / unit * unit;
   pl.split = a.N > 0 && a.N * per_token < want && total > least;
   if (!pl.split) pl.seg = std::max<int64_t>(128, (total + 127) / 128 * 128);
   // every sequence has at most ceil(len / seg) segments, and at least one
@@ -404,13 +407,24 @@ void launch_pass(const ScanParams& p, cudaStream_t s) {
 
 template <typename T, typename CT, int VEC, int LPR, int ITER, int R>
 void launch_upd(const UpdateParams& p, cudaStream_t s) {
-  constexpr int BLK = 4 * (32 / LPR) * R;
+  constexpr int BLK = kUpdWarps * (32 / LPR) * R;
   const dim3 grid(static_cast<unsigned>((p.P + BLK - 1) / BLK), static_cast<unsigned>(p.H), static_cast<unsigned>(p.N));
-  scan_update_kernel<T, CT, VEC, LPR, ITER, R><<<grid, 128, 0, s>>>(p);
+  scan_update_kernel<T, CT, VEC, LPR, ITER, R><<<grid, kUpdWarps * 32, 0, s>>>(p);
 }
 
-// Lanes per row: S in 16-byte vectors where the rows allow them, else
-// single columns.
+// Four or five rows per warp, whichever leaves fewer of a CTA's rows idle
+// (77 tokens of 40 heads of 80 rows on 16-bit lines: 16 us with five, 20 with
+// four, which fills a second CTA's row slots to a quarter).
+template <typename T, typename CT, int VEC, int LPR>
+void launch_rows(const UpdateParams& p, cudaStream_t s) {
+  constexpr int four = kUpdWarps * (32 / LPR) * 4, five = kUpdWarps * (32 / LPR) * 5;
+  if ((p.P + five - 1) / five * five < (p.P + four - 1) / four * four) launch_upd<T, CT, VEC, LPR, 1, 5>(p, s);
+  else launch_upd<T, CT, VEC, LPR, 1, 4>(p, s);
+}
+
+// Lanes per row: S in 16-byte vectors where the rows allow them, else single
+// columns; four rows per warp in flight (256 tokens on fp32 lines of 64 heads
+// x 64 x 128: 177 us, against 187 with eight rows, 212 with 16 and 262 with two).
 template <typename T, typename CT>
 void update_t(const UpdateParams& p, cudaStream_t s) {
   constexpr int V = 16 / sizeof(CT);
@@ -418,9 +432,9 @@ void update_t(const UpdateParams& p, cudaStream_t s) {
   if (vec) {
     const int n = p.S / V;
     if (n <= 4) launch_upd<T, CT, V, 4, 1, 4>(p, s);
-    else if (n <= 8) launch_upd<T, CT, V, 8, 1, 4>(p, s);
-    else if (n <= 16) launch_upd<T, CT, V, 16, 1, 4>(p, s);
-    else if (n <= 32) launch_upd<T, CT, V, 32, 1, 8>(p, s);
+    else if (n <= 8) launch_rows<T, CT, V, 8>(p, s);
+    else if (n <= 16) launch_rows<T, CT, V, 16>(p, s);
+    else if (n <= 32) launch_upd<T, CT, V, 32, 1, 4>(p, s);
     else launch_upd<T, CT, V, 32, 2, 4>(p, s);
   } else {
     if (p.S <= 32) launch_upd<T, CT, 1, 32, 1, 8>(p, s);

@@ -581,32 +581,50 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         if (want_state) sts16(sbase + M::kH + piece.at[q], low[q]);
       }
       publish(bar_px);
-      // ---- outputs ----
-      if (p.z && !wait(bar_z, c & 1, kSiteScanLoad)) break;
-      if (!wait(bar_y, c & 1, kSiteScanOut)) break;
-      umma::fence_after_sync();
+      // ---- outputs: first what does not need Ya (whose product runs now) ----
+      float2 part_y[8], gz[8];
       {
         const float g1 = ex2(ai);
         const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
         const bool has_yi = c > 0 || seg || ini;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          float yi[8], ya[8];
-          umma::tmem_ld8x2(tl + M::kYi + cq * 16 + q * 8, tl + M::kYa + cq * 16 + q * 8, yi, ya);
-          float2 xv[4], zv[4], o[4];
-          unpack8(lds16(st + M::kX + piece.at[q]), xv);
-          if (p.z) unpack8(lds16(st + M::kZ + piece.at[q]), zv);
+          unpack8(lds16(st + M::kX + piece.at[q]), part_y + q * 4);
+          float yi[8];
+          if (has_yi) umma::tmem_ld8(tl + M::kYi + cq * 16 + q * 8, yi);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 a2 = make_float2(ya[e * 2], ya[e * 2 + 1]);
-            // without a state Yi was not computed: its columns hold anything
-            o[e] = has_yi ? __ffma2_rn(g2, make_float2(yi[e * 2], yi[e * 2 + 1]), a2) : a2;
-            o[e] = __ffma2_rn(D2, xv[e], o[e]);
-            if (p.z) {
-              float zz[2] = {zv[e].x, zv[e].y};
-              conv::silu_vec<__nv_bfloat16, 2>(zz);
-              o[e] = __fmul2_rn(o[e], make_float2(zz[0], zz[1]));
-            }
+            part_y[q * 4 + e] = __fmul2_rn(D2, part_y[q * 4 + e]);
+            if (has_yi) part_y[q * 4 + e] = __ffma2_rn(g2, make_float2(yi[e * 2], yi[e * 2 + 1]), part_y[q * 4 + e]);
+          }
+        }
+      }
+      if (p.z) {
+        if (!wait(bar_z, c & 1, kSiteScanLoad)) break;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          unpack8(lds16(st + M::kZ + piece.at[q]), gz + q * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float zz[2] = {gz[q * 4 + e].x, gz[q * 4 + e].y};
+            conv::silu_vec<__nv_bfloat16, 2>(zz);
+            gz[q * 4 + e] = make_float2(zz[0], zz[1]);
+          }
+        }
+      }
+      if (!wait(bar_y, c & 1, kSiteScanOut)) break;
+      umma::fence_after_sync();
+      {
+        float ya[16];
+        umma::tmem_ld16(tl + M::kYa + cq * 16, ya);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float2 o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = q * 8 + e * 2;
+            o[e] = __fadd2_rn(part_y[q * 4 + e], make_float2(ya[i], ya[i + 1]));
+            if (p.z) o[e] = __fmul2_rn(o[e], gz[q * 4 + e]);
           }
           const uint4 u = pack8(o);
           if (len == kL) {
