@@ -74,7 +74,8 @@ struct Smem {
   static constexpr int kBar = kSc + 2 * 2 * kL * 4;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
   static constexpr int kBars = 9;
   static constexpr int kTmem = kBar + kBars * 8;
-  static constexpr int kBytes = kTmem + 8;
+  static constexpr int kBad = kTmem + 8;                    // [2][64 columns + 1]: see the kernel
+  static constexpr int kBytes = kBad + 2 * 65 * 4;
   static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile + 2 * kL * 4;
   static constexpr int kCols = 512, kYi = 256, kYa = 320, kDH = 384;  // TMEM columns: S[2] first
   static_assert(kBytes <= 227 * 1024, "shared memory");
@@ -280,6 +281,35 @@ __device__ __noinline__ void diag_by_difference(uint32_t ts, uint32_t prow_at, i
   }
 }
 
+// Non-zero when one of two bf16 values is infinite or NaN.
+__device__ __forceinline__ uint32_t all_ones_exponent(uint32_t w) {
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+// A thread's 16 columns of x with infinities or NaN: notes them and zeroes
+// them in the operand's tile.
+__device__ __forceinline__ void mark_not_finite(uint32_t tile, uint32_t at0, int* bad, int row, int chunk) {
+#pragma unroll 1
+  for (int e = 0; e < 16; ++e) {
+    const uint32_t at = tile + (at0 ^ ((e >> 3) * 16)) + (e & 7) * 2;
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    if ((v & 0x7f80) != 0x7f80) continue;
+    asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(static_cast<uint16_t>(0)) : "memory");
+    atomicMax(bad + e, (chunk + 1) * 256 + 255 - row);
+  }
+}
+// Token `row`'s outputs (in the tile, or at y) that follow a bad x: NaN.
+__device__ __forceinline__ void nan_after(uint32_t tile, uint32_t at0, const int* bad, int row, int chunk, __nv_bfloat16* y) {
+#pragma unroll 1
+  for (int e = 0; e < 16; ++e) {
+    const int v = *reinterpret_cast<const volatile int*>(bad + e);
+    if ((v >> 8) != chunk + 1 || row < 255 - (v & 255)) continue;
+    const uint16_t nan = 0x7fc0;
+    if (y) *reinterpret_cast<uint16_t*>(y + e) = nan;
+    else asm volatile("st.shared.u16 [%0], %1;" :: "r"(tile + (at0 ^ ((e >> 3) * 16)) + (e & 7) * 2), "h"(nan) : "memory");
+  }
+}
+
 template <int S_>
 __global__ void __launch_bounds__(kTcThreads, 1)
 scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const __grid_constant__ CUtensorMap tx,
@@ -322,6 +352,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     umma::tmem_alloc(tslot, M::kCols);
     umma::fence_before_sync();
   }
+  // An infinite or NaN x would reach earlier tokens of its chunk through P's
+  // zeros.  It is 0 as Ya's operand, and its column's outputs from its token on
+  // are NaN: bad[chunk parity][column] = (chunk + 1) * 256 + 255 - first such
+  // token, and [64] the last chunk that has any.
+  int* bad = reinterpret_cast<int*>(sm + M::kBad);
+  if (tid < 2 * 65) bad[tid] = 0;
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tslot, 0);
@@ -549,6 +585,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       // ---- w x in parts (x has been there since the scores were issued) ----
       uint4 part[2], low[2];
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      uint32_t not_finite = 0;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         uint4 u = lds16(st + M::kX + piece.at[q]);
@@ -556,6 +593,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
           u = zero;
           sts16(st + M::kX + piece.at[q], zero);
         }
+        not_finite |= all_ones_exponent(u.x) | all_ones_exponent(u.y) | all_ones_exponent(u.z) | all_ones_exponent(u.w);
         float2 v[4];
         unpack8(u, v);
 #pragma unroll
@@ -567,6 +605,11 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         } else {
           part[q] = pack8(v);
         }
+      }
+      if (__any_sync(0xffffffffu, not_finite != 0)) {
+        if (not_finite) mark_not_finite(st + M::kX, piece.at[0], bad + (c & 1) * 65 + cq * 16, row, c);
+        if (lane == 0) atomicMax(bad + (c & 1) * 65 + 64, c + 1);
+        __syncwarp();
       }
       if (row >= len)
 #pragma unroll
@@ -647,6 +690,9 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
           hr[j] = __ffma2_rn(make_float2(decay, decay), hr[j], make_float2(d[j * 2], d[j * 2 + 1]));
       }
       store_h();
+      if (*reinterpret_cast<volatile int*>(bad + (c & 1) * 65 + 64) == c + 1 && row < len)
+        nan_after(st + M::kX, piece.at[0], bad + (c & 1) * 65 + cq * 16, row, c,
+                  len == kL ? nullptr : static_cast<__nv_bfloat16*>(p.y) + (t0 + static_cast<int64_t>(c) * kL + row) * p.H * p.P + col);
       publish(bar_h);
     }
     if (mine && row < S_ && want_state)

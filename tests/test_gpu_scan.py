@@ -376,3 +376,27 @@ def test_refusals():
         upd(state=line[:3])
     with pytest.raises(ValueError, match="ssm_state_indices"):
         upd(state=line, ssm_state_indices=torch.zeros(3, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("generic", [False, True])
+@pytest.mark.parametrize("what", ["x", "B", "C", "dt", "z"])
+def test_later_tokens_stay_out_of_earlier_ones(what, generic):
+    """A NaN or infinity at one token of a sequence reaches no earlier output."""
+    lens = [300, 130]
+    i = make(sum(lens), 2, 64, 1, 128, bf16, True, seed=17)
+    clean, _ = run(i, lens, force_generic=generic)
+    for bad, at in ((float("nan"), 70), (float("inf"), 200), (float("-inf"), 429)):
+        j = dict(i)
+        base = i[what]._base.clone()
+        j[what] = base.as_strided(i[what].shape, i[what].stride(), i[what].storage_offset())
+        j[what][at].flatten()[:1] = bad  # one column (or the head's step) of one token
+        start = 0 if at < 300 else 300
+        y, h = run(j, lens, force_generic=generic)
+        assert torch.equal(y[start:at], clean[start:at])
+        other = slice(300, 430) if at < 300 else slice(0, 300)
+        assert torch.equal(y[other], clean[other])
+        if what in ("x", "C", "z"):
+            assert not torch.isfinite(y[at].float()).all()
+        if what == "x":  # the other columns of the head never see it; its own state does
+            assert torch.equal(y[:, 0, 1:], clean[:, 0, 1:]) and torch.equal(y[:, 1], clean[:, 1])
+            assert not torch.isfinite(h[0 if at < 300 else 1, 0, 0]).any()
