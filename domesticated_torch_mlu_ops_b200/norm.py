@@ -65,17 +65,12 @@ def _two_strides(x, z):
     return x, z, hx, sxt, sxh, szt, szh
 
 
-def _empty(dev, dtype):
-    return torch.empty(0, dtype=dtype, device=dev)
-
-
-def _norm_fwd_impl(x: Tensor, weight: Tensor, z: Optional[Tensor], residual: Optional[Tensor], eps: float,
-                   group_size: int, norm_before_gate: bool, zero_centered: bool, residual_scale: float,
-                   activation: int) -> tuple[Tensor, Tensor]:
-    """Returns ``(y, sum)``; sum is empty without a residual."""
+def _norm_fwd_impl(x, weight, z, residual, eps, group_size, norm_before_gate, zero_centered, residual_scale,
+                   activation):
+    """Returns ``(y, sum)``; sum is None without a residual."""
     dev = x.device
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    total = _empty(dev, x.dtype) if residual is None else torch.empty_like(residual)
+    total = None if residual is None else torch.empty_like(residual)
     if x.numel() == 0:
         return y, total
     D = x.shape[-1]
@@ -83,14 +78,21 @@ def _norm_fwd_impl(x: Tensor, weight: Tensor, z: Optional[Tensor], residual: Opt
     dt = _DT[x.dtype]
     packed = _lib.pack_norm(
         x.data_ptr(), _addr(z), _addr(residual), weight.data_ptr(), y.data_ptr(),
-        0 if residual is None else total.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, x.numel() // D, heads, D, sxt, sxh, szt, szh,
+        _addr(total), 0, 0, 0, 0, 0, 0, 0, 0, x.numel() // D, heads, D, sxt, sxh, szt, szh,
         group_size, dt, dt, dt if residual is None else _DT[residual.dtype], _DT[weight.dtype], not norm_before_gate,
         zero_centered, activation, eps, residual_scale)
     _launch(_lib.load().gdn_norm_fwd, packed, dev)
     return y, total
 
 
-_norm_fwd_op = torch.library.custom_op("gdn_b200::norm_fwd", mutates_args=(), device_types="cuda")(_norm_fwd_impl)
+@torch.library.custom_op("gdn_b200::norm_fwd", mutates_args=(), device_types="cuda")
+def _norm_fwd_op(x: Tensor, weight: Tensor, z: Optional[Tensor], residual: Optional[Tensor], eps: float,
+                 group_size: int, norm_before_gate: bool, zero_centered: bool, residual_scale: float,
+                 activation: int) -> tuple[Tensor, Tensor]:
+    """The sum is empty without a residual."""
+    y, total = _norm_fwd_impl(x, weight, z, residual, eps, group_size, norm_before_gate, zero_centered, residual_scale,
+                              activation)
+    return y, x.new_empty((0,)) if total is None else total
 
 
 @_norm_fwd_op.register_fake
@@ -108,15 +110,14 @@ def _bwd_workspace(rows, D, group, dtype, x_dtype):
     return n
 
 
-def _norm_bwd_impl(dy: Tensor, x: Tensor, weight: Tensor, z: Optional[Tensor], dsum: Optional[Tensor],
-                   want_dresidual: bool, eps: float, group_size: int, norm_before_gate: bool, zero_centered: bool,
-                   residual_scale: float, activation: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    """Returns ``(dx, dweight, dz, dresidual)``; the last two are empty when
+def _norm_bwd_impl(dy, x, weight, z, dsum, want_dresidual, eps, group_size, norm_before_gate, zero_centered,
+                   residual_scale, activation):
+    """Returns ``(dx, dweight, dz, dresidual)``; the last two are None when
     there is no z or dresidual is not wanted."""
     dev = dy.device
     dx = torch.empty_like(dy)  # dy is contiguous
-    dz = _empty(dev, dy.dtype) if z is None else torch.empty_like(dy)
-    dres = torch.empty_like(dy, dtype=x.dtype) if want_dresidual else _empty(dev, x.dtype)
+    dz = None if z is None else torch.empty_like(dy)
+    dres = torch.empty_like(dy, dtype=x.dtype) if want_dresidual else None
     if x.numel() == 0:
         return dx, torch.zeros_like(weight), dz, dres
     dw = torch.empty_like(weight)
@@ -127,14 +128,21 @@ def _norm_bwd_impl(dy: Tensor, x: Tensor, weight: Tensor, z: Optional[Tensor], d
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     packed = _lib.pack_norm(
         x.data_ptr(), _addr(z), 0, weight.data_ptr(), 0, 0, dy.data_ptr(), _addr(dsum), dx.data_ptr(),
-        0 if z is None else dz.data_ptr(), dres.data_ptr() if want_dresidual else 0, dw.data_ptr(), ws.data_ptr(), nbytes,
+        _addr(dz), _addr(dres), dw.data_ptr(), ws.data_ptr(), nbytes,
         rows, heads, D, sxt, sxh, szt, szh, group_size, dt, xt, xt, _DT[weight.dtype], not norm_before_gate,
         zero_centered, activation, eps, residual_scale)
     _launch(_lib.load().gdn_norm_bwd, packed, dev)
     return dx, dw, dz, dres
 
 
-_norm_bwd_op = torch.library.custom_op("gdn_b200::norm_bwd", mutates_args=(), device_types="cuda")(_norm_bwd_impl)
+@torch.library.custom_op("gdn_b200::norm_bwd", mutates_args=(), device_types="cuda")
+def _norm_bwd_op(dy: Tensor, x: Tensor, weight: Tensor, z: Optional[Tensor], dsum: Optional[Tensor],
+                 want_dresidual: bool, eps: float, group_size: int, norm_before_gate: bool, zero_centered: bool,
+                 residual_scale: float, activation: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """dz and dresidual are empty when there is no z or dresidual is not wanted."""
+    dx, dw, dz, dres = _norm_bwd_impl(dy, x, weight, z, dsum, want_dresidual, eps, group_size, norm_before_gate,
+                                      zero_centered, residual_scale, activation)
+    return dx, dw, dy.new_empty((0,)) if dz is None else dz, x.new_empty((0,)) if dres is None else dres
 
 
 @_norm_bwd_op.register_fake

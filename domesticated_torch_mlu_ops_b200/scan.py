@@ -175,8 +175,10 @@ def _check(name, lead, x, dt, A, B, C, D, z, dt_bias, dt_limit):
 
 
 def _no_grad(name, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise ValueError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
 def chunk_selective_scan(
