@@ -21,17 +21,28 @@ namespace scan {
 constexpr int kTok = 16;  // tokens staged together
 constexpr int kUpdWarps = 4;
 
+// Raw inputs of one tile of kTok tokens, on their way to shared memory.
+template <typename T, int NB, int NX, bool OUT>
+struct RecTile {
+  pk::Raw<T, 1> b[NB], c[OUT ? NB : 1], x[NX], z[OUT ? NX : 1];
+  float dt;
+};
+
 // One CTA per (segment, head, slice of ROWS state rows).  LPR lanes share a
 // state row; each holds SPT of its columns (columns i*4*LPR + 4*lane + e, so
 // that the lanes read 16-byte pieces of B and C side by side).  Per token and
-// thread: 2 SPT multiply-adds for the state, SPT for the output, a shuffle
-// reduction over LPR lanes.  Everything in fp32; issue-bound.
+// thread: SPT packed multiply-adds for the state and half as many for the
+// output, and three shuffles per four tokens that leave each of four lanes
+// with one token's sum.  Everything in fp32.  A tile's inputs are loaded
+// while the tile before it is computed; a tail is padded to four tokens of
+// step zero (decay 1, nothing added).
 template <typename T, int SPT, int LPR, bool OUT>
-__global__ void __launch_bounds__(256) scan_rec_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
   constexpr int SP = SPT * LPR;  // padded state width
   constexpr int ROWS = 256 / LPR;
-  __shared__ __align__(16) float sb[kTok][SP], sc[OUT ? kTok : 1][SP];
-  __shared__ float sx[kTok][ROWS + 1], sy[OUT ? kTok : 1][ROWS + 1], sdt[kTok], sda[kTok], sdecay[kTok];
+  constexpr int NB = kTok * SP / 256, NX = kTok * ROWS / 256;
+  __shared__ __align__(16) float sb[kTok][SP], sc[OUT ? kTok : 1][SP], sdt[kTok], sda[kTok], sdecay[kTok];
+  __shared__ float sx[kTok][ROWS + 8], sy[OUT ? kTok : 1][ROWS + 8];
   __shared__ int64_t seg_n, seg_t0, seg_t1;
   __shared__ int seg_ok, seg_last;
   const int64_t id = blockIdx.x;
@@ -55,80 +66,123 @@ __global__ void __launch_bounds__(256) scan_rec_kernel(const ScanParams p) {
   const int lane = threadIdx.x % LPR, r = threadIdx.x / LPR, row = row0 + r;
   const bool live = row < p.P;
   const float A = p.A[h], D = p.D ? p.D[h] : 0.f, bias = p.dt_bias ? p.dt_bias[h] : 0.f;
-  float st[SPT];
+  const T* bp = static_cast<const T*>(p.b) + static_cast<int64_t>(g) * p.S;
+  const T* cp = static_cast<const T*>(p.c) + static_cast<int64_t>(g) * p.S;
+  const int64_t col0 = static_cast<int64_t>(h) * p.P + row0;
+  RecTile<T, NB, NX, OUT> in;
+  auto fetch = [&](int64_t t, int cnt) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int i = threadIdx.x + j * 256, k = i / SP, s = i % SP;
+      if (k < cnt && s < p.S) {
+        pk::load(in.b[j], bp + (t + k) * p.sb + s);
+        if (OUT) pk::load(in.c[j], cp + (t + k) * p.sc + s);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+      const int i = threadIdx.x + j * 256, k = i / ROWS, q = i % ROWS;
+      if (k < cnt && row0 + q < p.P) {
+        pk::load(in.x[j], static_cast<const T*>(p.x) + (t + k) * p.sx + col0 + q);
+        if (OUT && p.z) pk::load(in.z[j], static_cast<const T*>(p.z) + (t + k) * p.sz + col0 + q);
+      }
+    }
+    if (threadIdx.x < cnt) in.dt = ld_any(p.dt, p.dt_dtype, (t + threadIdx.x) * p.sdt + h);
+  };
+  int cnt = static_cast<int>(min64(kTok, t1 - t0));
+  if (t0 < t1) fetch(t0, cnt);
+  float2 st[SPT / 2];
   const int64_t at_seq = ((n * p.H + h) * p.P + row) * p.S;
   const int64_t at_seg = ((id * p.H + h) * p.P + row) * p.S;
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
-    st[i] = 0.f;
+    float v = 0.f;
     if (OUT && live && s < p.S) {
-      if (p.seg_state) st[i] = p.seg_state[at_seg + s];
-      else if (p.init) st[i] = ld_any(p.init, p.init_dtype, at_seq + s);
+      if (p.seg_state) v = p.seg_state[at_seg + s];
+      else if (p.init) v = ld_any(p.init, p.init_dtype, at_seq + s);
     }
+    if (i & 1) st[i / 2].y = v;
+    else st[i / 2].x = v;
   }
   float logd = 0.f;
   for (int64_t t = t0; t < t1; t += kTok) {
-    const int cnt = static_cast<int>(min64(kTok, t1 - t));
-    for (int i = threadIdx.x; i < kTok * SP; i += 256) {
-      const int k = i / SP, s = i % SP;
-      const bool in = k < cnt && s < p.S;
-      sb[k][s] = in ? to_f<T>(static_cast<const T*>(p.b)[(t + k) * p.sb + static_cast<int64_t>(g) * p.S + s]) : 0.f;
-      if (OUT) sc[k][s] = in ? to_f<T>(static_cast<const T*>(p.c)[(t + k) * p.sc + static_cast<int64_t>(g) * p.S + s]) : 0.f;
+    __syncthreads();  // the tile before this one has been read
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int i = threadIdx.x + j * 256, k = i / SP, s = i % SP;
+      const bool there = k < cnt && s < p.S;
+      sb[k][s] = there ? pk::widen<T, 1>(in.b[j]).s : 0.f;
+      if (OUT) sc[k][s] = there ? pk::widen<T, 1>(in.c[j]).s : 0.f;
     }
-    for (int i = threadIdx.x; i < kTok * ROWS; i += 256) {
-      const int k = i / ROWS, q = i % ROWS;
-      sx[k][q] = k < cnt && row0 + q < p.P
-                     ? to_f<T>(static_cast<const T*>(p.x)[(t + k) * p.sx + static_cast<int64_t>(h) * p.P + row0 + q])
-                     : 0.f;
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+      const int i = threadIdx.x + j * 256, k = i / ROWS, q = i % ROWS;
+      sx[k][q] = k < cnt && row0 + q < p.P ? pk::widen<T, 1>(in.x[j]).s : 0.f;
     }
     if (threadIdx.x < kTok) {
-      float d = 0.f;
-      if (threadIdx.x < cnt)
-        d = step_of(ld_any(p.dt, p.dt_dtype, (t + threadIdx.x) * p.sdt + h), bias, p.softplus, p.dt_lo, p.dt_hi);
+      const bool there = threadIdx.x < cnt;
+      const float d = there ? step_of(in.dt, bias, p.softplus, p.dt_lo, p.dt_hi) : 0.f, a = there ? d * A : 0.f;
       sdt[threadIdx.x] = d;
-      sda[threadIdx.x] = d * A;
-      sdecay[threadIdx.x] = expf(d * A);
+      sda[threadIdx.x] = a;
+      sdecay[threadIdx.x] = expf(a);
     }
     __syncthreads();
-    for (int k = 0; k < cnt; ++k) {
-      const float decay = sdecay[k], u = sdt[k] * sx[k][r];
-      logd += sda[k];
-      float acc = 0.f;
-#pragma unroll
-      for (int i = 0; i < SPT; i += 4) {
-        const int s = i * LPR + lane * 4;
-        const float4 bv = *reinterpret_cast<const float4*>(&sb[k][s]);
-        st[i] = fmaf(decay, st[i], u * bv.x);
-        st[i + 1] = fmaf(decay, st[i + 1], u * bv.y);
-        st[i + 2] = fmaf(decay, st[i + 2], u * bv.z);
-        st[i + 3] = fmaf(decay, st[i + 3], u * bv.w);
-        if (OUT) {
-          const float4 cv = *reinterpret_cast<const float4*>(&sc[k][s]);
-          acc = fmaf(st[i], cv.x, acc);
-          acc = fmaf(st[i + 1], cv.y, acc);
-          acc = fmaf(st[i + 2], cv.z, acc);
-          acc = fmaf(st[i + 3], cv.w, acc);
-        }
-      }
-      if (OUT) {
-        acc = group_sum<LPR>(acc);
-        if (lane == 0) sy[k][r] = fmaf(D, sx[k][r], acc);
-      }
-    }
-    __syncthreads();
+    const int now = cnt;
+    pk::Raw<T, 1> z[OUT ? NX : 1];
     if (OUT) {
-      for (int i = threadIdx.x; i < cnt * ROWS; i += 256) {
-        const int k = i / ROWS, q = i % ROWS;
-        if (row0 + q >= p.P) continue;
-        float v = sy[k][q];
-        const int64_t col = static_cast<int64_t>(h) * p.P + row0 + q;
-        if (p.z) v *= silu(to_f<T>(static_cast<const T*>(p.z)[(t + k) * p.sz + col]));
-        static_cast<T*>(p.y)[(t + k) * p.H * p.P + col] = from_f<T>(v);
+#pragma unroll
+      for (int j = 0; j < NX; ++j) z[j] = in.z[j];
+    }
+    if (t + kTok < t1) {
+      cnt = static_cast<int>(min64(kTok, t1 - t - kTok));
+      fetch(t + kTok, cnt);
+    }
+    for (int k0 = 0; k0 < now; k0 += 4) {
+      const float4 dec4 = *reinterpret_cast<const float4*>(&sdecay[k0]), dt4 = *reinterpret_cast<const float4*>(&sdt[k0]);
+      float acc[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float dec = e == 0 ? dec4.x : e == 1 ? dec4.y : e == 2 ? dec4.z : dec4.w;
+        const float u = (e == 0 ? dt4.x : e == 1 ? dt4.y : e == 2 ? dt4.z : dt4.w) * sx[k0 + e][r];
+        const float2 dec2 = make_float2(dec, dec), u2 = make_float2(u, u);
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < SPT; i += 4) {
+          const int s = i * LPR + lane * 4;
+          const float4 bv = *reinterpret_cast<const float4*>(&sb[k0 + e][s]);
+          st[i / 2] = __ffma2_rn(dec2, st[i / 2], __fmul2_rn(u2, make_float2(bv.x, bv.y)));
+          st[i / 2 + 1] = __ffma2_rn(dec2, st[i / 2 + 1], __fmul2_rn(u2, make_float2(bv.z, bv.w)));
+          if (OUT) {
+            const float4 cv = *reinterpret_cast<const float4*>(&sc[k0 + e][s]);
+            sum = __ffma2_rn(st[i / 2], make_float2(cv.x, cv.y), sum);
+            sum = __ffma2_rn(st[i / 2 + 1], make_float2(cv.z, cv.w), sum);
+          }
+        }
+        acc[e] = sum.x + sum.y;
       }
-      // sx and sy are rewritten after the next tile's first barrier only
-      // when that tile's loads are done: keep the two phases apart
+      if (OUT) {  // lane e of each four ends with token k0 + e's sum
+        const bool hi = lane & 2, odd = lane & 1;
+        const float a0 = (hi ? acc[2] : acc[0]) + __shfl_xor_sync(0xffffffffu, hi ? acc[0] : acc[2], 2);
+        const float a1 = (hi ? acc[3] : acc[1]) + __shfl_xor_sync(0xffffffffu, hi ? acc[1] : acc[3], 2);
+        float v = (odd ? a1 : a0) + __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 1);
+        if (LPR == 8) v += __shfl_xor_sync(0xffffffffu, v, 4);
+        if (lane < 4) sy[k0 + lane][r] = fmaf(D, sx[k0 + lane][r], v);
+      } else {
+        const float4 a = *reinterpret_cast<const float4*>(&sda[k0]);
+        logd += (a.x + a.y) + (a.z + a.w);
+      }
+    }
+    if (OUT) {
       __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NX; ++j) {
+        const int i = threadIdx.x + j * 256, k = i / ROWS, q = i % ROWS;
+        if (k >= now || row0 + q >= p.P) continue;
+        float v = sy[k][q];
+        if (p.z) v *= silu(pk::widen<T, 1>(z[j]).s);
+        static_cast<T*>(p.y)[(t + k) * p.H * p.P + col0 + q] = from_f<T>(v);
+      }
     }
   }
   if (!live) return;
@@ -136,10 +190,20 @@ __global__ void __launch_bounds__(256) scan_rec_kernel(const ScanParams p) {
   for (int i = 0; i < SPT; ++i) {
     const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
     if (s >= p.S) continue;
-    if (!OUT) p.seg_state[at_seg + s] = st[i];
-    else if (last && p.final_state) st_any(p.final_state, p.final_dtype, at_seq + s, st[i]);
+    const float v = i & 1 ? st[i / 2].y : st[i / 2].x;
+    if (!OUT) p.seg_state[at_seg + s] = v;
+    else if (last && p.final_state) st_any(p.final_state, p.final_dtype, at_seq + s, v);
   }
   if (!OUT && row == 0 && lane == 0) p.seg_decay[id * p.H + h] = logd;
+}
+
+// Loads that stay before the stores that follow them: the kernel below
+// overwrites what it has read, so they are not of the read-only kind.
+__device__ __forceinline__ void load_state(pk::Raw<float, 4>& v, const float* p) {
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.a.x), "=r"(v.a.y), "=r"(v.a.z), "=r"(v.a.w) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void load_state(pk::Raw<float, 1>& v, const float* p) {
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v.a) : "l"(p) : "memory");
 }
 
 // States between segments: for each sequence, head and state element, in
@@ -181,27 +245,33 @@ __global__ void __launch_bounds__(256) scan_pass_kernel(const ScanParams p) {
 #pragma unroll
   for (int e = 0; e < VEC; ++e)
     pk::set(cur, e, p.init ? ld_any(p.init, p.init_dtype, (n * p.H + h) * PS + i + e) : 0.f);
+  if (count <= 0) return;
   float* st = p.seg_state + (first * p.subs * p.H + h) * PS + i;
   const float* ld = p.seg_decay + first * p.subs * p.H + h;
-  const int64_t step = p.H * PS;
-  for (int64_t k = 0; k < count; ++k, st += p.subs * step, ld += static_cast<int64_t>(p.subs) * p.H) {
-    const bool more = k + 1 < count;
-    constexpr int kAhead = 4;  // pieces whose loads are in flight together
-    for (int j0 = 0; j0 < (more ? p.subs : 1); j0 += kAhead) {
-      pk::Raw<float, VEC> v[kAhead];
-      float d[kAhead];
+  const int64_t step = p.H * PS, pieces = (count - 1) * p.subs;  // the last segment adds to nothing here
+  constexpr int kAhead = 8;                                      // pieces whose loads are in flight together
+  int sub = 0;
+  for (int64_t j0 = 0; j0 < pieces; j0 += kAhead) {
+    const int now = static_cast<int>(min64(kAhead, pieces - j0));
+    pk::Raw<float, VEC> v[kAhead];
+    float d[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (more && j0 + j < p.subs) {
-          pk::load(v[j], st + (j0 + j) * step);
-          d[j] = expf(ld[(j0 + j) * p.H]);
-        }
-      if (j0 == 0) pk::store<float, VEC>(st, cur);
+    for (int j = 0; j < kAhead; ++j)
+      if (j < now) {
+        load_state(v[j], st + j * step);
+        d[j] = ld[j * p.H];
+      }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (more && j0 + j < p.subs) cur = pk::fma(pk::splat<VEC>(d[j]), cur, pk::widen<float, VEC>(v[j]));
-    }
+    for (int j = 0; j < kAhead; ++j)
+      if (j < now) {
+        if (sub == 0) pk::store<float, VEC>(st + j * step, cur);
+        if (++sub == p.subs) sub = 0;
+        cur = pk::fma(pk::splat<VEC>(expf(d[j])), cur, pk::widen<float, VEC>(v[j]));
+      }
+    st += now * step;
+    ld += static_cast<int64_t>(now) * p.H;
   }
+  pk::store<float, VEC>(st, cur);
 }
 
 // ---- single tokens ---------------------------------------------------------
@@ -377,6 +447,7 @@ void launch_rec(ScanParams p, const Plan& pl, cudaStream_t s) {
   constexpr int ROWS = 256 / LPR;
   const dim3 grid(static_cast<unsigned>(pl.segments), static_cast<unsigned>(p.H),
                   static_cast<unsigned>((p.P + ROWS - 1) / ROWS));
+  p.subs = 1;  // this first pass takes whole segments, also in a plan made for the tensor cores
   if (pl.split) {
     note_launch();
     scan_rec_kernel<T, SPT, LPR, false><<<grid, 256, 0, s>>>(p);

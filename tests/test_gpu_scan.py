@@ -211,6 +211,22 @@ def test_layouts_give_the_same_values():
     assert torch.equal(y, y3) and torch.equal(h, h3)
 
 
+def test_misaligned_rows_of_a_split_prompt(monkeypatch):
+    """A C caller's misaligned rows: tensor-core shapes, cut into segments and
+    those into pieces, that the recurrent kernel has to take."""
+    import domesticated_torch_mlu_ops_b200.scan as scan
+    monkeypatch.setattr(scan, "_aligned_rows", scan._packed_rows)
+    lens = [1200]
+    i = make(sum(lens), 64, 64, 1, 64, bf16, True, seed=8)
+    base = torch.zeros(i["x"].numel() + 1, dtype=bf16)
+    base[1:] = i["x"].flatten()
+    i["x"] = base[1:].view(i["x"].shape)
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["dt_bias"], True, (0.0, float("inf")),
+                      None, lens)
+    y, h = run(i, lens)
+    assert rel(y, ry) <= tolerances(bf16, False) and rel(h, rh) <= 64 * F32
+
+
 @pytest.mark.parametrize("generic", [False, True])
 def test_neighbours_stay_out(generic):
     """NaN and infinity in one sequence reach no other, although tiles overlap them."""
