@@ -28,21 +28,23 @@ struct RecTile {
   float dt;
 };
 
-// One CTA per (segment, head, slice of ROWS state rows).  LPR lanes share a
-// state row; each holds SPT of its columns (columns i*4*LPR + 4*lane + e, so
-// that the lanes read 16-byte pieces of B and C side by side).  Per token and
-// thread: SPT packed multiply-adds for the state and half as many for the
-// output, and three shuffles per four tokens that leave each of four lanes
-// with one token's sum.  Everything in fp32.  A tile's inputs are loaded
+// One CTA per (segment, head, slice of ROWS state rows).  LPR lanes share R
+// state rows; each holds SPT of their columns (columns i*4*LPR + 4*lane + e,
+// so that the lanes read 16-byte pieces of B and C side by side; R rows use
+// what was read, which is what shared memory bounds).  The output sums of R
+// rows and four tokens are halved from lane to lane until each lane is left
+// with one of them.  Everything in fp32.  A tile's inputs are loaded
 // while the tile before it is computed; a tail is padded to four tokens of
 // step zero (decay 1, nothing added).
-template <typename T, int SPT, int LPR, bool OUT>
+template <typename T, int SPT, int LPR, int R, bool OUT>
 __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
   constexpr int SP = SPT * LPR;  // padded state width
-  constexpr int ROWS = 256 / LPR;
+  constexpr int ROWS = 256 / LPR * R;
+  constexpr int V = 4 * R;  // output sums of four tokens
+  static_assert(V <= LPR, "a lane per sum");
   constexpr int NB = kTok * SP / 256, NX = kTok * ROWS / 256;
   __shared__ __align__(16) float sb[kTok][SP], sc[OUT ? kTok : 1][SP], sdt[kTok], sda[kTok], sdecay[kTok];
-  __shared__ float sx[kTok][ROWS + 8], sy[OUT ? kTok : 1][ROWS + 8];
+  __shared__ __align__(16) float sx[kTok][ROWS + 8], sy[OUT ? kTok : 1][ROWS + 8];
   __shared__ int64_t seg_n, seg_t0, seg_t1;
   __shared__ int seg_ok, seg_last;
   const int64_t id = blockIdx.x;
@@ -63,8 +65,7 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
   if (!seg_ok || (!OUT && seg_last)) return;
   const int64_t n = seg_n, t0 = seg_t0, t1 = seg_t1;
   const bool last = seg_last;
-  const int lane = threadIdx.x % LPR, r = threadIdx.x / LPR, row = row0 + r;
-  const bool live = row < p.P;
+  const int lane = threadIdx.x % LPR, r = threadIdx.x / LPR * R, row = row0 + r;
   const float A = p.A[h], D = p.D ? p.D[h] : 0.f, bias = p.dt_bias ? p.dt_bias[h] : 0.f;
   const T* bp = static_cast<const T*>(p.b) + static_cast<int64_t>(g) * p.S;
   const T* cp = static_cast<const T*>(p.c) + static_cast<int64_t>(g) * p.S;
@@ -91,20 +92,22 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
   };
   int cnt = static_cast<int>(min64(kTok, t1 - t0));
   if (t0 < t1) fetch(t0, cnt);
-  float2 st[SPT / 2];
+  float2 st[R][SPT / 2];
   const int64_t at_seq = ((n * p.H + h) * p.P + row) * p.S;
   const int64_t at_seg = ((id * p.H + h) * p.P + row) * p.S;
 #pragma unroll
-  for (int i = 0; i < SPT; ++i) {
-    const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
-    float v = 0.f;
-    if (OUT && live && s < p.S) {
-      if (p.seg_state) v = p.seg_state[at_seg + s];
-      else if (p.init) v = ld_any(p.init, p.init_dtype, at_seq + s);
+  for (int q = 0; q < R; ++q)
+#pragma unroll
+    for (int i = 0; i < SPT; ++i) {
+      const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
+      float v = 0.f;
+      if (OUT && row + q < p.P && s < p.S) {
+        if (p.seg_state) v = p.seg_state[at_seg + q * p.S + s];
+        else if (p.init) v = ld_any(p.init, p.init_dtype, at_seq + q * p.S + s);
+      }
+      if (i & 1) st[q][i / 2].y = v;
+      else st[q][i / 2].x = v;
     }
-    if (i & 1) st[i / 2].y = v;
-    else st[i / 2].x = v;
-  }
   float logd = 0.f;
   for (int64_t t = t0; t < t1; t += kTok) {
     __syncthreads();  // the tile before this one has been read
@@ -140,34 +143,51 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
     }
     for (int k0 = 0; k0 < now; k0 += 4) {
       const float4 dec4 = *reinterpret_cast<const float4*>(&sdecay[k0]), dt4 = *reinterpret_cast<const float4*>(&sdt[k0]);
-      float acc[4];
+      float acc[V];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float dec = e == 0 ? dec4.x : e == 1 ? dec4.y : e == 2 ? dec4.z : dec4.w;
-        const float u = (e == 0 ? dt4.x : e == 1 ? dt4.y : e == 2 ? dt4.z : dt4.w) * sx[k0 + e][r];
-        const float2 dec2 = make_float2(dec, dec), u2 = make_float2(u, u);
-        float2 sum = make_float2(0.f, 0.f);
+        const float dt = e == 0 ? dt4.x : e == 1 ? dt4.y : e == 2 ? dt4.z : dt4.w;
+        const float2 dec2 = make_float2(dec, dec);
+        float2 u[R], sum[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+          const float v = dt * sx[k0 + e][r + q];
+          u[q] = make_float2(v, v);
+          sum[q] = make_float2(0.f, 0.f);
+        }
 #pragma unroll
         for (int i = 0; i < SPT; i += 4) {
           const int s = i * LPR + lane * 4;
-          const float4 bv = *reinterpret_cast<const float4*>(&sb[k0 + e][s]);
-          st[i / 2] = __ffma2_rn(dec2, st[i / 2], __fmul2_rn(u2, make_float2(bv.x, bv.y)));
-          st[i / 2 + 1] = __ffma2_rn(dec2, st[i / 2 + 1], __fmul2_rn(u2, make_float2(bv.z, bv.w)));
-          if (OUT) {
-            const float4 cv = *reinterpret_cast<const float4*>(&sc[k0 + e][s]);
-            sum = __ffma2_rn(st[i / 2], make_float2(cv.x, cv.y), sum);
-            sum = __ffma2_rn(st[i / 2 + 1], make_float2(cv.z, cv.w), sum);
+          const float4 b = *reinterpret_cast<const float4*>(&sb[k0 + e][s]);
+          float4 c;
+          if (OUT) c = *reinterpret_cast<const float4*>(&sc[k0 + e][s]);
+#pragma unroll
+          for (int q = 0; q < R; ++q) {
+            float2 &s0 = st[q][i / 2], &s1 = st[q][i / 2 + 1];
+            s0 = __ffma2_rn(dec2, s0, __fmul2_rn(u[q], make_float2(b.x, b.y)));
+            s1 = __ffma2_rn(dec2, s1, __fmul2_rn(u[q], make_float2(b.z, b.w)));
+            if (OUT) {
+              sum[q] = __ffma2_rn(s0, make_float2(c.x, c.y), sum[q]);
+              sum[q] = __ffma2_rn(s1, make_float2(c.z, c.w), sum[q]);
+            }
           }
         }
-        acc[e] = sum.x + sum.y;
+#pragma unroll
+        for (int q = 0; q < R; ++q) acc[e * R + q] = sum[q].x + sum[q].y;
       }
-      if (OUT) {  // lane e of each four ends with token k0 + e's sum
-        const bool hi = lane & 2, odd = lane & 1;
-        const float a0 = (hi ? acc[2] : acc[0]) + __shfl_xor_sync(0xffffffffu, hi ? acc[0] : acc[2], 2);
-        const float a1 = (hi ? acc[3] : acc[1]) + __shfl_xor_sync(0xffffffffu, hi ? acc[1] : acc[3], 2);
-        float v = (odd ? a1 : a0) + __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 1);
-        if (LPR == 8) v += __shfl_xor_sync(0xffffffffu, v, 4);
-        if (lane < 4) sy[k0 + lane][r] = fmaf(D, sx[k0 + lane][r], v);
+      if (OUT) {  // lane v of each V ends with sum v: token k0 + v / R, row v % R
+#pragma unroll
+        for (int m = V / 2; m > 0; m /= 2) {
+          const bool up = lane & m;
+#pragma unroll
+          for (int i = 0; i < m; ++i)
+            acc[i] = (up ? acc[i + m] : acc[i]) + __shfl_xor_sync(0xffffffffu, up ? acc[i] : acc[i + m], m);
+        }
+#pragma unroll
+        for (int m = V; m < LPR; m *= 2) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], m);
+        const int k = k0 + lane / R, q = r + lane % R;
+        if (lane < V) sy[k][q] = fmaf(D, sx[k][q], acc[0]);
       } else {
         const float4 a = *reinterpret_cast<const float4*>(&sda[k0]);
         logd += (a.x + a.y) + (a.z + a.w);
@@ -185,15 +205,16 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
       }
     }
   }
-  if (!live) return;
 #pragma unroll
-  for (int i = 0; i < SPT; ++i) {
-    const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
-    if (s >= p.S) continue;
-    const float v = i & 1 ? st[i / 2].y : st[i / 2].x;
-    if (!OUT) p.seg_state[at_seg + s] = v;
-    else if (last && p.final_state) st_any(p.final_state, p.final_dtype, at_seq + s, v);
-  }
+  for (int q = 0; q < R; ++q)
+#pragma unroll
+    for (int i = 0; i < SPT; ++i) {
+      const int s = (i / 4) * 4 * LPR + lane * 4 + (i & 3);
+      if (row + q >= p.P || s >= p.S) continue;
+      const float v = i & 1 ? st[q][i / 2].y : st[q][i / 2].x;
+      if (!OUT) p.seg_state[at_seg + q * p.S + s] = v;
+      else if (last && p.final_state) st_any(p.final_state, p.final_dtype, at_seq + q * p.S + s, v);
+    }
   if (!OUT && row == 0 && lane == 0) p.seg_decay[id * p.H + h] = logd;
 }
 
@@ -442,29 +463,29 @@ Plan plan(const gdn_scan_args& a) {
   return pl;
 }
 
-template <typename T, int SPT, int LPR>
+template <typename T, int SPT, int LPR, int R>
 void launch_rec(ScanParams p, const Plan& pl, cudaStream_t s) {
-  constexpr int ROWS = 256 / LPR;
+  constexpr int ROWS = 256 / LPR * R;
   const dim3 grid(static_cast<unsigned>(pl.segments), static_cast<unsigned>(p.H),
                   static_cast<unsigned>((p.P + ROWS - 1) / ROWS));
   p.subs = 1;  // this first pass takes whole segments, also in a plan made for the tensor cores
   if (pl.split) {
     note_launch();
-    scan_rec_kernel<T, SPT, LPR, false><<<grid, 256, 0, s>>>(p);
+    scan_rec_kernel<T, SPT, LPR, R, false><<<grid, 256, 0, s>>>(p);
     launch_pass(p, s);
     p.clear_err = 0;
   }
   note_launch();
-  scan_rec_kernel<T, SPT, LPR, true><<<grid, 256, 0, s>>>(p);
+  scan_rec_kernel<T, SPT, LPR, R, true><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T>
 void launch_t(const ScanParams& p, const Plan& pl, cudaStream_t s) {
-  if (p.S <= 16) launch_rec<T, 4, 4>(p, pl, s);
-  else if (p.S <= 32) launch_rec<T, 8, 4>(p, pl, s);
-  else if (p.S <= 64) launch_rec<T, 16, 4>(p, pl, s);
-  else if (p.S <= 128) launch_rec<T, 32, 4>(p, pl, s);
-  else launch_rec<T, 32, 8>(p, pl, s);
+  if (p.S <= 16) launch_rec<T, 4, 4, 1>(p, pl, s);
+  else if (p.S <= 32) launch_rec<T, 4, 8, 2>(p, pl, s);
+  else if (p.S <= 64) launch_rec<T, 4, 16, 4>(p, pl, s);
+  else if (p.S <= 128) launch_rec<T, 8, 16, 4>(p, pl, s);
+  else launch_rec<T, 16, 16, 2>(p, pl, s);
 }
 
 void launch_pass(const ScanParams& p, cudaStream_t s) {
