@@ -84,7 +84,8 @@ def _scan_fwd_impl(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Op
     G, S = B.shape[2], B.shape[3]
     N = Bt if cu_seqlens is None else cu_seqlens.numel() - 1
     dev = x.device
-    rows = _aligned_rows if x.dtype == torch.bfloat16 else _packed_rows
+    tensor_cores = x.dtype == torch.bfloat16 and P % 64 == 0 and S in (64, 128) and not force_generic
+    rows = _aligned_rows if tensor_cores else _packed_rows  # the recurrent kernel reads any rows in place
     (x, sx), (dt, sdt), (B, sb), (C, sc) = rows(x, 2), _packed_rows(dt, 1), rows(B, 2), rows(C, 2)
     z, sz = (None, 0) if z is None else rows(z, 2)
     y = torch.empty((Bt, T, H, P), dtype=x.dtype, device=dev)
