@@ -10,12 +10,18 @@
 //
 // Both passes are streams: each input is read once and each output written
 // once, so HBM bounds them.  A row's group stays in the registers of a team
-// of threads between its reduction and its outputs: 8, 16 or 32 lanes of a
-// warp (several teams per warp share its reductions) up to 128 vectors, a
-// whole CTA above.  The backward recomputes rstd (one more value in a
-// reduction that it needs anyway) instead of reading a saved one; its teams
-// walk the rows of one group with dw in registers, CTAs leave their dw in
-// the workspace and a second kernel adds those in order.
+// of threads between its reduction and its outputs, one vector per thread: 8,
+// 16 or 32 lanes of a warp (several teams per warp share its reductions) up
+// to 32 vectors, a whole CTA above.  The backward recomputes rstd (one more
+// value in a reduction that it needs anyway) instead of reading a saved one;
+// its teams walk the rows of one group with dw in registers, CTAs leave their
+// dw in the workspace and a second kernel adds those in order.
+//
+// Measured: 262144 bf16 rows of 128 with a gate, forward 36 us for 201 MB
+// (5.6 TB/s, 85 % of a plain copy's rate), backward 66 + 4 us for 336 MB (4.8
+// TB/s); 5001 bf16 rows of 2048 with an fp32 residual, forward 18 us for 123
+// MB (the sum stays partly in L2), backward 31 + 4 us for 143 MB.  A few rows
+// (64 x 32 of 128): 2.2 us, a launch and one trip to memory.
 
 #include "conv_math.cuh"
 #include "gdn_common.cuh"
@@ -358,8 +364,8 @@ constexpr int kMaxScalar = 16 * 1024, kMaxVector = 4 * 1024;  // elements / vect
 
 // 16-byte vectors when the group, the strides and every pointer allow them.
 int vec_of(const gdn_norm_args& a) {
-  const int v = 16 / esize(a.x_dtype), xv = 16 / esize(a.x_dtype);
-  const bool ok = a.group % v == 0 && a.D % v == 0 && a.stride_x_token % xv == 0 && a.stride_x_head % xv == 0 &&
+  const int v = 16 / esize(a.x_dtype);
+  const bool ok = a.group % v == 0 && a.D % v == 0 && a.stride_x_token % v == 0 && a.stride_x_head % v == 0 &&
                   a.stride_z_token % v == 0 && a.stride_z_head % v == 0 && al16(a.x) && al16(a.z) && al16(a.residual) &&
                   al16(a.weight) && al16(a.y) && al16(a.sum) && al16(a.dy) && al16(a.dsum) && al16(a.dx) && al16(a.dz) &&
                   al16(a.dresidual) && a.group / v <= kMaxVector;

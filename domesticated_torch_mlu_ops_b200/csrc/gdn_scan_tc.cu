@@ -24,7 +24,17 @@
 // scan_tc_state_kernel, the first pass over split sequences: dH of a whole
 // segment in one accumulator, chunks from the last to the first, each
 // weighted by the decay to the segment's end.
-
+//
+// What bounds it.  The products of a chunk take about 2.4 K cycles of the
+// tensor pipe (64 per step of 16 at 128 columns, 48 at 64: half of it is the
+// three parts of w x), a chunk step about 6 K: the sixteen warps' conversions
+// between TMEM and shared memory stand in a chain with the products, and
+// shared memory (two stages of operands) leaves room for one CTA per SM.  64
+// heads of 64 x 128: 8192 tokens 25.5 us (first pass) and 106 us, with prep
+// and hand-over 141 us for 208 MB; 29,893 packed tokens that start from
+// states 417 us and 14 us of prep.  Measured and set aside: w x before P with
+// Yi double-buffered (113 us), products issued by a working warp (1.7 times).
+//
 // Rounding.  x, B and C are bf16 already.  P and h are rounded to bf16 as
 // operands, as y is rounded to bf16 in the end.  w x is split into bf16 parts
 // whose products are summed: two parts (16 bits) where the state only feeds
@@ -49,8 +59,8 @@ namespace scan {
 
 constexpr int kL = 128;             // tokens per chunk
 constexpr int kTile = kL * 128;     // 128 rows x 128 bytes (64 bf16 columns)
-constexpr int kWork = 512;                // threads of the sixteen working warps
-constexpr int kTcThreads = kWork + 32;    // and the issuing warp
+constexpr int kWork = 512;          // threads of the sixteen working warps
+constexpr int kTcThreads = kWork + 32;  // and the issuing warp
 constexpr int kLead = kWork / 32;
 constexpr long long kWaitLimit = 2000000000LL;
 
@@ -62,22 +72,22 @@ struct PrepOut {
 template <int S_>
 struct Smem {
   // two stages of operands
-  static constexpr int kC = 0;                              // C, then the second part of w x, and z
-  static constexpr int kZ = kC + kTile;
+  static constexpr int kC = 0;                              // C
+  static constexpr int kZ = kC + kTile;                     // z: in C's second tile, or its own (S = 64)
   static constexpr int kB = kC + 2 * kTile;
   static constexpr int kX = kB + S_ / 64 * kTile;           // x, then y
   static constexpr int kStage = kX + kTile;
-  static constexpr int kXs = 2 * kStage;                    // first part of w x
-  static constexpr int kH = kXs + kTile;                    // h, then the third part of w x
-  static constexpr int kP = kH + kTile;
-  static constexpr int kSc = kP + 2 * kTile;                // two stages of a and k
+  static constexpr int kXs = 2 * kStage;                    // the parts of w x
+  static constexpr int kH = kXs + 3 * kTile;                // h
+  static constexpr int kSc = kH + kTile;              // two stages of a and k
   static constexpr int kBar = kSc + 2 * 2 * kL * 4;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
   static constexpr int kBars = 9;
   static constexpr int kTmem = kBar + kBars * 8;
   static constexpr int kBad = kTmem + 8;                    // [2][64 columns + 1]: see the kernel
   static constexpr int kBytes = kBad + 2 * 65 * 4;
   static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile + 2 * kL * 4;
-  static constexpr int kCols = 512, kYi = 256, kYa = 320, kDH = 384;  // TMEM columns: S[2] first
+  // TMEM columns: S first (P in its place), dH one accumulator per part of w x
+  static constexpr int kCols = 512, kYi = 128, kYa = 192, kDH = 256;
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -92,7 +102,7 @@ struct StateSmem {
   static constexpr int kBar = kSc + 2 * 2 * kL * 4;  // B[3], x[2], parts ready[2], products[2]
   static constexpr int kTmem = kBar + 9 * 8;
   static constexpr int kBytes = kTmem + 8;
-  static constexpr int kCols = 64;
+  static constexpr int kCols = 256;  // an accumulator per part
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -251,6 +261,9 @@ __device__ __forceinline__ void publish(uint32_t bar) {
   __syncwarp();
 }
 
+// P's columns of k-step ks in TMEM: each block of 32 in the first half of the
+// scores that it came from.
+__host__ __device__ constexpr uint32_t p_step(int ks) { return (ks >> 1) * 32 + (ks & 1) * 8; }
 // What k-step ks of 16 adds to an operand descriptor.
 __host__ __device__ constexpr uint64_t k_step(int ks) { return ((ks >> 2) * kTile + (ks & 3) * 32) >> 4; }
 __host__ __device__ constexpr uint64_t mn_step(int ks) { return (ks * 2048) >> 4; }
@@ -265,7 +278,7 @@ __device__ __forceinline__ bool base_ok(const ScanParams& p, uint32_t sbase) {
 
 // A diagonal block of P under decays past 2^100 within it: the difference of
 // each pair.  Out of line: its registers would push the common path's out.
-__device__ __noinline__ void diag_by_difference(uint32_t ts, uint32_t prow_at, int piece0, int row, float ai, float dt) {
+__device__ __noinline__ void diag_by_difference(uint32_t ts, int row, float ai, float dt) {
   const int lane = row & 31;
 #pragma unroll 1
   for (int q = 0; q < 4; ++q) {
@@ -277,7 +290,7 @@ __device__ __noinline__ void diag_by_difference(uint32_t ts, uint32_t prow_at, i
       const float aj = __shfl_sync(0xffffffffu, ai, j), dj = __shfl_sync(0xffffffffu, dt, j);
       v[e] = j <= lane ? v[e] * (ex2(ai - aj) * dj) : 0.f;
     }
-    sts16(prow_at + (((piece0 + q) ^ (row & 7)) << 4), tc::pack8<__nv_bfloat16>(v));
+    umma::tmem_st4(ts + q * 4, tc::pack8<__nv_bfloat16>(v));
   }
 }
 
@@ -375,14 +388,14 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     // ---- copies and products ----
     constexpr uint32_t id_s = umma::idesc_f16(128, 128, true, false, false);
     constexpr uint32_t id_y = umma::idesc_f16(128, 64, true, false, true);
-    constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
+    constexpr uint32_t id_h2 = umma::idesc_f16(128, 128, true, true, true), id_h3 = umma::idesc_f16(128, 192, true, true, true);
     // operand descriptors: rows of x and of the parts are tokens (K) with 64
     // columns (N), B is read both ways; a k-step of 16 advances 32 bytes
     // within a K-major atom of 64 columns and 2048 bytes over MN-major rows
     const uint64_t d_c = umma::smem_desc_sw128(sbase + M::kC, 16, 1024), d_bk = umma::smem_desc_sw128(sbase + M::kB, 16, 1024);
     const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_x = umma::smem_desc_sw128(sbase + M::kX, kTile, 1024);
-    const uint64_t d_cm = umma::smem_desc_sw128(sbase + M::kC, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
-    const uint64_t d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024), d_p = umma::smem_desc_sw128(sbase + M::kP, 16, 1024);
+    const uint64_t d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
+    const uint64_t d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024);
     auto fetch_cb = [&](int c) {
       const uint32_t bar = bar_ld + (c & 1) * 8;
       uint8_t* st = sm + (c & 1) * M::kStage;
@@ -406,7 +419,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       const uint64_t st = (c & 1) * (M::kStage >> 4);
 #pragma unroll
       for (int ks = 0; ks < S_ / 16; ++ks)
-        umma::mma_f16(tmem + (c & 1) * 128, d_c + st + k_step(ks), d_bk + st + k_step(ks), id_s, ks > 0);
+        umma::mma_f16(tmem, d_c + st + k_step(ks), d_bk + st + k_step(ks), id_s, ks > 0);
       umma::mma_commit(bar_s);
     };
     int loads = 0, n_s = 0, n_yi = 0, n_y = 0, n_dh = 0, n_z = 0;  // issued so far
@@ -459,20 +472,15 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         const uint64_t st = (c & 1) * (M::kStage >> 4);
 #pragma unroll
         for (int ks = 0; ks < kL / 16; ++ks)
-          umma::mma_f16(tmem + M::kYa, d_p + k_step(ks), d_x + st + mn_step(ks), id_y, ks > 0);
+          umma::mma_f16_ta(tmem + M::kYa, tmem + p_step(ks), d_x + st + mn_step(ks), id_y, ks > 0);
         umma::mma_commit(bar_y);
-        // With S = 64 rows 64-127 of the accumulator are the product of the
+        // The parts of w x side by side: one product reads B once for all.
+        // With S = 64 rows 64-127 of the accumulators are the product of the
         // tile after B: never read.
+        const uint32_t id_h = want_state ? id_h3 : id_h2;
 #pragma unroll
         for (int ks = 0; ks < kL / 16; ++ks)
           umma::mma_f16(tmem + M::kDH, d_bm + st + mn_step(ks), d_xs + mn_step(ks), id_h, ks > 0);
-#pragma unroll
-        for (int ks = 0; ks < kL / 16; ++ks)
-          umma::mma_f16(tmem + M::kDH, d_bm + st + mn_step(ks), d_cm + st + mn_step(ks), id_h, 1);
-        if (want_state)
-#pragma unroll
-          for (int ks = 0; ks < kL / 16; ++ks)
-            umma::mma_f16(tmem + M::kDH, d_bm + st + mn_step(ks), d_h + mn_step(ks), id_h, 1);
         umma::mma_commit(bar_dh);
       }
       __syncwarp();
@@ -480,6 +488,8 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       ++n_dh;
       if (c + 1 < nch) {
         if (!wait(bar_ld + ((c + 1) & 1) * 8, ((c + 1) >> 1) & 1, kSiteScanLoad)) break;
+        if (!wait(bar_y, c & 1, kSiteScanOut)) break;  // P is read: the scores take its place
+        umma::fence_after_sync();
         if (umma::elect_one()) scores(c + 1);
         __syncwarp();
         ++n_s;
@@ -541,13 +551,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       const float ai = sc.a, all = sc.end[3];
       const float wj = sc.k * ex2(all - pick4(sc.end, quad));
       // ---- P from the scores: block of columns J = cq ----
-      const uint32_t prow_at = sbase + M::kP + (cq >> 1) * kTile + row * 128;
       if (!wait(bar_s, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
+      const uint32_t ts = tl + cq * 32;
       if (cq <= quad) {
         const float far = ai - pick4(sc.end, cq);
         const bool diag = cq == quad;
-        const uint32_t ts = tl + (c & 1) * 128 + cq * 32;
         // far is largest in the block's first row: one answer per warp
         if (!diag || __shfl_sync(0xffffffffu, far, 0) < 100.f) {
           const uint32_t cf = sc_at + (kL + cq * 32) * 4;
@@ -556,6 +565,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {  // 16 columns at a time: registers
             float v[16];
+            uint4 u[2];
             umma::tmem_ld16(ts + hf * 16, v);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -572,18 +582,19 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
                   if (j + 1 > lane) w[e].y = 0.f;
                 }
               }
-              sts16(prow_at + ((((cq & 1) * 4 + hf * 2 + q) ^ (row & 7)) << 4), pack8(w));
+              u[q] = pack8(w);
             }
+            umma::tmem_st8(ts + hf * 8, u[0], u[1]);  // over scores that have been read
           }
         } else {
-          diag_by_difference(ts, prow_at, (cq & 1) * 4, row, ai, __ldg(prep.dt + prow + c * kL + row));
+          diag_by_difference(ts, row, ai, __ldg(prep.dt + prow + c * kL + row));
         }
-      } else if (c == 0) {  // nothing else is written there
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sts16(prow_at + ((((cq & 1) * 4 + q) ^ (row & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
+      } else {
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        umma::tmem_st8(ts, zero, zero);
+        umma::tmem_st8(ts + 8, zero, zero);
       }
       // ---- w x in parts (x has been there since the scores were issued) ----
-      uint4 part[2], low[2];
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
       uint32_t not_finite = 0;
 #pragma unroll
@@ -600,10 +611,10 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(wj, wj));
         sts16(sbase + M::kXs + piece.at[q], take_part(v));
         if (want_state) {
-          part[q] = take_part(v);
-          low[q] = pack8(v);
+          sts16(sbase + M::kXs + kTile + piece.at[q], take_part(v));
+          sts16(sbase + M::kXs + 2 * kTile + piece.at[q], pack8(v));
         } else {
-          part[q] = pack8(v);
+          sts16(sbase + M::kXs + kTile + piece.at[q], pack8(v));
         }
       }
       if (__any_sync(0xffffffffu, not_finite != 0)) {
@@ -617,15 +628,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
           const int at = cq * (S_ / 32) + q;  // of S_ / 8 pieces
           sts16(st + M::kB + (at >> 3) * kTile + row * 128 + (((at & 7) ^ (row & 7)) << 4), zero);
         }
-      if (!wait(bar_yi, c & 1, kSiteScanScores)) break;  // C and h are read
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        sts16(st + M::kC + piece.at[q], part[q]);
-        if (want_state) sts16(sbase + M::kH + piece.at[q], low[q]);
-      }
+      umma::tmem_st_wait();
       publish(bar_px);
       // ---- outputs: first what does not need Ya (whose product runs now) ----
       float2 part_y[8], gz[8];
+      if (!wait(bar_yi, c & 1, kSiteScanScores)) break;
+      umma::fence_after_sync();
       {
         const float g1 = ex2(ai);
         const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
@@ -683,11 +691,19 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       umma::fence_after_sync();
       const float decay = ex2(all);
       {
-        float d[16];
-        umma::tmem_ld16(tl + M::kDH + cq * 16, d);
+        const float2 decay2 = make_float2(decay, decay);
+        float d[16], e[16];
+        umma::tmem_ld16x2(tl + M::kDH + cq * 16, tl + M::kDH + 64 + cq * 16, d, e);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          hr[j] = __ffma2_rn(make_float2(decay, decay), hr[j], make_float2(d[j * 2], d[j * 2 + 1]));
+        for (int j = 0; j < 8; ++j) {
+          hr[j] = __ffma2_rn(decay2, hr[j], make_float2(d[j * 2], d[j * 2 + 1]));
+          hr[j] = __fadd2_rn(hr[j], make_float2(e[j * 2], e[j * 2 + 1]));
+        }
+        if (want_state) {
+          umma::tmem_ld16(tl + M::kDH + 128 + cq * 16, d);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) hr[j] = __fadd2_rn(hr[j], make_float2(d[j * 2], d[j * 2 + 1]));
+        }
       }
       store_h();
       if (*reinterpret_cast<volatile int*>(bad + (c & 1) * 65 + 64) == c + 1 && row < len)
@@ -754,7 +770,7 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
   };
   // step i works on chunk nch - 1 - i
   if (warp == kLead) {
-    constexpr uint32_t id_h = umma::idesc_f16(128, 64, true, true, true);
+    constexpr uint32_t id_h = umma::idesc_f16(128, 192, true, true, true);
     const uint64_t d_b = umma::smem_desc_sw128(sbase, kTile, 1024), d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
     auto token = [&](int i) { return static_cast<int>(t0) + (nch - 1 - i) * kL; };
     auto fetch_b = [&](int i) {
@@ -797,11 +813,7 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
       if (umma::elect_one()) {
         const uint64_t db = d_b + (i % 3) * (M::kBStage >> 4), dx = d_xs + (i & 1) * ((3 * kTile) >> 4);
 #pragma unroll
-        for (int part = 0; part < 3; ++part)
-#pragma unroll
-          for (int ks = 0; ks < kL / 16; ++ks)
-            umma::mma_f16(tmem, db + mn_step(ks), dx + ((part * kTile) >> 4) + mn_step(ks), id_h,
-                          i > 0 || part > 0 || ks > 0);
+        for (int ks = 0; ks < kL / 16; ++ks) umma::mma_f16(tmem, db + mn_step(ks), dx + mn_step(ks), id_h, i > 0 || ks > 0);
         umma::mma_commit(bar_dh + (i & 1) * 8);
       }
       __syncwarp();
@@ -842,12 +854,14 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     const int i = nch - 1;
     if (mine && wait(bar_dh + (i & 1) * 8, (i >> 1) & 1, kSiteScanState)) {
       umma::fence_after_sync();
-      float d[16];
-      umma::tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + cq * 16, d);
+      const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + cq * 16;
+      float d[16], e[16], f[16];
+      umma::tmem_ld16x2(at, at + 64, d, e);
+      umma::tmem_ld16(at + 128, f);
       if (row < S_) {
         float* out = p.seg_state + ((piece_id * p.H + h) * p.P + p0 + cq * 16) * S_ + row;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) out[j * S_] = d[j];
+        for (int j = 0; j < 16; ++j) out[j * S_] = d[j] + (e[j] + f[j]);
       }
       if (tid == 0 && p0 == 0) p.seg_decay[piece_id * p.H + h] = later * 0.6931471805599453f;
     }
@@ -927,7 +941,6 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
   kern<<<grid, kTcThreads, Smem<S_>::kBytes, s>>>(p, prep, slices, tx, tb, tcm, ty, tz);
   return cudaGetLastError();
 }
-
 
 cudaError_t launch_tc(const ScanParams& p, const gdn_scan_args& a, float* scratch, cudaStream_t s) {
   if (p.segments * p.subs * p.H * (a.P / 64) > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
