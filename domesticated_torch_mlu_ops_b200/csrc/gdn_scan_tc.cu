@@ -411,6 +411,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     auto fetch_x = [&](int c) {
       umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kX, &tx, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_ld + (c & 1) * 8);
     };
+    // z has room only for the time between Yi and the outputs: to L2 a chunk ahead
+    auto prefetch_z = [&](int c) { umma::tma_prefetch_2d(&tz, h * p.P + p0, static_cast<int>(t0) + c * kL); };
+    auto fetch_z = [&](int c) {
+      umma::mbar_arrive_expect_tx(bar_z, kTile);
+      umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kZ, &tz, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_z);
+    };
     auto store_y = [&](int c) {
       umma::tma_store_2d(&ty, sm + (c & 1) * M::kStage + M::kX, h * p.P + p0, static_cast<int>(t0) + c * kL);
       umma::bulk_commit();
@@ -427,6 +433,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       if (umma::elect_one()) {
         fetch_cb(0);
         fetch_x(0);
+        if (p.z) prefetch_z(0);
       }
       __syncwarp();
       loads = 1;
@@ -448,23 +455,24 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
             umma::mma_f16(tmem + M::kYi, d_c + st + k_step(ks), d_h + mn_step(ks), id_y, ks > 0);
         umma::mma_commit(bar_yi);
         if (c > 0) store_y(c - 1);  // a whole chunk
-        if (c + 1 < nch) {
-          fetch_cb(c + 1);
-          umma::bulk_wait_read_all();  // x goes where that y was
-          fetch_x(c + 1);
-        }
       }
       __syncwarp();
       ++n_yi;
-      loads += c + 1 < nch;
-      if (p.z) {  // beside what C's tile takes next, once Yi has read it
+      if (p.z) {  // beside C's first tile, once Yi has read the second; before the next chunk's loads, which are not in a hurry
         if (!wait(bar_yi, c & 1, kSiteScanScores)) break;
-        if (umma::elect_one()) {
-          umma::mbar_arrive_expect_tx(bar_z, kTile);
-          umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kZ, &tz, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_z);
-        }
+        if (umma::elect_one()) fetch_z(c);
         __syncwarp();
         ++n_z;
+      }
+      if (c + 1 < nch) {
+        if (umma::elect_one()) {
+          fetch_cb(c + 1);
+          if (p.z) prefetch_z(c + 1);
+          umma::bulk_wait_read_all();  // x goes where that y was
+          fetch_x(c + 1);
+        }
+        __syncwarp();
+        ++loads;
       }
       if (!wait(bar_px, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
