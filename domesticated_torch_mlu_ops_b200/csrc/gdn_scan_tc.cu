@@ -396,17 +396,25 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_x = umma::smem_desc_sw128(sbase + M::kX, kTile, 1024);
     const uint64_t d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
     const uint64_t d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024);
-    auto fetch_cb = [&](int c) {
+    // a chunk's operands in the order in which their places become free: B and
+    // C's first tile with the products of the chunk before the last, C's
+    // second tile (where z was) and x (where y was) with its outputs
+    auto load_c = [&](int c, int q) {
+      umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kC + q * kTile, &tcm, g * S_ + q * 64, static_cast<int>(t0) + c * kL,
+                        bar_ld + (c & 1) * 8);
+    };
+    auto fetch_bc = [&](int c) {
       const uint32_t bar = bar_ld + (c & 1) * 8;
-      uint8_t* st = sm + (c & 1) * M::kStage;
       umma::mbar_arrive_expect_tx(bar, M::kTx);
       umma::bulk_g2s(sm + M::kSc + (c & 1) * 2 * kL * 4, prep.a + prow + c * kL, kL * 4, bar);
       umma::bulk_g2s(sm + M::kSc + (c & 1) * 2 * kL * 4 + kL * 4, prep.k + prow + c * kL, kL * 4, bar);
 #pragma unroll
-      for (int q = 0; q < S_ / 64; ++q) {
-        umma::tma_load_2d(st + M::kC + q * kTile, &tcm, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
-        umma::tma_load_2d(st + M::kB + q * kTile, &tb, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
-      }
+      for (int q = 0; q < S_ / 64; ++q)
+        umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kB + q * kTile, &tb, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
+      load_c(c, 0);
+    };
+    auto fetch_c2 = [&](int c) {
+      if (S_ == 128) load_c(c, 1);
     };
     auto fetch_x = [&](int c) {
       umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kX, &tx, h * p.P + p0, static_cast<int>(t0) + c * kL, bar_ld + (c & 1) * 8);
@@ -431,12 +439,15 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     int loads = 0, n_s = 0, n_yi = 0, n_y = 0, n_dh = 0, n_z = 0;  // issued so far
     if (nch > 0) {
       if (umma::elect_one()) {
-        fetch_cb(0);
-        fetch_x(0);
-        if (p.z) prefetch_z(0);
+        for (int c = 0; c < min(nch, 2); ++c) {
+          fetch_bc(c);
+          fetch_c2(c);
+          fetch_x(c);
+          if (p.z && c == 0) prefetch_z(0);
+        }
       }
       __syncwarp();
-      loads = 1;
+      loads = min(nch, 2);
       if (wait(bar_ld, 0, kSiteScanLoad)) {
         if (umma::elect_one()) scores(0);
         __syncwarp();
@@ -448,31 +459,29 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       if (!wait(bar_h, c & 1, kSiteScanState)) break;
       umma::fence_after_sync();
       if (umma::elect_one()) {
+        if (c > 0) store_y(c - 1);  // a whole chunk
+        if (c > 0 && c + 1 < nch) fetch_c2(c + 1);
         const uint64_t st = (c & 1) * (M::kStage >> 4);
         if (c > 0 || seg || ini)
 #pragma unroll
           for (int ks = 0; ks < S_ / 16; ++ks)
             umma::mma_f16(tmem + M::kYi, d_c + st + k_step(ks), d_h + mn_step(ks), id_y, ks > 0);
         umma::mma_commit(bar_yi);
-        if (c > 0) store_y(c - 1);  // a whole chunk
+        if (c > 0 && c + 1 < nch) {
+          umma::bulk_wait_read_all();
+          fetch_x(c + 1);
+        }
       }
       __syncwarp();
       ++n_yi;
-      if (p.z) {  // beside C's first tile, once Yi has read the second; before the next chunk's loads, which are not in a hurry
+      if (p.z) {  // in C's second tile once Yi has read it
         if (!wait(bar_yi, c & 1, kSiteScanScores)) break;
-        if (umma::elect_one()) fetch_z(c);
-        __syncwarp();
-        ++n_z;
-      }
-      if (c + 1 < nch) {
         if (umma::elect_one()) {
-          fetch_cb(c + 1);
-          if (p.z) prefetch_z(c + 1);
-          umma::bulk_wait_read_all();  // x goes where that y was
-          fetch_x(c + 1);
+          fetch_z(c);
+          if (c + 1 < nch) prefetch_z(c + 1);
         }
         __syncwarp();
-        ++loads;
+        ++n_z;
       }
       if (!wait(bar_px, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
@@ -501,6 +510,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         if (umma::elect_one()) scores(c + 1);
         __syncwarp();
         ++n_s;
+        if (c + 2 < nch) {
+          if (!wait(bar_dh, c & 1, kSiteScanState)) break;
+          if (umma::elect_one()) fetch_bc(c + 2);
+          __syncwarp();
+          ++loads;
+        }
       }
     }
     if (mine && nch > 0 && wait(bar_h, nch & 1, kSiteScanState)) {  // the last chunk's y
