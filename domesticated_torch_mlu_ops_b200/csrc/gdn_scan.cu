@@ -33,7 +33,11 @@ struct RecTile {
 // so that the lanes read 16-byte pieces of B and C side by side; R rows use
 // what was read, which is what shared memory bounds).  The output sums of R
 // rows and four tokens are halved from lane to lane until each lane is left
-// with one of them.  Everything in fp32.  A tile's inputs are loaded
+// with one of them.  Everything in fp32, bound by the fp32 pipes (five packed
+// operations per two state elements over both passes; about half their rate):
+// 8192 fp16 tokens of 32 heads of 64 x 128 take 216 us (first pass) and 400
+// us (319 and 629 with one row per lane group), 1377 fp32 tokens of 6 heads
+// of 48 x 40 take 8.3 and 12 us.  A tile's inputs are loaded
 // while the tile before it is computed; a tail is padded to four tokens of
 // step zero (decay 1, nothing added).
 template <typename T, int SPT, int LPR, int R, bool OUT>
@@ -230,7 +234,8 @@ __device__ __forceinline__ void load_state(pk::Raw<float, 1>& v, const float* p)
 // States between segments: for each sequence, head and state element, in
 // order of its segments, the state that the segment starts from (in place of
 // its first piece's) and h <- exp(log decay) h + state over its pieces.  A
-// stream over the pieces' states; VEC elements per thread.
+// stream over the pieces' states, eight ahead (one at a time took twice as
+// long: 22 segments 11.6 against 5.8 us); VEC elements per thread.
 template <int VEC>
 __global__ void __launch_bounds__(256) scan_pass_kernel(const ScanParams p) {
   __shared__ int64_t first_sh, count_sh;
@@ -427,15 +432,15 @@ struct Plan {
 // Segment length: enough (segment, head, row slice) CTAs to fill the GPU (one
 // per SM on the tensor cores, four of the recurrent kernel), but no segment
 // under `least` tokens, below which handing states on costs more than it
-// saves: four chunks on the tensor cores, 64 tokens (about 15 us of the
-// recurrence) otherwise.  Without a device query, so the result depends on
+// saves: four chunks on the tensor cores, 32 tokens otherwise (1377 tokens of
+// 6 heads: 29 us, 31 with 64 tokens; 70 tokens of 24 heads: 27 and 29 us).  Without a device query, so the result depends on
 // the shapes alone.
 Plan plan(const gdn_scan_args& a) {
   Plan pl{};
   const bool tc = tc_shape(a);
   const int64_t total = a.B * a.T;
   const int64_t slices = tc ? tc_slices(a) : (a.P + 63) / 64;
-  const int64_t want = 148 * (tc ? 1 : 4), least = tc ? 512 : 64, unit = tc ? 128 : kTok;
+  const int64_t want = 148 * (tc ? 1 : 4), least = tc ? 512 : 32, unit = tc ? 128 : kTok;
   const int64_t per_token = std::max<int64_t>(1, a.H * slices);
   const int64_t pieces = std::max<int64_t>(1, want / per_token);
   pl.seg = std::max(least, (total + pieces - 1) / pieces);

@@ -14,26 +14,36 @@
 //   Ya = P x;   y = exp(a_i) Yi + Ya + D x       in fp32, then the gate
 //   dH = B^T (w x),  w_j = exp(a_end - a_j) dt'_j
 //   h <- exp(a_end) h + dH                       fp32, in registers
-// Four products with fp32 accumulators in TMEM; x, B and C come by TMA, a
-// chunk ahead, into 128-byte-swizzled tiles that serve as operands in both
-// directions, y takes x's place (from where a TMA store moves it), the second
-// and third part of w x those of C and h once Yi has read them.  A chunk's
-// chain is P and w x from the scores (which run behind the previous chunk's
-// products), Ya and dH, and the new h.
+// Four products with fp32 accumulators in TMEM.  P replaces the scores there
+// and is Ya's operand from there; the parts of w x lie side by side, so that
+// dH is one product that reads B once.  x, B and C come by TMA into
+// 128-byte-swizzled tiles that serve as operands in both directions, each as
+// soon as its place is free: B and C's first half behind the products of the
+// chunk before the last, x after that chunk's y, which takes x's place and
+// leaves by a TMA store.  z has room only in C's second half between Yi and
+// the outputs, so it is brought to L2 a chunk ahead.  A chunk's chain is P and
+// w x from the scores (which run behind the previous chunk's products), Ya and
+// dH, and the new h.
 //
 // scan_tc_state_kernel, the first pass over split sequences: dH of a whole
 // segment in one accumulator, chunks from the last to the first, each
 // weighted by the decay to the segment's end.
 //
-// What bounds it.  The products of a chunk take about 2.4 K cycles of the
-// tensor pipe (64 per step of 16 at 128 columns, 48 at 64: half of it is the
-// three parts of w x), a chunk step about 6 K: the sixteen warps' conversions
-// between TMEM and shared memory stand in a chain with the products, and
-// shared memory (two stages of operands) leaves room for one CTA per SM.  64
-// heads of 64 x 128: 8192 tokens 25.5 us (first pass) and 106 us, with prep
-// and hand-over 141 us for 208 MB; 29,893 packed tokens that start from
-// states 417 us and 14 us of prep.  Measured and set aside: w x before P with
-// Yi double-buffered (113 us), products issued by a working warp (1.7 times).
+// What bounds it.  The products of a chunk take about 1.9 K cycles of the
+// tensor pipe (per step of 16 measured 64 at 128 columns and 48 at 64, by rate 96 at 192), a
+// chunk step 4.2 to 4.7 K: P and w x 2 K, Ya and dH 1.2 K beside the first
+// part of the outputs, the rest of them and h 1 K.  The sixteen warps' own
+// work takes as long as that chain (56 % of the issue slots, 36 % of the
+// tensor pipe), and shared memory leaves room for one CTA per SM.  64 heads of
+// 64 x 128: 8192 tokens 22 us (first pass) and 85 us, with steps and hand-over
+// 117 us for 208 MB; 29,893 packed tokens that start from states 331 us and 14
+// us of steps.  What each choice gave on those two: P through TMEM and one
+// product for dH 106 -> 105 and 417 -> 410 us (first pass 25.5 -> 22), z
+// before the next chunk's operands and in L2 88 and 351, operands as their
+// places become free 85 and 331.  Measured and set aside: w x before P (113
+// against 106), both halves of the scores behind one wait (86 and 336), w x
+// shared out by who has no block of P (84.5 and 330), products issued by a
+// working warp (1.7 times).
 //
 // Rounding.  x, B and C are bf16 already.  P and h are rounded to bf16 as
 // operands, as y is rounded to bf16 in the end.  w x is split into bf16 parts
