@@ -416,3 +416,33 @@ def test_later_tokens_stay_out_of_earlier_ones(what, generic):
         if what == "x":  # the other columns of the head never see it; its own state does
             assert torch.equal(y[:, 0, 1:], clean[:, 0, 1:]) and torch.equal(y[:, 1], clean[:, 1])
             assert not torch.isfinite(h[0 if at < 300 else 1, 0, 0]).any()
+
+
+def test_calls_in_a_graph():
+    """A prompt, a token and the norm behind them captured once and replayed on
+    new inputs."""
+    i = cuda({k: None if t is None else t.clone(memory_format=torch.contiguous_format)
+              for k, t in make(300, 4, 64, 1, 128, bf16, True, seed=11).items()})
+    cu = torch.tensor([0, 131, 300], dtype=torch.int32).cuda()
+    w = torch.rand(64, device="cuda")
+
+    def step(x, cache):
+        y, h = ops.chunk_selective_scan(x[None], i["dt"][None], i["A"], i["B"][None], i["C"][None], i["D"], i["z"][None],
+                                        i["dt_bias"], dt_softplus=True, output_final_state=True, cu_seqlens=cu)
+        cache.copy_(h)
+        t, _ = ops.selective_scan_update(x[:2], i["dt"][:2], i["A"], i["B"][:2], i["C"][:2], i["D"], i["z"][:2],
+                                         i["dt_bias"], dt_softplus=True, state=cache)
+        return y, t, ops.gated_rms_norm(y[0], w, i["z"])
+
+    x, cache = i["x"].clone(), torch.zeros(2, 4, 64, 128, device="cuda")
+    step(x, cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, cache)
+    x.copy_(i["x"].flip(0))
+    graph.replay()
+    other = torch.zeros_like(cache)
+    want = step(i["x"].flip(0).contiguous(), other)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(cache, other)
