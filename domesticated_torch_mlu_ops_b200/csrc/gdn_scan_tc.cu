@@ -35,15 +35,15 @@
 // part of the outputs, the rest of them and h 1 K.  The sixteen warps' own
 // work takes as long as that chain (56 % of the issue slots, 36 % of the
 // tensor pipe), and shared memory leaves room for one CTA per SM.  64 heads of
-// 64 x 128: 8192 tokens 22 us (first pass) and 85 us, with steps and hand-over
-// 117 us for 208 MB; 29,893 packed tokens that start from states 331 us and 14
+// 64 x 128: 8192 tokens 22 us (first pass) and 82 us, with steps and hand-over
+// 115 us for 208 MB; 29,893 packed tokens that start from states 327 us and 14
 // us of steps.  What each choice gave on those two: P through TMEM and one
 // product for dH 106 -> 105 and 417 -> 410 us (first pass 25.5 -> 22), z
 // before the next chunk's operands and in L2 88 and 351, operands as their
-// places become free 85 and 331.  Measured and set aside: w x before P (113
-// against 106), both halves of the scores behind one wait (86 and 336), w x
-// shared out by who has no block of P (84.5 and 330), products issued by a
-// working warp (1.7 times).
+// places become free 82 to 85 and 330.  Measured and set aside: w x and dH
+// before P, so that h is ready before the outputs (96 and 381), both halves of
+// the scores behind one wait (86 and 336), w x shared out by who has no block
+// of P (84 and 330), products issued by a working warp (1.7 times).
 //
 // Rounding.  x, B and C are bf16 already.  P and h are rounded to bf16 as
 // operands, as y is rounded to bf16 in the end.  w x is split into bf16 parts
