@@ -124,6 +124,18 @@ def _bwd_workspace(B, T, N, D, W, x_dtype):
     return n
 
 
+def _token_rows(t):
+    """(tensor, distance between its B*T token rows) of ``t [B, T, D]``: in
+    place when only the rows are strided (a view of one projection), else a
+    packed copy."""
+    B, T, D = t.shape
+    if not t.is_contiguous() and t.stride(2) == 1:
+        row = t.stride(1) if T > 1 else t.stride(0) if B > 1 else D
+        if row >= D and (B == 1 or t.stride(0) == T * row):
+            return t, row
+    return t.contiguous(), D
+
+
 def _conv1d_bwd_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], dy: torch.Tensor,
                      initial_state: Optional[torch.Tensor], activation: int,
                      cu_seqlens: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor,
@@ -135,12 +147,7 @@ def _conv1d_bwd_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     N = B if cu_seqlens is None else cu_seqlens.numel() - 1
     dev = x.device
 
-    def rows(t):  # token rows may be strided (a view of one projection), else a packed copy
-        if not t.is_contiguous() and t.stride(2) == 1 and t.stride(1) >= D and (B == 1 or t.stride(0) == T * t.stride(1)):
-            return t, t.stride(1) if T > 1 else D
-        return t.contiguous(), D
-
-    (x, sx), (dy, sdy) = rows(x), rows(dy)
+    (x, sx), (dy, sdy) = _token_rows(x), _token_rows(dy)
     dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
     dw = torch.empty_like(weight)
     db = torch.empty(0 if bias is None else D, dtype=weight.dtype, device=dev)

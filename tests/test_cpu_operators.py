@@ -12,6 +12,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 import domesticated_torch_mlu_ops_b200 as ops
 from domesticated_torch_mlu_ops_b200 import _lib
+from domesticated_torch_mlu_ops_b200.conv import _token_rows
 from domesticated_torch_mlu_ops_b200.norm import _row_strides, _two_strides
 from domesticated_torch_mlu_ops_b200.scan import _aligned_rows, _packed_rows
 
@@ -161,3 +162,19 @@ def test_views_are_read_in_place_where_they_can_be():
     x, z, heads, sxt, sxh, szt, szh = _two_strides(wide.contiguous().view(10, 5, 8), wide[..., :24].unflatten(-1, (3, 8)).
                                                    reshape(10, 3, 8)[:, :1].expand(10, 5, 8))
     assert (heads, sxt, sxh) == (5, 40, 8) and (szt, szh) == (40, 0)
+
+
+@pytest.mark.parametrize("B,T", [(1, 1), (3, 1), (1, 5), (3, 5), (2, 0), (0, 4)])
+def test_token_rows_of_batched_views(B, T):
+    """Row r of the B*T token rows lies r strides from the first, also where
+    one token per sequence leaves the distance between batches to tell it."""
+    D = 6
+    wide = torch.arange(B * T * 10.).view(B, T, 10)
+    for view in (wide, wide[..., 3:3 + D], wide[..., :D].contiguous(), wide[:1, :, :D].expand(B, T, D) if B else wide,
+                 torch.zeros(B, 2 * T + 1, 10)[:, :T, 2:2 + D]):
+        t, row = _token_rows(view)
+        assert row >= view.shape[2] and torch.equal(t, view)
+        n = B * T
+        if n:
+            seen = t.as_strided((n, view.shape[2]), (row, 1), t.storage_offset())
+            assert torch.equal(seen, view.reshape(n, view.shape[2]))

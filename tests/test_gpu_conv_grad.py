@@ -200,3 +200,23 @@ def test_refusals():
         ops.causal_conv1d_bwd(x.double(), w, None, x.double())
     with pytest.raises(ValueError, match="width"):
         ops.causal_conv1d_bwd(x, torch.randn(16, 17, device="cuda"), None, x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("strided", ["x", "dy", "autograd"])
+def test_single_tokens_of_a_strided_batch(dtype, strided):
+    """One token per sequence: the rows are a batch stride apart."""
+    B, D, W = 3, 96, 4
+    g = torch.Generator().manual_seed(7)
+    proj = torch.randn(B, 1, D + 40, generator=g).to(dtype).cuda()
+    view, whole = proj[..., 8:8 + D], torch.randn(B, 1, D, generator=g).to(dtype).cuda()
+    x, dy = (whole, view) if strided == "dy" else (view, whole)
+    w = torch.randn(D, W, generator=g).cuda()
+    rx, rw, _, _ = reference(x.reshape(B, D).cpu(), dy.reshape(B, D).cpu(), w.cpu(), None, None, [1] * B, True)
+    if strided == "autograd":
+        leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+        dx, dw = torch.autograd.grad(ops.causal_conv1d(*leaves, activation="silu")[0], leaves, dy)
+    else:
+        dx, dw, _, _ = ops.causal_conv1d_bwd(x, w, None, dy, activation="silu")
+    assert rel(dx.reshape(B, D), rx) <= U[dtype] + 64 * F32
+    assert rel(dw, rw) <= U[torch.float32] + F32 * (64 + 4 * B ** 0.5)
