@@ -4,6 +4,7 @@ fakes, host-side view handling (no GPU needed)."""
 
 import ctypes
 import os
+import re
 import subprocess
 
 import pytest
@@ -178,3 +179,21 @@ def test_token_rows_of_batched_views(B, T):
         if n:
             seen = t.as_strided((n, view.shape[2]), (row, 1), t.storage_offset())
             assert torch.equal(seen, view.reshape(n, view.shape[2]))
+
+
+def test_loads_of_tensor_memory_are_fenced_behind_their_wait():
+    """Every helper that loads from tensor memory and waits passes each loaded
+    register through a fence after the wait: nothing else keeps the compiler
+    from scheduling a use before it."""
+    src = open(os.path.join(os.path.dirname(HEADER), "..", "domesticated_torch_mlu_ops_b200", "csrc", "umma.cuh")).read()
+    helpers = [h for h in src.split("__device__ __forceinline__")[1:] if "tcgen05.ld.sync" in h]
+    assert len(helpers) >= 4
+    for h in helpers:
+        name = h.split("(")[0].split()[-1]
+        loaded = sum(int(n) for n in re.findall(r"tcgen05\.ld\.sync\.aligned\.32x32b\.x(\d+)", h))
+        if name.endswith("_nw"):  # the caller waits and fences
+            assert "tmem_wait_ld" not in h
+            continue
+        assert "tcgen05.wait" not in h and h.count("tmem_wait_ld();") == 1, name
+        behind = h.split("tmem_wait_ld();")[1]
+        assert sum(int(n) for n in re.findall(r"reg_fence(\d+)\(", behind)) == loaded, name
