@@ -1,19 +1,19 @@
 // Selective scan over prompts on the tensor cores (tcgen05), bf16.
 //
 // A small kernel first turns the raw steps into what the tiles need per token
-// and head: a_i, the log2 decay from the start of the token's 128-token chunk
-// to it, and k_i = dt'_i times the decay from it to the end of its block of
-// 32 (scan_prep_kernel).
+// and head: a_i, the log2 decay from the start of the token's block of 32 to
+// it, k_i = dt'_i times the decay from it to the block's end, and the log2
+// decays over whole blocks (scan_prep_kernel).
 //
 // scan_tc_kernel: one CTA per (segment of a sequence, head, 64 columns of P),
 // one per SM: sixteen warps that share the elementwise work and one that
 // issues copies and products.  It walks the segment in chunks of 128 tokens:
 //   S  = C B^T                                   [128, 128]
 //   Yi = C h                                     [128, 64], h as bf16
-//   P_ij = S_ij exp(a_i - a_j) dt'_j  (j <= i)   rounded to bf16 once
-//   Ya = P x;   y = exp(a_i) Yi + Ya + D x       in fp32, then the gate
-//   dH = B^T (w x),  w_j = exp(a_end - a_j) dt'_j
-//   h <- exp(a_end) h + dH                       fp32, in registers
+//   P_ij = S_ij decay(j to i) dt'_j  (j <= i)    rounded to bf16 once
+//   Ya = P x;   y = decay(to i) Yi + Ya + D x    in fp32, then the gate
+//   dH = B^T (w x),  w_j = decay(j to the end) dt'_j
+//   h <- decay(chunk) h + dH                     fp32, in registers
 // Four products with fp32 accumulators in TMEM.  P replaces the scores there
 // and is Ya's operand from there; the parts of w x lie side by side, so that
 // dH is one product that reads B once.  x, B and C come by TMA into
@@ -51,12 +51,15 @@
 // y, three (24 bits) where it is returned or handed on, so that a returned
 // fp32 state has fp32 precision.
 //
-// exp(a_i - a_j) = exp(a_i - a_r) (exp(a_r - a_j) dt'_j) with r the end of j's
-// block: one exponential per row and block instead of one per element.  Left
-// of the diagonal both factors are at most 1.  In the diagonal block the
-// first grows as the block decays; above 2^100 that block takes the
-// difference itself.  k is summed from the block's end, not as a difference
-// of prefix sums, so w keeps its relative precision under fast decays.
+// Decays are products of sums that only add: the decay between two blocks' is
+// exp(a_i + the blocks between) k_j, w is k times the blocks after.  No
+// difference of long prefix sums occurs, whose rounding would stay behind a
+// fast decay as the error of the slow ones after it.  Within the diagonal
+// block P takes exp(a_i) kd_j with kd_j = dt'_j / exp(a_j) while no a reaches
+// 100 there (kd stays in range, and the rounding of a under 2^-17); rows past
+// that take the sum between the two tokens itself.  Either way it depends on
+// no later token.  One exponential per row and block instead of one per
+// element.
 
 #include <cuda.h>
 
@@ -75,9 +78,14 @@ constexpr int kLead = kWork / 32;
 constexpr long long kWaitLimit = 2000000000LL;
 
 struct PrepOut {
-  float *a, *k, *dt;  // [H][chunks][128]; past a sequence's end a stays, k and dt are 0
+  float *a, *k, *dt;  // [H][chunks][128]; past a sequence's end the step dt is 0
+  float* sums;        // [H][chunks][kSums], of a over whole blocks of 32:
   int64_t chunks;
 };
+// before block b, after it, between block J and block I > J, and of the chunk
+constexpr int kSums = 28, kBefore = 0, kAfter = 4, kBetween = 8, kWhole = 24;
+constexpr int kStepBytes = 2 * kL * 4 + kSums * 4;  // a stage of a, k and the sums
+constexpr float kFar = 100.f;                       // see the diagonal block above
 
 template <int S_>
 struct Smem {
@@ -89,13 +97,13 @@ struct Smem {
   static constexpr int kStage = kX + kTile;
   static constexpr int kXs = 2 * kStage;                    // the parts of w x
   static constexpr int kH = kXs + 3 * kTile;                // h
-  static constexpr int kSc = kH + kTile;              // two stages of a and k
-  static constexpr int kBar = kSc + 2 * 2 * kL * 4;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
+  static constexpr int kSc = kH + kTile;               // two stages of a, k and the sums
+  static constexpr int kBar = kSc + 2 * kStepBytes;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
   static constexpr int kBars = 9;
   static constexpr int kTmem = kBar + kBars * 8;
   static constexpr int kBad = kTmem + 8;                    // [2][64 columns + 1]: see the kernel
   static constexpr int kBytes = kBad + 2 * 65 * 4;
-  static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile + 2 * kL * 4;
+  static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile + kStepBytes;
   // TMEM columns: S first (P in its place), dH one accumulator per part of w x
   static constexpr int kCols = 512, kYi = 128, kYa = 192, kDH = 256;
   static_assert(kBytes <= 227 * 1024, "shared memory");
@@ -108,8 +116,9 @@ struct StateSmem {
   static constexpr int kBStage = S_ / 64 * kTile;
   static constexpr int kX = 3 * kBStage;
   static constexpr int kXs = kX + 2 * kTile;
-  static constexpr int kSc = kXs + 6 * kTile;   // two stages of a and k, with x
-  static constexpr int kBar = kSc + 2 * 2 * kL * 4;  // B[3], x[2], parts ready[2], products[2]
+  static constexpr int kStep = (kL + kSums) * 4;
+  static constexpr int kSc = kXs + 6 * kTile;   // two stages of k and the sums, with x
+  static constexpr int kBar = kSc + 2 * kStep;  // B[3], x[2], parts ready[2], products[2]
   static constexpr int kTmem = kBar + 9 * 8;
   static constexpr int kBytes = kTmem + 8;
   static constexpr int kCols = 256;  // an accumulator per part
@@ -145,7 +154,7 @@ __device__ __forceinline__ uint4 take_part(float2* v) {
 // Steps of one chunk of 128 tokens for 16 heads per block (a 32-byte sector
 // of 16-bit steps): raw steps in through shared memory (rows of heads are what
 // is contiguous), a, k and dt out per head with tokens contiguous.  A warp
-// scans a head's 128 tokens, four per lane.
+// scans a head's 128 tokens, four per lane, a block of 32 per eight lanes.
 constexpr int kPrepHeads = 16;
 __global__ void __launch_bounds__(kPrepHeads * 32) scan_prep_kernel(const ScanParams p, const PrepOut o) {
   __shared__ float raw[kL][kPrepHeads + 1];
@@ -185,40 +194,36 @@ __global__ void __launch_bounds__(kPrepHeads * 32) scan_prep_kernel(const ScanPa
     for (int e = 1; e < 4; ++e) pre[e] = pre[e - 1] + a[e];
 #pragma unroll
     for (int e = 2; e >= 0; --e) suf[e] = suf[e + 1] + a[e + 1];
-    float up = pre[3], dn = suf[0] + a[0];  // lane totals -> sums over earlier lanes, later lanes of the block
+    float up = pre[3], dn = suf[0] + a[0];  // lane totals -> sums over the block's earlier lanes, and its later ones
 #pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const float v = __shfl_up_sync(0xffffffffu, up, s);
-      if (lane >= s) up += v;
-    }
-    up = __shfl_up_sync(0xffffffffu, up, 1);
-    if (lane == 0) up = 0.f;
-#pragma unroll
-    for (int s = 1; s < 8; s <<= 1) {  // a block of 32 tokens is 8 lanes
-      const float v = __shfl_down_sync(0xffffffffu, dn, s, 8);
+    for (int s = 1; s < 8; s <<= 1) {
+      const float u = __shfl_up_sync(0xffffffffu, up, s, 8), v = __shfl_down_sync(0xffffffffu, dn, s, 8);
+      if ((lane & 7) >= s) up += u;
       if ((lane & 7) + s < 8) dn += v;
     }
+    up = __shfl_up_sync(0xffffffffu, up, 1, 8);
     dn = __shfl_down_sync(0xffffffffu, dn, 1, 8);
+    if ((lane & 7) == 0) up = 0.f;
     if ((lane & 7) == 7) dn = 0.f;
-    const int64_t at = (h * o.chunks + blockIdx.x) * kL + lane * 4;
-    float4 oa, ok;
-    oa = make_float4(up + pre[0], up + pre[1], up + pre[2], up + pre[3]);
-    if (len > 0 && len < kL) {
-      // past the end a is the last token's to the bit: the decay between the
-      // two is exactly 1, whatever the size of a (another lane's sum of the
-      // same terms may round otherwise)
-      const int e = (len - 1) & 3;
-      const float mine = e < 2 ? (e == 0 ? oa.x : oa.y) : (e == 2 ? oa.z : oa.w);
-      const float end = __shfl_sync(0xffffffffu, mine, (len - 1) >> 2);
-      if (lane * 4 >= len) oa.x = end;
-      if (lane * 4 + 1 >= len) oa.y = end;
-      if (lane * 4 + 2 >= len) oa.z = end;
-      if (lane * 4 + 3 >= len) oa.w = end;
-    }
-    ok = make_float4(ex2(suf[0] + dn) * d[0], ex2(suf[1] + dn) * d[1], ex2(suf[2] + dn) * d[2], ex2(suf[3] + dn) * d[3]);
-    *reinterpret_cast<float4*>(o.a + at) = oa;
-    *reinterpret_cast<float4*>(o.k + at) = ok;
+    const int64_t chunk = h * o.chunks + blockIdx.x, at = chunk * kL + lane * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pre[e] += up;
+    *reinterpret_cast<float4*>(o.a + at) = make_float4(pre[0], pre[1], pre[2], pre[3]);
+    *reinterpret_cast<float4*>(o.k + at) =
+        make_float4(ex2(suf[0] + dn) * d[0], ex2(suf[1] + dn) * d[1], ex2(suf[2] + dn) * d[2], ex2(suf[3] + dn) * d[3]);
     *reinterpret_cast<float4*>(o.dt + at) = make_float4(d[0], d[1], d[2], d[3]);
+    float tot[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) tot[b] = __shfl_sync(0xffffffffu, pre[3], b * 8 + 7);
+    if (lane < kSums) {
+      const int from = lane < kAfter ? 0 : lane < kBetween ? lane - kAfter + 1 : lane < kWhole ? (lane & 3) + 1 : 0;
+      const int to = lane < kAfter ? lane : lane < kBetween ? 4 : lane < kWhole ? (lane - kBetween) >> 2 : 4;
+      float v = 0.f;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (b >= from && b < to) v += tot[b];
+      o.sums[chunk * kSums + lane] = v;
+    }
   }
 }
 
@@ -226,21 +231,6 @@ __device__ __forceinline__ float lds4(uint32_t a) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
   return v;
-}
-
-// What a thread (token `row` of a chunk) needs of a and k, from their stage.
-struct TokenScalars {
-  float a, k;    // its own
-  float end[4];  // a at the end of each block of 32
-  __device__ __forceinline__ void load(uint32_t at, int row) {
-    a = lds4(at + row * 4);
-    k = lds4(at + (kL + row) * 4);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) end[b] = lds4(at + (b * 32 + 31) * 4);
-  }
-};
-__device__ __forceinline__ float pick4(const float* v, int q) {
-  return q < 2 ? (q == 0 ? v[0] : v[1]) : (q == 2 ? v[2] : v[3]);
 }
 
 // Byte offsets of a thread's two 16-byte pieces (columns 16 cq .. 16 cq + 15
@@ -257,6 +247,11 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void sts4(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" :: "r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ float4 lds16f(uint32_t a) {
+  const uint4 v = lds16(a);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
 __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -271,9 +266,9 @@ __device__ __forceinline__ void publish(uint32_t bar) {
   __syncwarp();
 }
 
-// P's columns of k-step ks in TMEM: each block of 32 in the first half of the
-// scores that it came from.
-__host__ __device__ constexpr uint32_t p_step(int ks) { return (ks >> 1) * 32 + (ks & 1) * 8; }
+// P's columns of k-step ks in TMEM: in the first half of the 16 scores that
+// they came from.
+__host__ __device__ constexpr uint32_t p_step(int ks) { return ks * 16; }
 // What k-step ks of 16 adds to an operand descriptor.
 __host__ __device__ constexpr uint64_t k_step(int ks) { return ((ks >> 2) * kTile + (ks & 3) * 32) >> 4; }
 __host__ __device__ constexpr uint64_t mn_step(int ks) { return (ks * 2048) >> 4; }
@@ -286,21 +281,43 @@ __device__ __forceinline__ bool base_ok(const ScanParams& p, uint32_t sbase) {
   return false;
 }
 
-// A diagonal block of P under decays past 2^100 within it: the difference of
-// each pair.  Out of line: its registers would push the common path's out.
-__device__ __noinline__ void diag_by_difference(uint32_t ts, int row, float ai, float dt) {
+// Where value 4 r of the diagonal block's kd is: a warp keeps them in the first
+// pieces that it will write of the block's first eight rows of w x.
+__device__ __forceinline__ uint32_t kd_at(uint32_t tile, int quad, int r) {
+  return tile + (quad * 32 + r) * 128 + (((quad * 2) ^ r) << 4);
+}
+
+// A diagonal block of P with rows whose a, or an earlier one, is not under
+// kFar: those take the sum of the steps between the two tokens.  `step` is the
+// row's own log2 decay, dt its step.  Out of line: its registers would push the
+// common path's out.
+__device__ __noinline__ void diag_by_sums(uint32_t ts, int row, float ai, float step, float dt, uint32_t tile) {
   const int lane = row & 31;
-#pragma unroll 1
-  for (int q = 0; q < 4; ++q) {
-    float v[8];
-    umma::tmem_ld8(ts + q * 8, v);
+  float most = fabsf(ai) < kFar ? 0.f : 1.f;  // a NaN counts
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = q * 8 + e;
-      const float aj = __shfl_sync(0xffffffffu, ai, j), dj = __shfl_sync(0xffffffffu, dt, j);
-      v[e] = j <= lane ? v[e] * (ex2(ai - aj) * dj) : 0.f;
+  for (int s = 1; s < 32; s <<= 1) {
+    const float v = __shfl_up_sync(0xffffffffu, most, s);
+    if (lane >= s) most = fmaxf(most, v);
+  }
+  const float f = ex2(ai);
+  float sum = 0.f;  // of the steps after token j up to the row's
+#pragma unroll 1
+  for (int hf = 1; hf >= 0; --hf) {
+    float v[16];
+    umma::tmem_ld16(ts + hf * 16, v);
+#pragma unroll
+    for (int q = 3; q >= 0; --q) {
+      const float4 k4 = lds16f(kd_at(tile, row >> 5, hf * 4 + q));
+      const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int e = 3; e >= 0; --e) {
+        const int i = q * 4 + e, j = hf * 16 + i;
+        const float next = __shfl_sync(0xffffffffu, step, (j + 1) & 31), dj = __shfl_sync(0xffffffffu, dt, j);
+        if (j < lane) sum += next;
+        v[i] = j <= lane ? v[i] * (most == 0.f ? f * kk[e] : ex2(sum) * dj) : 0.f;
+      }
     }
-    umma::tmem_st4(ts + q * 4, tc::pack8<__nv_bfloat16>(v));
+    umma::tmem_st8(ts + hf * 16, tc::pack8<__nv_bfloat16>(v), tc::pack8<__nv_bfloat16>(v + 8));
   }
 }
 
@@ -416,8 +433,10 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     auto fetch_bc = [&](int c) {
       const uint32_t bar = bar_ld + (c & 1) * 8;
       umma::mbar_arrive_expect_tx(bar, M::kTx);
-      umma::bulk_g2s(sm + M::kSc + (c & 1) * 2 * kL * 4, prep.a + prow + c * kL, kL * 4, bar);
-      umma::bulk_g2s(sm + M::kSc + (c & 1) * 2 * kL * 4 + kL * 4, prep.k + prow + c * kL, kL * 4, bar);
+      uint8_t* sc = sm + M::kSc + (c & 1) * kStepBytes;
+      umma::bulk_g2s(sc, prep.a + prow + c * kL, kL * 4, bar);
+      umma::bulk_g2s(sc + kL * 4, prep.k + prow + c * kL, kL * 4, bar);
+      umma::bulk_g2s(sc + 2 * kL * 4, prep.sums + (prow / kL + c) * kSums, kSums * 4, bar);
 #pragma unroll
       for (int q = 0; q < S_ / 64; ++q)
         umma::tma_load_2d(sm + (c & 1) * M::kStage + M::kB + q * kTile, &tb, g * S_ + q * 64, static_cast<int>(t0) + c * kL, bar);
@@ -555,7 +574,8 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     const int64_t col = static_cast<int64_t>(h) * p.P + p0 + cq * 16;
     auto state_at = [&](int64_t i) { return ((i * p.H + h) * p.P + p0 + cq * 16) * S_ + row; };
     const float D = p.D ? p.D[h] : 0.f;
-    TokenScalars sc;
+    float dt_next = 0.f;  // of the diagonal block, loaded a chunk ahead
+    if (cq == quad && nch > 0) dt_next = __ldg(prep.dt + prow + row);
     float2 hr[8];  // h[s = row][16 columns of P]
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -578,22 +598,26 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     for (int c = 0; c < nch; ++c) {
       const int len = length(c);
       const uint32_t st = sbase + (c & 1) * M::kStage;
-      const uint32_t sc_at = sbase + M::kSc + (c & 1) * 2 * kL * 4;
+      const uint32_t sc_at = sbase + M::kSc + (c & 1) * kStepBytes;
+      const float dt = dt_next;
+      if (cq == quad && c + 1 < nch) dt_next = __ldg(prep.dt + prow + (c + 1) * kL + row);
       if (!wait(bar_ld + (c & 1) * 8, (c >> 1) & 1, kSiteScanLoad)) break;
-      sc.load(sc_at, row);
-      const float ai = sc.a, all = sc.end[3];
-      const float wj = sc.k * ex2(all - pick4(sc.end, quad));
+      const uint32_t sums_at = sc_at + 2 * kL * 4;
+      const float ai = lds4(sc_at + row * 4), wj = lds4(sc_at + (kL + row) * 4) * ex2(lds4(sums_at + (kAfter + quad) * 4));
+      const float g1 = ex2(lds4(sums_at + (kBefore + quad) * 4) + ai), decay = ex2(lds4(sums_at + kWhole * 4));
       // ---- P from the scores: block of columns J = cq ----
+      if (cq == quad) {
+        sts4(kd_at(sbase + M::kXs, quad, lane >> 2) + (lane & 3) * 4, ex2(-ai) * dt);
+        __syncwarp();
+      }
       if (!wait(bar_s, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
       const uint32_t ts = tl + cq * 32;
       if (cq <= quad) {
-        const float far = ai - pick4(sc.end, cq);
         const bool diag = cq == quad;
-        // far is largest in the block's first row: one answer per warp
-        if (!diag || __shfl_sync(0xffffffffu, far, 0) < 100.f) {
+        if (!diag || __all_sync(0xffffffffu, fabsf(ai) < kFar)) {
           const uint32_t cf = sc_at + (kL + cq * 32) * 4;
-          const float f = ex2(far);
+          const float f = ex2(diag ? ai : ai + lds4(sums_at + (kBetween + quad * 4 + cq) * 4));
           const float2 f2 = make_float2(f, f);
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {  // 16 columns at a time: registers
@@ -602,7 +626,9 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
             umma::tmem_ld16(ts + hf * 16, v);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              const uint4 k0 = lds16(cf + hf * 64 + q * 32), k1 = lds16(cf + hf * 64 + q * 32 + 16);
+              const int r = hf * 4 + q * 2;
+              const uint4 k0 = lds16(diag ? kd_at(sbase + M::kXs, quad, r) : cf + r * 16),
+                          k1 = lds16(diag ? kd_at(sbase + M::kXs, quad, r + 1) : cf + r * 16 + 16);
               const uint32_t kk[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
               float2 w[4];
 #pragma unroll
@@ -617,15 +643,15 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
               }
               u[q] = pack8(w);
             }
-            umma::tmem_st8(ts + hf * 8, u[0], u[1]);  // over scores that have been read
+            umma::tmem_st8(ts + hf * 16, u[0], u[1]);  // over scores that have been read
           }
         } else {
-          diag_by_difference(ts, row, ai, __ldg(prep.dt + prow + c * kL + row));
+          diag_by_sums(ts, row, ai, dt * (p.A[h] * tc::kLog2e), dt, sbase + M::kXs);
         }
       } else {
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
         umma::tmem_st8(ts, zero, zero);
-        umma::tmem_st8(ts + 8, zero, zero);
+        umma::tmem_st8(ts + 16, zero, zero);
       }
       // ---- w x in parts (x has been there since the scores were issued) ----
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
@@ -668,7 +694,6 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       if (!wait(bar_yi, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
       {
-        const float g1 = ex2(ai);
         const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
         const bool has_yi = c > 0 || seg || ini;
 #pragma unroll
@@ -722,7 +747,6 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       // ---- state ----
       if (!wait(bar_dh, c & 1, kSiteScanState)) break;
       umma::fence_after_sync();
-      const float decay = ex2(all);
       {
         const float2 decay2 = make_float2(decay, decay);
         float d[16], e[16];
@@ -814,10 +838,10 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     };
     auto fetch_x = [&](int i) {
       const uint32_t bar = bar_x + (i & 1) * 8;
-      uint8_t* sc = sm + M::kSc + (i & 1) * 2 * kL * 4;
-      umma::mbar_arrive_expect_tx(bar, kTile + 2 * kL * 4);
-      umma::bulk_g2s(sc, prep.a + prow + (nch - 1 - i) * kL, kL * 4, bar);
-      umma::bulk_g2s(sc + kL * 4, prep.k + prow + (nch - 1 - i) * kL, kL * 4, bar);
+      uint8_t* sc = sm + M::kSc + (i & 1) * M::kStep;
+      umma::mbar_arrive_expect_tx(bar, kTile + M::kStep);
+      umma::bulk_g2s(sc, prep.k + prow + (nch - 1 - i) * kL, kL * 4, bar);
+      umma::bulk_g2s(sc + kL * 4, prep.sums + (prow / kL + nch - 1 - i) * kSums, kSums * 4, bar);
       umma::tma_load_2d(sm + M::kX + (i & 1) * kTile, &tx, h * p.P + p0, token(i), bar);
     };
     if (umma::elect_one()) {
@@ -862,13 +886,13 @@ scan_tc_state_kernel(const ScanParams p, const PrepOut prep, const int slices, c
     const int quad = warp & 3, cq = warp >> 2, row = quad * 32 + lane;
     const Pieces piece(row, cq);
     float later = 0.f;  // log2 decay from the chunk's end to the piece's
-    TokenScalars sc;
     for (int i = 0; i < nch; ++i) {
       const uint32_t xt = sbase + M::kX + (i & 1) * kTile, xs = sbase + M::kXs + (i & 1) * 3 * kTile;
       if (!wait(bar_x + (i & 1) * 8, (i >> 1) & 1, kSiteScanLoad)) break;
-      sc.load(sbase + M::kSc + (i & 1) * 2 * kL * 4, row);
-      const float wj = sc.k * ex2(sc.end[3] - pick4(sc.end, quad)) * ex2(later);
-      later += sc.end[3];
+      const uint32_t sc_at = sbase + M::kSc + (i & 1) * M::kStep;
+      const uint32_t sums_at = sc_at + kL * 4;
+      const float wj = lds4(sc_at + row * 4) * ex2(lds4(sums_at + (kAfter + quad) * 4)) * ex2(later);
+      later += lds4(sums_at + kWhole * 4);
       if (i >= 2 && !wait(bar_dh + (i & 1) * 8, ((i - 2) >> 1) & 1, kSiteScanState)) break;  // the parts' tiles are read
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -936,7 +960,7 @@ static cudaError_t make_rows_map(CUtensorMap* m, const void* ptr, int64_t cols, 
 // Chunks of 128 tokens: every sequence has at most ceil(len / 128), and at least one.
 static int64_t prep_chunks(const gdn_scan_args& a) { return a.B * a.T / kL + a.N; }
 size_t tc_scratch_bytes(const gdn_scan_args& a) {
-  return static_cast<size_t>(prep_chunks(a)) * kL * a.H * 3 * sizeof(float);
+  return static_cast<size_t>(prep_chunks(a)) * a.H * (3 * kL + kSums) * sizeof(float);
 }
 
 template <int S_>
@@ -951,7 +975,7 @@ static cudaError_t run_tc(ScanParams p, const gdn_scan_args& a, float* scratch, 
   if ((e = make_rows_map(&tz, a.z ? a.z : a.y, hp, total, a.z ? a.stride_z : hp)) != cudaSuccess) return e;
   const int slices = a.P / 64;
   const int64_t chunks = prep_chunks(a), each = chunks * kL * a.H;
-  const PrepOut prep{scratch, scratch + each, scratch + 2 * each, chunks};
+  const PrepOut prep{scratch, scratch + each, scratch + 2 * each, scratch + 3 * each, chunks};
   ScanParams q = p;
   q.seg = kL;
   note_launch();

@@ -446,3 +446,21 @@ def test_calls_in_a_graph():
     want = step(i["x"].flip(0).contiguous(), other)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(cache, other)
+
+
+@pytest.mark.parametrize("lens,every", [([120, 128, 33], 128), ([17, 400], 128), ([1400], 1400)])
+@pytest.mark.parametrize("S", [64, 128])
+def test_slow_decays_behind_a_fast_one(lens, every, S):
+    """Sixteen tokens that wipe the state out, then hundreds that hardly decay:
+    the weights of the slow ones keep fp32 precision, in the last segment
+    (bursts in every chunk) and in the segments before it (one burst)."""
+    i = make(sum(lens), 2, 64, 1, S, bf16, False, seed=18)
+    i["A"], i["dt_bias"] = torch.tensor([-1.0, -0.5]), torch.zeros(2)
+    at = torch.cat([torch.arange(n) for n in lens]) % every
+    burst = (at >= 20) & (at < 36) if every > 128 else at < 16
+    i["dt"] = torch.where(burst, 300.0, -6.9)[:, None].expand(-1, 2).to(bf16).contiguous()
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], None, i["dt_bias"], True, (0.0, float("inf")),
+                      None, lens)
+    y, h = run(i, lens)
+    assert rel(h, rh) <= 64 * F32
+    assert rel(y, ry) <= tolerances(bf16, True)
