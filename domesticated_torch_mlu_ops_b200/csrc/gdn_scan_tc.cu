@@ -9,14 +9,14 @@
 // one per SM: sixteen warps that share the elementwise work and one that
 // issues copies and products.  It walks the segment in chunks of 128 tokens:
 //   S  = C B^T                                   [128, 128]
-//   Yi = C h                                     [128, 64], h as bf16
-//   P_ij = S_ij decay(j to i) dt'_j  (j <= i)    rounded to bf16 once
-//   Ya = P x;   y = decay(to i) Yi + Ya + D x    in fp32, then the gate
+//   Yi = C h                                     [128, 64]
+//   P_ij = S_ij decay(j to i) dt'_j  (j <= i),   P_ii += D
+//   Ya = P x;   y = decay(to i) Yi + Ya          in fp32, then the gate
 //   dH = B^T (w x),  w_j = decay(j to the end) dt'_j
 //   h <- decay(chunk) h + dH                     fp32, in registers
 // Four products with fp32 accumulators in TMEM.  P replaces the scores there
-// and is Ya's operand from there; the parts of w x lie side by side, so that
-// dH is one product that reads B once.  x, B and C come by TMA into
+// and is Ya's operand from there; the parts of h and of w x lie side by side,
+// so that Yi reads C and dH reads B once.  x, B and C come by TMA into
 // 128-byte-swizzled tiles that serve as operands in both directions, each as
 // soon as its place is free: B and C's first half behind the products of the
 // chunk before the last, x after that chunk's y, which takes x's place and
@@ -45,11 +45,13 @@
 // the scores behind one wait (86 and 336), w x shared out by who has no block
 // of P (84 and 330), products issued by a working warp (1.7 times).
 //
-// Rounding.  x, B and C are bf16 already.  P and h are rounded to bf16 as
-// operands, as y is rounded to bf16 in the end.  w x is split into bf16 parts
-// whose products are summed: two parts (16 bits) where the state only feeds
-// y, three (24 bits) where it is returned or handed on, so that a returned
-// fp32 state has fp32 precision.
+// Rounding.  x, B and C are bf16 already.  P, h and w x are split into bf16
+// parts whose products are summed: two parts (16 bits) where they only feed y,
+// which is rounded to 8 bits in the end, so that an output in 64 at most rounds
+// otherwise than the exact one; three (24 bits) of w x where the state is
+// returned or handed on, so that a returned fp32 state has fp32 precision.
+// One part of P and h each would take 22 and 77 us less on the two prompts
+// above and turn a fifth of the outputs.
 //
 // Decays are products of sums that only add: the decay between two blocks' is
 // exp(a_i + the blocks between) k_j, w is k times the blocks after.  No
@@ -96,7 +98,8 @@ struct Smem {
   static constexpr int kX = kB + S_ / 64 * kTile;           // x, then y
   static constexpr int kStage = kX + kTile;
   static constexpr int kXs = 2 * kStage;                    // the parts of w x
-  static constexpr int kH = kXs + 3 * kTile;                // h
+  static constexpr int kHlo = kXs + 2 * kTile;              // h's second part, in turns with the third of w x
+  static constexpr int kH = kXs + 3 * kTile;                // h's first part
   static constexpr int kSc = kH + kTile;               // two stages of a, k and the sums
   static constexpr int kBar = kSc + 2 * kStepBytes;    // loads[2], S, Yi, Ya, dH, z, h ready, P and w x ready
   static constexpr int kBars = 9;
@@ -104,8 +107,9 @@ struct Smem {
   static constexpr int kBad = kTmem + 8;                    // [2][64 columns + 1]: see the kernel
   static constexpr int kBytes = kBad + 2 * 65 * 4;
   static constexpr uint32_t kTx = (S_ / 64 * 2 + 1) * kTile + kStepBytes;
-  // TMEM columns: S first (P in its place), dH one accumulator per part of w x
-  static constexpr int kCols = 512, kYi = 128, kYa = 192, kDH = 256;
+  // TMEM columns: S first (P in its place), Yi one accumulator per part of h
+  // (the second part's first), dH one per part of w x
+  static constexpr int kCols = 512, kYi = 128, kDH = 256, kYa = 448;
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -266,9 +270,9 @@ __device__ __forceinline__ void publish(uint32_t bar) {
   __syncwarp();
 }
 
-// P's columns of k-step ks in TMEM: in the first half of the 16 scores that
-// they came from.
-__host__ __device__ constexpr uint32_t p_step(int ks) { return ks * 16; }
+// Columns of k-step ks of P's two parts in TMEM: side by side where the 16
+// scores were that they came from.
+__host__ __device__ constexpr uint32_t p_step(int ks, int part) { return ks * 16 + part * 8; }
 // What k-step ks of 16 adds to an operand descriptor.
 __host__ __device__ constexpr uint64_t k_step(int ks) { return ((ks >> 2) * kTile + (ks & 3) * 32) >> 4; }
 __host__ __device__ constexpr uint64_t mn_step(int ks) { return (ks * 2048) >> 4; }
@@ -291,7 +295,8 @@ __device__ __forceinline__ uint32_t kd_at(uint32_t tile, int quad, int r) {
 // kFar: those take the sum of the steps between the two tokens.  `step` is the
 // row's own log2 decay, dt its step.  Out of line: its registers would push the
 // common path's out.
-__device__ __noinline__ void diag_by_sums(uint32_t ts, int row, float ai, float step, float dt, uint32_t tile) {
+__device__ __noinline__ void diag_by_sums(uint32_t ts, int row, float ai, float step, float dt, float D,
+                                          uint32_t tile) {
   const int lane = row & 31;
   float most = fabsf(ai) < kFar ? 0.f : 1.f;  // a NaN counts
 #pragma unroll
@@ -305,6 +310,7 @@ __device__ __noinline__ void diag_by_sums(uint32_t ts, int row, float ai, float 
   for (int hf = 1; hf >= 0; --hf) {
     float v[16];
     umma::tmem_ld16(ts + hf * 16, v);
+    uint4 hi[2], lo[2];
 #pragma unroll
     for (int q = 3; q >= 0; --q) {
       const float4 k4 = lds16f(kd_at(tile, row >> 5, hf * 4 + q));
@@ -315,9 +321,19 @@ __device__ __noinline__ void diag_by_sums(uint32_t ts, int row, float ai, float 
         const float next = __shfl_sync(0xffffffffu, step, (j + 1) & 31), dj = __shfl_sync(0xffffffffu, dt, j);
         if (j < lane) sum += next;
         v[i] = j <= lane ? v[i] * (most == 0.f ? f * kk[e] : ex2(sum) * dj) : 0.f;
+        if (j == lane) v[i] += D;
       }
     }
-    umma::tmem_st8(ts + hf * 16, tc::pack8<__nv_bfloat16>(v), tc::pack8<__nv_bfloat16>(v + 8));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      float2 w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = make_float2(v[q * 8 + e * 2], v[q * 8 + e * 2 + 1]);
+      hi[q] = take_part(w);
+      lo[q] = pack8(w);
+    }
+    umma::tmem_st8(ts + p_step(hf, 0), hi[0], hi[1]);
+    umma::tmem_st8(ts + p_step(hf, 1), lo[0], lo[1]);
   }
 }
 
@@ -414,7 +430,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
   if (warp == kLead) {
     // ---- copies and products ----
     constexpr uint32_t id_s = umma::idesc_f16(128, 128, true, false, false);
-    constexpr uint32_t id_y = umma::idesc_f16(128, 64, true, false, true);
+    constexpr uint32_t id_y = umma::idesc_f16(128, 64, true, false, true), id_yi = umma::idesc_f16(128, 128, true, false, true);
     constexpr uint32_t id_h2 = umma::idesc_f16(128, 128, true, true, true), id_h3 = umma::idesc_f16(128, 192, true, true, true);
     // operand descriptors: rows of x and of the parts are tokens (K) with 64
     // columns (N), B is read both ways; a k-step of 16 advances 32 bytes
@@ -422,7 +438,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     const uint64_t d_c = umma::smem_desc_sw128(sbase + M::kC, 16, 1024), d_bk = umma::smem_desc_sw128(sbase + M::kB, 16, 1024);
     const uint64_t d_bm = umma::smem_desc_sw128(sbase + M::kB, kTile, 1024), d_x = umma::smem_desc_sw128(sbase + M::kX, kTile, 1024);
     const uint64_t d_xs = umma::smem_desc_sw128(sbase + M::kXs, kTile, 1024);
-    const uint64_t d_h = umma::smem_desc_sw128(sbase + M::kH, kTile, 1024);
+    const uint64_t d_h = umma::smem_desc_sw128(sbase + M::kHlo, kTile, 1024);  // both parts side by side
     // a chunk's operands in the order in which their places become free: B and
     // C's first tile with the products of the chunk before the last, C's
     // second tile (where z was) and x (where y was) with its outputs
@@ -494,7 +510,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         if (c > 0 || seg || ini)
 #pragma unroll
           for (int ks = 0; ks < S_ / 16; ++ks)
-            umma::mma_f16(tmem + M::kYi, d_c + st + k_step(ks), d_h + mn_step(ks), id_y, ks > 0);
+            umma::mma_f16(tmem + M::kYi, d_c + st + k_step(ks), d_h + mn_step(ks), id_yi, ks > 0);
         umma::mma_commit(bar_yi);
         if (c > 0 && c + 1 < nch) {
           umma::bulk_wait_read_all();
@@ -518,7 +534,10 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         const uint64_t st = (c & 1) * (M::kStage >> 4);
 #pragma unroll
         for (int ks = 0; ks < kL / 16; ++ks)
-          umma::mma_f16_ta(tmem + M::kYa, tmem + p_step(ks), d_x + st + mn_step(ks), id_y, ks > 0);
+          umma::mma_f16_ta(tmem + M::kYa, tmem + p_step(ks, 0), d_x + st + mn_step(ks), id_y, ks > 0);
+#pragma unroll
+        for (int ks = 0; ks < kL / 16; ++ks)  // the parts in turns, step by step, took 19 us longer over 32 chunks
+          umma::mma_f16_ta(tmem + M::kYa, tmem + p_step(ks, 1), d_x + st + mn_step(ks), id_y, 1);
         umma::mma_commit(bar_y);
         // The parts of w x side by side: one product reads B once for all.
         // With S = 64 rows 64-127 of the accumulators are the product of the
@@ -589,8 +608,12 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
     }
     auto store_h = [&]() {
       if (row < S_) {
-        sts16(sbase + M::kH + piece.at[0], pack8(hr));
-        sts16(sbase + M::kH + piece.at[1], pack8(hr + 4));
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float2 v[4] = {hr[q * 4], hr[q * 4 + 1], hr[q * 4 + 2], hr[q * 4 + 3]};
+          sts16(sbase + M::kH + piece.at[q], take_part(v));
+          sts16(sbase + M::kHlo + piece.at[q], pack8(v));
+        }
       }
     };
     store_h();
@@ -622,7 +645,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {  // 16 columns at a time: registers
             float v[16];
-            uint4 u[2];
+            uint4 hi[2], lo[2];
             umma::tmem_ld16(ts + hf * 16, v);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -637,25 +660,28 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
                 const float2 k2 = make_float2(__uint_as_float(kk[e * 2]), __uint_as_float(kk[e * 2 + 1]));
                 w[e] = __fmul2_rn(make_float2(v[q * 8 + e * 2], v[q * 8 + e * 2 + 1]), __fmul2_rn(f2, k2));
                 if (diag) {
-                  if (j > lane) w[e].x = 0.f;
-                  if (j + 1 > lane) w[e].y = 0.f;
+                  w[e].x = j < lane ? w[e].x : j == lane ? w[e].x + D : 0.f;
+                  w[e].y = j + 1 < lane ? w[e].y : j + 1 == lane ? w[e].y + D : 0.f;
                 }
               }
-              u[q] = pack8(w);
+              hi[q] = take_part(w);
+              lo[q] = pack8(w);
             }
-            umma::tmem_st8(ts + hf * 16, u[0], u[1]);  // over scores that have been read
+            umma::tmem_st8(ts + p_step(hf, 0), hi[0], hi[1]);  // over scores that have been read
+            umma::tmem_st8(ts + p_step(hf, 1), lo[0], lo[1]);
           }
         } else {
-          diag_by_sums(ts, row, ai, dt * (p.A[h] * tc::kLog2e), dt, sbase + M::kXs);
+          diag_by_sums(ts, row, ai, dt * (p.A[h] * tc::kLog2e), dt, D, sbase + M::kXs);
         }
       } else {
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        umma::tmem_st8(ts, zero, zero);
-        umma::tmem_st8(ts + 16, zero, zero);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) umma::tmem_st8(ts + q * 8, zero, zero);
       }
       // ---- w x in parts (x has been there since the scores were issued) ----
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
       uint32_t not_finite = 0;
+      if (want_state && !wait(bar_yi, c & 1, kSiteScanScores)) break;  // the third part takes the place of h's second
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         uint4 u = lds16(st + M::kX + piece.at[q]);
@@ -694,18 +720,18 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
       if (!wait(bar_yi, c & 1, kSiteScanScores)) break;
       umma::fence_after_sync();
       {
-        const float2 g2 = make_float2(g1, g1), D2 = make_float2(D, D);
-        const bool has_yi = c > 0 || seg || ini;
+        const float2 g2 = make_float2(g1, g1);
+        if (c > 0 || seg || ini) {
+          float lo[16], hi[16];
+          umma::tmem_ld16x2(tl + M::kYi + cq * 16, tl + M::kYi + 64 + cq * 16, lo, hi);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          unpack8(lds16(st + M::kX + piece.at[q]), part_y + q * 4);
-          float yi[8];
-          if (has_yi) umma::tmem_ld8(tl + M::kYi + cq * 16 + q * 8, yi);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            part_y[q * 4 + e] = __fmul2_rn(D2, part_y[q * 4 + e]);
-            if (has_yi) part_y[q * 4 + e] = __ffma2_rn(g2, make_float2(yi[e * 2], yi[e * 2 + 1]), part_y[q * 4 + e]);
+          for (int e = 0; e < 8; ++e) {
+            const float2 yi = __fadd2_rn(make_float2(hi[e * 2], hi[e * 2 + 1]), make_float2(lo[e * 2], lo[e * 2 + 1]));
+            part_y[e] = __fmul2_rn(g2, yi);
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) part_y[e] = make_float2(0.f, 0.f);
         }
       }
       if (p.z) {

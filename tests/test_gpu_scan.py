@@ -464,3 +464,20 @@ def test_slow_decays_behind_a_fast_one(lens, every, S):
     y, h = run(i, lens)
     assert rel(h, rh) <= 64 * F32
     assert rel(y, ry) <= tolerances(bf16, True)
+
+
+@pytest.mark.parametrize("lens,S,init,final", [([300], 128, True, True), ([300], 128, True, False), ([200, 129], 64, False, True),
+                                               ([1400], 128, False, False)])
+def test_outputs_are_rounded_once(lens, S, init, final):
+    """The scores and the state go into the products as two bf16 parts (16
+    bits): an output's error before its own rounding is about 2^-17 of its
+    terms, and they are some four times the output where terms cancel, so one
+    in 2^-8 / (2 * 4 * 2^-17) = 64 outputs may round the other way; operands of
+    one part (2^-9) would turn a third of them."""
+    i = make(sum(lens), 2, 64, 1, S, bf16, False, seed=19)
+    h0 = torch.randn(len(lens), 2, 64, S, generator=torch.Generator().manual_seed(20)) if init else None
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], None, i["dt_bias"], True, (0.0, float("inf")),
+                      h0, lens)
+    y, h = run(i, lens, h0, final=final)
+    assert (y.cpu() != ry.to(bf16)).double().mean() <= 1 / 64
+    assert h is None or rel(h, rh) <= 64 * F32
