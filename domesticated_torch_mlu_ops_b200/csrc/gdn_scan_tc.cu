@@ -135,6 +135,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void unpack8(uint4 u, float2* v) {
   v[0] = conv::unpack2<__nv_bfloat16>(u.x);
   v[1] = conv::unpack2<__nv_bfloat16>(u.y);
@@ -335,6 +341,13 @@ __device__ __noinline__ void diag_by_sums(uint32_t ts, int row, float ai, float 
     umma::tmem_st8(ts + p_step(hf, 0), hi[0], hi[1]);
     umma::tmem_st8(ts + p_step(hf, 1), lo[0], lo[1]);
   }
+}
+
+// z / (1 + exp(-z)) of two values, to a few fp32 ulp.
+__device__ __forceinline__ float2 silu2(float2 z) {
+  const float2 t = __fmul2_rn(z, make_float2(-tc::kLog2e, -tc::kLog2e));
+  const float2 u = __fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.f, 1.f));
+  return __fmul2_rn(z, make_float2(rcp(u.x), rcp(u.y)));
 }
 
 // Non-zero when one of two bf16 values is infinite or NaN.
@@ -740,11 +753,7 @@ scan_tc_kernel(const ScanParams p, const PrepOut prep, const int slices, const _
         for (int q = 0; q < 2; ++q) {
           unpack8(lds16(st + M::kZ + piece.at[q]), gz + q * 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float zz[2] = {gz[q * 4 + e].x, gz[q * 4 + e].y};
-            conv::silu_vec<__nv_bfloat16, 2>(zz);
-            gz[q * 4 + e] = make_float2(zz[0], zz[1]);
-          }
+          for (int e = 0; e < 4; ++e) gz[q * 4 + e] = silu2(gz[q * 4 + e]);
         }
       }
       if (!wait(bar_y, c & 1, kSiteScanOut)) break;

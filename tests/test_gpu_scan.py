@@ -481,3 +481,22 @@ def test_outputs_are_rounded_once(lens, S, init, final):
     y, h = run(i, lens, h0, final=final)
     assert (y.cpu() != ry.to(bf16)).double().mean() <= 1 / 64
     assert h is None or rel(h, rh) <= 64 * F32
+
+
+def test_gate_is_not_rounded():
+    """One token, B = 0, D = 1: y = x silu(z) in fp32 (a few ulp of 2^-24),
+    rounded once, for z over the whole range; at most one output in
+    2^-8 / (2 * 16 * 2^-24) = 2^11 may round the other way, which is none or a
+    few of these 8192; tanh.approx (2^-11) would turn one in twenty."""
+    g = torch.Generator().manual_seed(21)
+    n = 64
+    x = torch.randn(n, 2, 64, generator=g).to(bf16)
+    z = (torch.randn(n, 2, 64, generator=g) * 4).to(bf16)
+    zero = torch.zeros(n, 1, 128, dtype=bf16)
+    i = dict(x=x, dt=torch.zeros(n, 2, dtype=bf16), A=-torch.ones(2), B=zero, C=zero, D=torch.ones(2), z=z,
+             dt_bias=torch.zeros(2))
+    y, _ = run(i, [n])
+    want = x.double() * z.double() * torch.sigmoid(z.double())
+    assert (y.cpu() != want.to(bf16)).sum() <= 8
+    y, _ = run({**i, "z": torch.full_like(z, -200.0)}, [n])
+    assert torch.count_nonzero(y) == 0
