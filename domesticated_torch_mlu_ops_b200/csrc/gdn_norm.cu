@@ -48,7 +48,7 @@ struct Params {
   float* partial;  // [gridDim.x][D]
   int64_t D;
   int64_t sx_tok, sx_head, sz_tok, sz_head;  // row (t, h) of x and z, in elements
-  int rows, heads;
+  unsigned rows, heads;
   int group;
   int w_dtype, res_f32, gate_before, sigmoid_gate;
   float eps, alpha, w_off;
@@ -129,13 +129,15 @@ struct Team {
   __device__ __forceinline__ int at(int k) const { return in(k) ? col(k) : 0; }
 };
 
-__device__ __forceinline__ void row_of(const Params& p, int row, int64_t& x_at, int64_t& z_at) {
+// Rows are counted without sign: up to 2^31 - 1 of them, a step behind the last
+// still fits.
+__device__ __forceinline__ void row_of(const Params& p, unsigned row, int64_t& x_at, int64_t& z_at) {
   if (p.heads == 1) {
     x_at = row * p.sx_tok;
     z_at = row * p.sz_tok;
   } else {
-    const unsigned t = static_cast<unsigned>(row) / static_cast<unsigned>(p.heads);
-    const int64_t h = row - static_cast<int>(t * p.heads);
+    const unsigned t = row / p.heads;
+    const int64_t h = row - t * p.heads;
     x_at = t * p.sx_tok + h * p.sx_head;
     z_at = t * p.sz_tok + h * p.sz_head;
   }
@@ -154,13 +156,13 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const Params p) {
   const Team<VEC, ITER, TS> tm(p.group);
   const int64_t g0 = static_cast<int64_t>(blockIdx.y) * p.group;
   const float inv = 1.f / static_cast<float>(p.group);
-  const int step = gridDim.x * tm.teams;
+  const unsigned step = gridDim.x * tm.teams;
   V w[ITER];
 #pragma unroll
   for (int k = 0; k < ITER; ++k) w[k] = ld_weight<VEC>(p, g0 + tm.at(k));
   pk::Raw<T, VEC> rx[ITER], rz[ITER];
   pk::Raw<RT, VEC> rr[ITER];
-  auto load = [&](int row) {
+  auto load = [&](unsigned row) {
     int64_t xa, za;
     row_of(p, min(row, p.rows - 1), xa, za);
     const int64_t at = static_cast<int64_t>(min(row, p.rows - 1)) * p.D + g0;
@@ -171,11 +173,12 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const Params p) {
       if constexpr (kRes) pk::load(rr[k], static_cast<const RT*>(p.residual) + at + tm.at(k));
     }
   };
-  int row0 = blockIdx.x * tm.teams, par = 0;
+  unsigned row0 = blockIdx.x * tm.teams;
+  int par = 0;
   if (kAhead && row0 < p.rows) load(row0 + tm.team);
   // the CTA's teams walk together (shuffles and barriers are for all of them)
   for (; row0 < p.rows; row0 += step) {
-    const int row = row0 + tm.team;
+    const unsigned row = row0 + tm.team;
     if (!kAhead) load(row);
     V u[ITER], a[ITER];
 #pragma unroll
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const Params p) {
   const Team<VEC, ITER, TS> tm(p.group);
   const int64_t g0 = static_cast<int64_t>(blockIdx.y) * p.group;
   const float inv = 1.f / static_cast<float>(p.group);
-  const int step = gridDim.x * tm.teams;
+  const unsigned step = gridDim.x * tm.teams;
   constexpr bool kAhead = MAXT <= 256;  // larger CTAs have no registers for the next row
   V w[ITER], dw[ITER];
 #pragma unroll
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const Params p) {
   }
   pk::Raw<X, VEC> nx[ITER], rs[ITER];
   pk::Raw<T, VEC> nd[ITER], nz[ITER];
-  auto load = [&](int row) {
+  auto load = [&](unsigned row) {
     int64_t xa, za;
     row_of(p, min(row, p.rows - 1), xa, za);
     const int64_t at = static_cast<int64_t>(min(row, p.rows - 1)) * p.D + g0;
@@ -242,10 +245,11 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const Params p) {
       if (p.z) pk::load(nz[k], static_cast<const T*>(p.z) + za + g0 + tm.at(k));
     }
   };
-  int row0 = blockIdx.x * tm.teams, par = 0;
+  unsigned row0 = blockIdx.x * tm.teams;
+  int par = 0;
   if (kAhead && row0 < p.rows) load(row0 + tm.team);
   for (; row0 < p.rows; row0 += step) {
-    const int row = row0 + tm.team;
+    const unsigned row = row0 + tm.team;
     if (!kAhead) load(row);
     const bool live = row < p.rows;
     const int64_t at = static_cast<int64_t>(row) * p.D + g0;
@@ -441,7 +445,7 @@ Params params(const gdn_norm_args& a) {
   p.x = a.x; p.z = a.z; p.residual = a.residual; p.weight = a.weight; p.y = a.y; p.sum = a.sum;
   p.dy = a.dy; p.dsum = a.dsum; p.dx = a.dx; p.dz = a.dz; p.dresidual = a.dresidual;
   p.partial = static_cast<float*>(a.workspace);
-  p.rows = static_cast<int>(a.rows); p.heads = static_cast<int>(a.heads); p.D = a.D;
+  p.rows = static_cast<unsigned>(a.rows); p.heads = static_cast<unsigned>(a.heads); p.D = a.D;
   p.sx_tok = a.stride_x_token; p.sx_head = a.stride_x_head; p.sz_tok = a.stride_z_token; p.sz_head = a.stride_z_head;
   p.group = a.group; p.w_dtype = a.w_dtype; p.res_f32 = a.res_dtype == GDN_F32;
   p.gate_before = a.z && a.gate_before; p.sigmoid_gate = a.activation == GDN_GATE_SIGMOID;

@@ -212,3 +212,25 @@ def test_refusals():
         ops.gated_rms_norm(torch.randn(1, 17000, device="cuda"), torch.rand(17000, device="cuda"))
     with pytest.raises(ValueError, match="has_residual"):
         ops.gated_rms_norm_bwd(x, x, w, None, x)
+
+
+def test_most_rows():
+    """2^31 - 1 rows of one value: no row index overflows behind the last.  In
+    fp32 y = x w / sqrt(x^2 + eps) and dx = dy w eps / (x^2 + eps)^(3/2); the
+    forms below take the same few fp32 roundings, then one to bf16, so they
+    may differ by one unit in the last place.  A thread adds up to 2^20 terms
+    of dweight: about 2^10 2^-24 of error, 2^-10 allowed."""
+    n, eps = 2 ** 31 - 1, 1.0
+    x = torch.empty(n, 1, dtype=bf16, device="cuda").normal_()
+    w = torch.full((1,), 1.5, device="cuda")
+    y = ops.gated_rms_norm(x, w, eps=eps)
+    dx, dw, _, _ = ops.gated_rms_norm_bwd(x, x, w, eps=eps)
+    total, at = 0.0, 0
+    while at < n:
+        v = x[at:at + 2 ** 28].float()
+        r = torch.rsqrt(v * v + eps)
+        for got, want in ((y, v * r * 1.5), (dx, v * 1.5 * r * eps * r * r)):
+            assert ((got[at:at + 2 ** 28].float() - want).abs() <= 2 ** -7 * want.abs()).all()
+        total += (v * v * r).double().sum().item()
+        at += 2 ** 28
+    assert abs(dw.item() - total) <= 2 ** -10 * total
