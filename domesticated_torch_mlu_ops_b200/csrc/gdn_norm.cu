@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const Params p) {
     for (int k = 0; k < ITER; ++k) {
       pk::load(rx[k], static_cast<const T*>(p.x) + xa + g0 + tm.at(k));
       if (p.z) pk::load(rz[k], static_cast<const T*>(p.z) + za + g0 + tm.at(k));
-      if constexpr (kRes) pk::load(rr[k], static_cast<const RT*>(p.residual) + at + tm.at(k));
+      if constexpr (kRes) pk::load_rw(rr[k], static_cast<const RT*>(p.residual) + at + tm.at(k));  // may be the sum
     }
   };
   unsigned row0 = blockIdx.x * tm.teams;

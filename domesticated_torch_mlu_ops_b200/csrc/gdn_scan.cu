@@ -222,15 +222,6 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
   if (!OUT && row == 0 && lane == 0) p.seg_decay[id * p.H + h] = logd;
 }
 
-// Loads that stay before the stores that follow them: the kernel below
-// overwrites what it has read, so they are not of the read-only kind.
-__device__ __forceinline__ void load_state(pk::Raw<float, 4>& v, const float* p) {
-  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.a.x), "=r"(v.a.y), "=r"(v.a.z), "=r"(v.a.w) : "l"(p) : "memory");
-}
-__device__ __forceinline__ void load_state(pk::Raw<float, 1>& v, const float* p) {
-  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v.a) : "l"(p) : "memory");
-}
-
 // States between segments: for each sequence, head and state element, in
 // order of its segments, the state that the segment starts from (in place of
 // its first piece's) and h <- exp(log decay) h + state over its pieces.  A
@@ -284,7 +275,7 @@ __global__ void __launch_bounds__(256) scan_pass_kernel(const ScanParams p) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (j < now) {
-        load_state(v[j], st + j * step);
+        pk::load_rw(v[j], st + j * step);  // overwritten below
         d[j] = ld[j * p.H];
       }
 #pragma unroll

@@ -123,12 +123,31 @@ __device__ __forceinline__ void ldg_now(uint32_t& v, const void* p) {
 __device__ __forceinline__ void ldg_now(uint16_t& v, const void* p) {
   asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(v) : "l"(p));
 }
+// The same from memory that the kernel may write later: ordinary loads, which
+// stay before the stores that follow them.
+__device__ __forceinline__ void ld_now(uint4& v, const void* p) {
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void ld_now(uint2& v, const void* p) {
+  asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void ld_now(uint32_t& v, const void* p) {
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void ld_now(uint16_t& v, const void* p) {
+  asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+}
 template <typename T, int VEC>
 using Raw = Bits<VEC * sizeof(T)>;
 template <int BYTES>
 __device__ __forceinline__ void load(Bits<BYTES>& v, const void* p) {
   ldg_now(v.a, p);
   if constexpr (BYTES == 32) ldg_now(v.b, static_cast<const char*>(p) + 16);
+}
+template <int BYTES>
+__device__ __forceinline__ void load_rw(Bits<BYTES>& v, const void* p) {
+  ld_now(v.a, p);
+  if constexpr (BYTES == 32) ld_now(v.b, static_cast<const char*>(p) + 16);
 }
 
 template <typename T, int VEC>

@@ -197,3 +197,19 @@ def test_loads_of_tensor_memory_are_fenced_behind_their_wait():
         assert "tcgen05.wait" not in h and h.count("tmem_wait_ld();") == 1, name
         behind = h.split("tmem_wait_ld();")[1]
         assert sum(int(n) for n in re.findall(r"reg_fence(\d+)\(", behind)) == loaded, name
+
+
+def _kernel_source(file, name):
+    src = open(os.path.join(os.path.dirname(HEADER), "..", "domesticated_torch_mlu_ops_b200", "csrc", file)).read()
+    at = src.index(f" {name}(")
+    return src[at:src.index("\n}\n", at)]
+
+
+@pytest.mark.parametrize("file,kernel,array", [("gdn_norm.cu", "norm_fwd_kernel", "p.residual"),
+                                               ("gdn_scan.cu", "scan_pass_kernel", "st + j * step")])
+def test_memory_that_a_kernel_writes_is_not_read_as_read_only(file, kernel, array):
+    """The norm's sum may be its residual, a state is replaced in place: loads
+    of the read-only kind promise that the memory does not change."""
+    body = _kernel_source(file, kernel)
+    loads = [line for line in body.splitlines() if array in line and "load" in line]
+    assert loads and all("load_rw(" in line for line in loads)

@@ -234,3 +234,18 @@ def test_most_rows():
         total += (v * v * r).double().sum().item()
         at += 2 ** 28
     assert abs(dw.item() - total) <= 2 ** -10 * total
+
+
+@pytest.mark.parametrize("dtype,rd,D", [(bf16, f32, 2048), (bf16, bf16, 64), (f32, f32, 77)])
+def test_sum_in_the_residual_s_place(dtype, rd, D):
+    """The C entry may be given one buffer as residual and sum."""
+    from domesticated_torch_mlu_ops_b200 import _lib
+    from domesticated_torch_mlu_ops_b200.gdn import _DT, _launch
+    x, w, _, res, _, _ = make((4001, D), dtype, f32, False, rd, seed=5)
+    x, w, res = x.cuda(), w.cuda(), res.cuda()
+    y, total = ops.gated_rms_norm(x, w, residual=res)
+    again = torch.empty_like(y)
+    _launch(_lib.load().gdn_norm_fwd, _lib.pack_norm(
+        x.data_ptr(), 0, res.data_ptr(), w.data_ptr(), again.data_ptr(), res.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 4001, 1, D,
+        D, D, 0, 0, D, _DT[dtype], _DT[dtype], _DT[rd], _DT[f32], 0, 0, _lib.GDN_GATE_SILU, 1e-6, 1.0), x.device)
+    assert torch.equal(again, y) and torch.equal(res, total)
