@@ -308,11 +308,13 @@ struct UpdateParams {
 // The state line of (token, head) is read and written once; nothing else is
 // of its size, so HBM bounds the kernel.  LPR lanes hold one row of S (VEC
 // columns each, ITER times); a warp moves R rows at a time, all of whose
-// loads are in flight together.
+// loads are in flight together.  256 tokens on fp32 lines of 64 heads x 64 x
+// 128 (1.08 GB): 169 us with 32-byte accesses, 98 % of a plain copy's rate.
 template <typename T, typename CT, int VEC, int LPR, int ITER, int R>
 __global__ void __launch_bounds__(kUpdWarps * 32) scan_update_kernel(const UpdateParams p) {
   constexpr int RW = 32 / LPR;  // rows side by side in a warp
   constexpr int BLK = kUpdWarps * RW * R;
+  constexpr bool kWide = VEC * sizeof(CT) == 32;
   const int64_t n = blockIdx.z;
   const int h = blockIdx.y, g = h / (p.H / p.G);
   const int lane = threadIdx.x % LPR, sub = (threadIdx.x & 31) / LPR, warp = threadIdx.x >> 5;
@@ -327,16 +329,16 @@ __global__ void __launch_bounds__(kUpdWarps * 32) scan_update_kernel(const Updat
     return;
   }
   CT* st = static_cast<CT*>(p.state) + slot * p.s_slot + static_cast<int64_t>(h) * p.P * p.S;
-  float v[R][ITER][VEC];
+  pk::Raw<CT, VEC> raw[R][ITER];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
       const int row = row0 + r * RW, s = (k * LPR + lane) * VEC;
-      if (row < p.P && s < p.S) conv::ldv<CT, VEC>(st + static_cast<int64_t>(row) * p.S + s, v[r][k]);
-      else
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[r][k][e] = 0.f;
+      const CT* from = st + static_cast<int64_t>(row) * p.S + s;  // replaced below: no load of the read-only kind
+      if (row >= p.P || s >= p.S) raw[r][k] = {};
+      else if constexpr (kWide) pk::load_rw_wide(raw[r][k], from);
+      else pk::load_rw(raw[r][k], from);
     }
   const float dt = step_of(ld_any(p.dt, p.dt_dtype, n * p.sdt + h), p.dt_bias ? p.dt_bias[h] : 0.f, p.softplus,
                            p.dt_lo, p.dt_hi);
@@ -362,12 +364,18 @@ __global__ void __launch_bounds__(kUpdWarps * 32) scan_update_kernel(const Updat
 #pragma unroll
     for (int k = 0; k < ITER; ++k) {
       const int s = (k * LPR + lane) * VEC;
+      pk::Vec<VEC> h = pk::widen<CT, VEC>(raw[r][k]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        v[r][k][e] = fmaf(decay, v[r][k][e], u * bv[k][e]);
-        acc = fmaf(v[r][k][e], cv[k][e], acc);
+        const float v = fmaf(decay, pk::get(h, e), u * bv[k][e]);
+        acc = fmaf(v, cv[k][e], acc);
+        pk::set(h, e, v);
       }
-      if (row < p.P && s < p.S) conv::stv<CT, VEC>(st + static_cast<int64_t>(row) * p.S + s, v[r][k]);
+      if (row < p.P && s < p.S) {
+        CT* to = st + static_cast<int64_t>(row) * p.S + s;
+        if constexpr (kWide) pk::store_wide(to, reinterpret_cast<const pk::Bits<32>&>(h));
+        else pk::store<CT, VEC>(to, h);
+      }
     }
     acc = group_sum<LPR>(acc);
     if (lane == r % LPR) {
@@ -510,14 +518,27 @@ void launch_rows(const UpdateParams& p, cudaStream_t s) {
   else launch_upd<T, CT, VEC, LPR, 1, 4>(p, s);
 }
 
-// Lanes per row: S in 16-byte vectors where the rows allow them, else single
-// columns; four rows per warp in flight (256 tokens on fp32 lines of 64 heads
-// x 64 x 128: 177 us, against 187 with eight rows, 212 with 16 and 262 with two).
+// Lanes per row: S in 32-byte vectors of fp32 lines, or 16-byte ones, where
+// the rows allow them, else single columns; four rows per warp and lane in
+// flight (256 tokens on fp32 lines of 64 heads x 64 x 128: 169 us; 213 with two
+// rows, 192 to 195 with 16-byte vectors and four or eight rows).
 template <typename T, typename CT>
 void update_t(const UpdateParams& p, cudaStream_t s) {
   constexpr int V = 16 / sizeof(CT);
-  const bool vec = p.S % V == 0 && p.s_slot % V == 0 && (reinterpret_cast<uintptr_t>(p.state) & 15) == 0;
-  if (vec) {
+  auto fits = [&](int v) {
+    return p.S % v == 0 && p.s_slot % v == 0 && (reinterpret_cast<uintptr_t>(p.state) & (v * sizeof(CT) - 1)) == 0;
+  };
+  if constexpr (sizeof(CT) == 4) {
+    if (fits(8)) {
+      const int n = p.S / 8;
+      if (n <= 4) launch_upd<T, CT, 8, 4, 1, 4>(p, s);
+      else if (n <= 8) launch_rows<T, CT, 8, 8>(p, s);
+      else if (n <= 16) launch_rows<T, CT, 8, 16>(p, s);
+      else launch_upd<T, CT, 8, 32, 1, 4>(p, s);
+      return;
+    }
+  }
+  if (fits(V)) {
     const int n = p.S / V;
     if (n <= 4) launch_upd<T, CT, V, 4, 1, 4>(p, s);
     else if (n <= 8) launch_rows<T, CT, V, 8>(p, s);

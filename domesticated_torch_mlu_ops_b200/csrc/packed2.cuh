@@ -150,6 +150,18 @@ __device__ __forceinline__ void load_rw(Bits<BYTES>& v, const void* p) {
   if constexpr (BYTES == 32) ld_now(v.b, static_cast<const char*>(p) + 16);
 }
 
+// 32 bytes in one access, where the address is a multiple of 32.
+__device__ __forceinline__ void load_rw_wide(Bits<32>& v, const void* p) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v.a.x), "=r"(v.a.y), "=r"(v.a.z), "=r"(v.a.w), "=r"(v.b.x), "=r"(v.b.y), "=r"(v.b.z), "=r"(v.b.w)
+               : "l"(p) : "memory");
+}
+__device__ __forceinline__ void store_wide(void* p, const Bits<32>& v) {
+  asm volatile("st.global.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+               :: "r"(v.a.x), "r"(v.a.y), "r"(v.a.z), "r"(v.a.w), "r"(v.b.x), "r"(v.b.y), "r"(v.b.z), "r"(v.b.w), "l"(p)
+               : "memory");
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ Vec<VEC> widen(const Raw<T, VEC>& v) {
   Vec<VEC> r;

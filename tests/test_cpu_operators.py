@@ -206,10 +206,11 @@ def _kernel_source(file, name):
 
 
 @pytest.mark.parametrize("file,kernel,array", [("gdn_norm.cu", "norm_fwd_kernel", "p.residual"),
-                                               ("gdn_scan.cu", "scan_pass_kernel", "st + j * step")])
+                                               ("gdn_scan.cu", "scan_pass_kernel", "st + j * step"),
+                                               ("gdn_scan.cu", "scan_update_kernel", ", from)")])
 def test_memory_that_a_kernel_writes_is_not_read_as_read_only(file, kernel, array):
     """The norm's sum may be its residual, a state is replaced in place: loads
     of the read-only kind promise that the memory does not change."""
     body = _kernel_source(file, kernel)
-    loads = [line for line in body.splitlines() if array in line and "load" in line]
-    assert loads and all("load_rw(" in line for line in loads)
+    loads = [line for line in body.splitlines() if array in line and ("load" in line or "ldv" in line)]
+    assert loads and all("load_rw" in line for line in loads)

@@ -500,3 +500,23 @@ def test_gate_is_not_rounded():
     assert (y.cpu() != want.to(bf16)).sum() <= 8
     y, _ = run({**i, "z": torch.full_like(z, -200.0)}, [n])
     assert torch.count_nonzero(y) == 0
+
+
+@pytest.mark.parametrize("S", [8, 32, 36, 64, 100, 128, 256])
+@pytest.mark.parametrize("offset", [0, 4])
+def test_update_of_fp32_lines_at_every_width(S, offset):
+    """Lines that begin on 32 bytes or on 16, of widths that fill lanes or not."""
+    i = make(3, 2, 37, 1, S, bf16, True, seed=22)
+    lines = torch.randn(4, 2, 37, S, generator=torch.Generator().manual_seed(23))
+    flat = torch.zeros(lines.numel() + offset, device="cuda")
+    flat[offset:] = lines.flatten().cuda()
+    cache = flat[offset:].view(lines.shape)
+    dt = steps(i["dt"].double(), i["dt_bias"].double(), True, (0.0, float("inf")))
+    c = cuda(i)
+    y, _ = ops.selective_scan_update(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"],
+                                     dt_softplus=True, state=cache, ssm_state_indices=torch.tensor([3, 0, 2]).cuda())
+    for n, slot in enumerate((3, 0, 2)):
+        h, want = ref_token(lines[slot].double(), i["x"][n].double(), dt[n], i["A"].double(), i["B"][n].double(),
+                            i["C"][n].double(), i["D"].double(), i["z"][n].double())
+        assert rel(cache[slot], h) <= 64 * F32 and rel(y[n], want) <= U[bf16] + 64 * F32
+    assert torch.equal(cache[1].cpu(), lines[1])
