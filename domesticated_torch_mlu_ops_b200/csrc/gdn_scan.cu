@@ -579,7 +579,13 @@ extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
   const Plan pl = plan(*a);
   if (!a->workspace || a->workspace_bytes < pl.bytes)
     return set_last_error(GDN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", a->workspace_bytes, pl.bytes);
-  if (a->N == 0) return GDN_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (a->N == 0) {  // no kernel clears the error word
+    e = cudaMemsetAsync(a->workspace, 0, 4 * sizeof(int32_t), s);
+    if (e != cudaSuccess) return set_last_error(GDN_ERR_CUDA, "gdn_scan_fwd: %s", cudaGetErrorString(e));
+    return GDN_OK;
+  }
   ScanParams p{};
   p.x = a->x; p.dt = a->dt; p.b = a->b; p.c = a->c; p.z = a->z; p.A = a->A; p.D = a->D; p.dt_bias = a->dt_bias;
   p.init = a->initial_state; p.y = a->y; p.final_state = a->final_state; p.cu = a->cu_seqlens;
@@ -595,8 +601,6 @@ extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
   p.H = a->H; p.P = a->P; p.G = a->G; p.S = a->S;
   p.dt_dtype = a->dt_dtype; p.init_dtype = a->init_dtype; p.final_dtype = a->final_dtype; p.cu_dtype = a->cu_dtype;
   p.softplus = a->dt_softplus; p.dt_lo = a->dt_min; p.dt_hi = a->dt_max;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaSuccess;
   if (total > 0 && tc_shape(*a) && tc_layout(*a)) e = launch_tc(p, *a, reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.scratch_off), s);
   else if (a->dtype == GDN_F32) launch_t<float>(p, pl, s);
   else if (a->dtype == GDN_BF16) launch_t<__nv_bfloat16>(p, pl, s);

@@ -520,3 +520,20 @@ def test_update_of_fp32_lines_at_every_width(S, offset):
                             i["C"][n].double(), i["D"].double(), i["z"][n].double())
         assert rel(cache[slot], h) <= 64 * F32 and rel(y[n], want) <= U[bf16] + 64 * F32
     assert torch.equal(cache[1].cpu(), lines[1])
+
+
+def poison(*shape, dtype):
+    """Fills memory that the allocator hands out next."""
+    t = torch.full(shape, 99 if dtype is torch.uint8 else float("nan"), dtype=dtype, device="cuda")
+    torch.cuda.synchronize()
+    del t
+
+
+def test_empty_batches_have_no_errors():
+    e = lambda *s: torch.empty(*s, device="cuda", dtype=bf16)  # noqa: E731
+    A = -torch.ones(2, device="cuda")
+    for _ in range(3):
+        poison(256, dtype=torch.uint8)
+        y, h = ops.chunk_selective_scan(e(0, 5, 2, 64), e(0, 5, 2), A, e(0, 5, 1, 128), e(0, 5, 1, 128),
+                                        output_final_state=True, check_errors=True)
+        assert y.shape == (0, 5, 2, 64) and h.shape == (0, 2, 64, 128)
