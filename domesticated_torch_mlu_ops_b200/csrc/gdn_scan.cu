@@ -55,6 +55,7 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
   const int h = blockIdx.y, g = h / (p.H / p.G);
   const int row0 = blockIdx.z * ROWS;
   clear_error(p);
+  if (OUT) zero_outside(p, sizeof(T));
   if (threadIdx.x < 32) {
     int64_t n = 0, ls = 0, t0 = 0, t1 = 0;
     bool last = false;
@@ -581,8 +582,10 @@ extern "C" GDN_API int gdn_scan_fwd(const gdn_scan_args* a, void* stream) {
     return set_last_error(GDN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", a->workspace_bytes, pl.bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (a->N == 0) {  // no kernel clears the error word
+  if (a->N == 0) {  // no kernel: the error word, and the outputs of tokens without a sequence
     e = cudaMemsetAsync(a->workspace, 0, 4 * sizeof(int32_t), s);
+    if (e == cudaSuccess && total > 0)
+      e = cudaMemsetAsync(a->y, 0, static_cast<size_t>(total) * a->H * a->P * (a->dtype == GDN_F32 ? 4 : 2), s);
     if (e != cudaSuccess) return set_last_error(GDN_ERR_CUDA, "gdn_scan_fwd: %s", cudaGetErrorString(e));
     return GDN_OK;
   }

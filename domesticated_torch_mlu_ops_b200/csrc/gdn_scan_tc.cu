@@ -169,6 +169,7 @@ constexpr int kPrepHeads = 16;
 __global__ void __launch_bounds__(kPrepHeads * 32) scan_prep_kernel(const ScanParams p, const PrepOut o) {
   __shared__ float raw[kL][kPrepHeads + 1];
   clear_error(p);
+  zero_outside(p, 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = blockIdx.y * kPrepHeads;
   int64_t n, ls, t0, t1;
   bool last;

@@ -69,6 +69,25 @@ __device__ __forceinline__ void clear_error(const ScanParams& p) {
   if (p.clear_err && threadIdx.x < 4 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) p.err[threadIdx.x] = 0;
 }
 
+// Outputs of tokens outside every sequence (before the first, behind the last)
+// are zero: by all blocks (x, 0, 0) of a kernel, bytes in all.
+__device__ __forceinline__ void zero_outside(const ScanParams& p, int esize) {
+  if (!p.cu || blockIdx.y || blockIdx.z) return;
+  const int64_t first = min64(max(load_index(p.cu, p.cu_dtype, 0), static_cast<int64_t>(0)), p.total);
+  const int64_t end = min64(max(load_index(p.cu, p.cu_dtype, p.N), first), p.total), outside = first + p.total - end;
+  if (outside == 0) return;
+  char* y = static_cast<char*>(p.y);
+  const int64_t row = static_cast<int64_t>(p.H) * p.P * esize;
+  const int unit = row % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0 ? 16 : 2;
+  const int64_t head = first * row, gap = (end - first) * row;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * unit; i < outside * row;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x * unit) {
+    char* at = y + (i < head ? i : i + gap);
+    if (unit == 16) *reinterpret_cast<uint4*>(at) = make_uint4(0u, 0u, 0u, 0u);
+    else *reinterpret_cast<uint16_t*>(at) = 0;
+  }
+}
+
 // Segment `id` of the batch: segment `ls` of sequence n, tokens [t0, t1);
 // `last` when it is the sequence's last.  An empty sequence has one empty
 // segment.  `chunk0` is the segment's first 128-token chunk, counted over the

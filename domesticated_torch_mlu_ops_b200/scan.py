@@ -206,8 +206,9 @@ def chunk_selective_scan(
     x, z ``[B, T, H, P]``; dt ``[B, T, H]``; B, C ``[B, T, G, S]`` (head h uses
     group ``h // (H // G)``); A, D, dt_bias ``[H]``; initial_state
     ``[N, H, P, S]`` of any float type; with ``cu_seqlens [N + 1]`` the batch
-    size is 1 and the tokens are N packed sequences.  Token rows may be strided
-    (views of one projection).  ``dt_limit`` clamps the steps after softplus.
+    size is 1 and the tokens are N packed sequences (outputs of tokens outside
+    them, of a padded batch, are zero).  Token rows may be strided (views of one
+    projection).  ``dt_limit`` clamps the steps after softplus.
     Returns ``(y [B, T, H, P] in x's dtype, final_state [N, H, P, S] of
     state_dtype or None)``.
 

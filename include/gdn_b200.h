@@ -591,7 +591,8 @@ GDN_API int gdn_norm_bwd(const gdn_norm_args* args, void* stream);
  *   initial_state [N, H, P, S] of init_dtype or NULL (zeros); final_state
  *     [N, H, P, S] of final_dtype or NULL;
  *   cu_seqlens [N+1] (I32/I64): B == 1 and the T tokens are N packed
- *     sequences (an empty one passes its state on); or NULL, N == B.
+ *     sequences (an empty one passes its state on; the outputs of tokens
+ *     before cu_seqlens[0] or from cu_seqlens[N] on are 0); or NULL, N == B.
  *   P, S <= 256.  bf16 with S of 64 or 128 and P a multiple of 64 runs on the
  *   tensor cores (unless force_generic): bf16 products, states and sums in
  *   fp32.  The first 16 bytes of the workspace are the device error word

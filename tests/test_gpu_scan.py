@@ -537,3 +537,27 @@ def test_empty_batches_have_no_errors():
         y, h = ops.chunk_selective_scan(e(0, 5, 2, 64), e(0, 5, 2), A, e(0, 5, 1, 128), e(0, 5, 1, 128),
                                         output_final_state=True, check_errors=True)
         assert y.shape == (0, 5, 2, 64) and h.shape == (0, 2, 64, 128)
+    poison(1, 5, 2, 64, dtype=bf16)
+    y, _ = ops.chunk_selective_scan(e(1, 5, 2, 64), e(1, 5, 2), A, e(1, 5, 1, 128), e(1, 5, 1, 128),
+                                    cu_seqlens=torch.zeros(1, dtype=torch.int32, device="cuda"), check_errors=True)
+    assert torch.count_nonzero(y) == 0
+
+
+@pytest.mark.parametrize("cu", [[5, 60, 100], [0, 100], [0, 0, 128], [130, 130], [3, 130]])
+@pytest.mark.parametrize("dtype,H,P,S", [(bf16, 2, 64, 128), (f32, 3, 5, 7), (f16, 1, 3, 9)])
+def test_tokens_outside_every_sequence(cu, dtype, H, P, S):
+    """A padded batch: the tokens around the sequences are zero, the others as without them."""
+    T = 130
+    i = make(T, H, P, 1, S, dtype, True, seed=24)
+    c = {k: None if t is None or t.dim() == 1 else t[None] for k, t in cuda(i).items()}
+    f = cuda(i)
+    call = lambda a, b, cu: ops.chunk_selective_scan(  # noqa: E731
+        c["x"][:, a:b], c["dt"][:, a:b], f["A"], c["B"][:, a:b], c["C"][:, a:b], f["D"], c["z"][:, a:b], f["dt_bias"],
+        dt_softplus=True, output_final_state=True, cu_seqlens=torch.tensor(cu, device="cuda"), check_errors=True)
+    poison(1, T, H, P, dtype=dtype)
+    y, h = call(0, T, cu)
+    first, end = cu[0], cu[-1]
+    assert torch.count_nonzero(y[:, :first]) == 0 and torch.count_nonzero(y[:, end:]) == 0
+    if end > first:
+        want, wh = call(first, end, [v - first for v in cu])
+        assert torch.equal(y[:, first:end], want) and torch.equal(h, wh)
