@@ -116,7 +116,7 @@ struct GradLane {
       for (int j = 0; j < WM - 1; ++j)
         if (j < W - 1) pre = pk::fma(w[j], win[j], pre);
       pre = pk::fma(w[W - 1], xv, pre);
-      const V s = pk::sigmoid(pre), one = pk::splat<VEC>(1.f);
+      const V s = pk::sigmoid<T>(pre), one = pk::splat<VEC>(1.f);
       const V r = pk::fma(s, pk::splat<VEC>(-1.f), one);
       d = pk::mul(pk::mul(dyv, s), pk::fma(pre, r, one));
     }

@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const Params p) {
       if constexpr (kRes)
         if (live && tm.in(k)) pk::store<RT, VEC>(static_cast<RT*>(p.sum) + at + tm.col(k), u[k]);
       if (p.z) {
-        a[k] = gate(a[k], pk::sigmoid(a[k]), p.sigmoid_gate);
+        a[k] = gate(a[k], pk::sigmoid<T>(a[k]), p.sigmoid_gate);
         if (p.gate_before) u[k] = pk::mul(u[k], a[k]);
       }
       if (tm.in(k)) sq = pk::fma(u[k], u[k], sq);
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const Params p) {
       V u = pk::widen<X, VEC>(rx[k]), g = pk::mul(pk::widen<T, VEC>(rd[k]), w[k]);
       if (p.z) {
         const V z = pk::widen<T, VEC>(rz[k]);
-        s[k] = pk::sigmoid(z);
+        s[k] = pk::sigmoid<T>(z);
         const V a = gate(z, s[k], p.sigmoid_gate);
         if (p.gate_before) u = pk::mul(u, a);
         else g = pk::mul(g, a);

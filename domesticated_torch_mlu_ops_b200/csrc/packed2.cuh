@@ -82,21 +82,27 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + exp(-x)), two special-function instructions per lane; a few fp32
-// ulp, 0 and 1 at the ends.
-template <int VEC>
+// 1 / (1 + exp(-x)) for results of type T, two special-function instructions
+// per lane; 0 and 1 at the ends.  exp(-x) = 2^t with t = -x log2(e): rounding t
+// to fp32 costs 2^-24 |t| of the result, which 16 bits do not see; for fp32
+// the rest of t, and of log2(e), comes back as a factor 1 + rest ln(2), so that
+// a few ulp are left for every x.
+template <typename T, int VEC>
 __device__ __forceinline__ Vec<VEC> sigmoid(const Vec<VEC>& x) {
-  constexpr float kNegLog2e = -1.4426950408889634f;
-  Vec<VEC> r;
-  if constexpr (VEC == 1) {
-    r.s = rcp(1.f + ex2(x.s * kNegLog2e));
-  } else {
-    GDN_PK_LOOP {
-      float2 t = __fmul2_rn(x.p[i], make_float2(kNegLog2e, kNegLog2e));
-      t = __fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.f, 1.f));
-      r.p[i] = make_float2(rcp(t.x), rcp(t.y));
-    }
+  constexpr float kNegLog2e = -1.4426950408889634f, kNegLog2eRest = -1.9259630e-8f, kLn2 = 0.69314718f;
+  const Vec<VEC> c = splat<VEC>(kNegLog2e), t = mul(x, c);
+  Vec<VEC> e, r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) set(e, i, ex2(get(t, i)));
+  if constexpr (sizeof(T) == 4) {
+    const Vec<VEC> rest = fma(x, splat<VEC>(kNegLog2eRest), fma(x, c, mul(t, splat<VEC>(-1.f))));
+    const Vec<VEC> f = fma(e, mul(rest, splat<VEC>(kLn2)), e);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) set(e, i, get(t, i) < 127.f ? get(f, i) : get(e, i));  // infinite, or a NaN
   }
+  e = add(e, splat<VEC>(1.f));
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) set(r, i, rcp(get(e, i)));
   return r;
 }
 

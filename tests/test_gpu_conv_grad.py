@@ -220,3 +220,17 @@ def test_single_tokens_of_a_strided_batch(dtype, strided):
         dx, dw, _, _ = ops.causal_conv1d_bwd(x, w, None, dy, activation="silu")
     assert rel(dx.reshape(B, D), rx) <= U[dtype] + 64 * F32
     assert rel(dw, rw) <= U[torch.float32] + F32 * (64 + 4 * B ** 0.5)
+
+
+def test_small_sigmoids_keep_fp32_precision():
+    """Width 1, weight 1: dx = dy s (1 + x (1 - s)) element by element, for x
+    down to where s is 1e-26.  expf (2 ulp), the sum, the reciprocal and five
+    more roundings: 8 ulp of 2^-24 each allowed twice."""
+    x = torch.linspace(-60.0, -5.0, 4096).view(1, 64, 64)
+    x[0, 0] = torch.linspace(5.0, 60.0, 64)
+    dx, _, _, _ = ops.causal_conv1d_bwd(x.cuda(), torch.ones(64, 1, device="cuda"), None, torch.ones(1, 64, 64).cuda(),
+                                        activation="silu")
+    v = x.double()
+    s = torch.sigmoid(v)
+    want = s * (1 + v * (1 - s))
+    assert ((dx.double().cpu() - want).abs() <= 16 * F32 * want.abs()).all()

@@ -249,3 +249,22 @@ def test_sum_in_the_residual_s_place(dtype, rd, D):
         x.data_ptr(), 0, res.data_ptr(), w.data_ptr(), again.data_ptr(), res.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 4001, 1, D,
         D, D, 0, 0, D, _DT[dtype], _DT[dtype], _DT[rd], _DT[f32], 0, 0, _lib.GDN_GATE_SILU, 1e-6, 1.0), x.device)
     assert torch.equal(again, y) and torch.equal(res, total)
+
+
+@pytest.mark.parametrize("D", [64, 33])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_small_gates_keep_fp32_precision(D, act):
+    """Element by element, for gates down to 1e-26: the row's 1 / rms (a sum of
+    D squares in fp32 and an approximate root, 8 ulp) and the gate (8 ulp)."""
+    z = torch.linspace(-60.0, 60.0, 50 * D).view(50, D)
+    g = torch.Generator().manual_seed(6)
+    x = 1 + torch.rand(50, D, generator=g)
+    y = ops.gated_rms_norm(x.cuda(), torch.ones(D, device="cuda"), z.cuda(), activation=act)
+    want, _ = ref(x.double(), torch.ones(D).double(), z.double(), None, 1e-6, None, False, False, 1.0, act)
+    assert ((y.double().cpu() - want).abs() <= 16 * F32 * want.abs()).all()
+    dy = torch.ones_like(x)
+    _, _, dz, _ = ops.gated_rms_norm_bwd(dy.cuda(), x.cuda(), torch.ones(D, device="cuda"), z.cuda(), activation=act)
+    s, n = torch.sigmoid(z.double()), (x.double() / (x.double().square().mean(-1, keepdim=True) + 1e-6).sqrt())
+    # the derivative is a sum that cancels near z = -1.28 (silu) or a product with 1 - s, which has an absolute error of 2^-24
+    want, terms = (n * s * (1 + z.double() * (1 - s)), n * s * (1 + z.double().abs())) if act == "silu" else (n * s * (1 - s), n * s)
+    assert ((dz.double().cpu() - want).abs() <= 24 * F32 * terms).all()
