@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256, 2) scan_rec_kernel(const ScanParams p) {
         const int i = threadIdx.x + j * 256, k = i / ROWS, q = i % ROWS;
         if (k >= now || row0 + q >= p.P) continue;
         float v = sy[k][q];
-        if (p.z) v *= silu(pk::widen<T, 1>(z[j]).s);
+        if (p.z) v *= silu<T>(pk::widen<T, 1>(z[j]).s);
         static_cast<T*>(p.y)[(t + k) * p.H * p.P + col0 + q] = from_f<T>(v);
       }
     }
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kUpdWarps * 32) scan_update_kernel(const Updat
   if (lane < R) {
     const int row = row0 + lane * RW;
     if (row < p.P) {
-      if (p.z) out *= silu(to_f<T>(static_cast<const T*>(p.z)[n * p.sz + static_cast<int64_t>(h) * p.P + row]));
+      if (p.z) out *= silu<T>(to_f<T>(static_cast<const T*>(p.z)[n * p.sz + static_cast<int64_t>(h) * p.P + row]));
       y[row] = from_f<T>(out);
     }
   }

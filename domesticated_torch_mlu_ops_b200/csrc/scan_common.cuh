@@ -7,6 +7,7 @@
 
 #include "conv_math.cuh"
 #include "gdn_common.cuh"
+#include "packed2.cuh"
 
 namespace gdn {
 namespace scan {
@@ -38,7 +39,12 @@ __device__ __forceinline__ float step_of(float raw, float bias, int softplus, fl
   return v > hi ? hi : v;
 }
 
-__device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.f + __expf(-z)); }
+// z / (1 + exp(-z)) for outputs of type T.
+template <typename T>
+__device__ __forceinline__ float silu(float z) {
+  const pk::Vec<1> v{z};
+  return z * pk::sigmoid<T>(v).s;
+}
 
 struct ScanParams {
   const void *x, *dt, *b, *c, *z;

@@ -561,3 +561,20 @@ def test_tokens_outside_every_sequence(cu, dtype, H, P, S):
     if end > first:
         want, wh = call(first, end, [v - first for v in cu])
         assert torch.equal(y[:, first:end], want) and torch.equal(h, wh)
+
+
+def test_small_fp32_gates():
+    """Step 0, D = 1: y = x silu(z) element by element, for z down to where the
+    gate is 1e-26; sigmoid and two products, 8 ulp allowed."""
+    n = 64
+    g = torch.Generator().manual_seed(25)
+    x, z = 1 + torch.rand(n, 2, 20, generator=g), torch.linspace(-60.0, 60.0, n * 40).view(n, 2, 20)
+    zero = torch.zeros(n, 1, 8)
+    i = dict(x=x, dt=torch.zeros(n, 2), A=-torch.ones(2), B=zero, C=zero, D=torch.ones(2), z=z, dt_bias=torch.full((2,), -50.0))
+    want = x.double() * z.double() * torch.sigmoid(z.double())
+    y, _ = run(i, [n])
+    c = cuda(i)
+    u, _ = ops.selective_scan_update(*[c[k] for k in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")], dt_softplus=True,
+                                     state=torch.zeros(n, 2, 20, 8, device="cuda"))
+    for got in (y, u):
+        assert ((got.double().cpu() - want).abs() <= 8 * F32 * want.abs()).all()
