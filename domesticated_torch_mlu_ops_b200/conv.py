@@ -200,6 +200,9 @@ def causal_conv1d_bwd(
         raise ValueError(f"[CausalConv1d] bias {tuple(bias.shape)} must be ({x.shape[2]},)")
     _cuda("causal_conv1d_bwd", x, weight, bias, dy, initial_state, cu_seqlens)
     _fdt(x, "x"), _fdt(weight, "weight")
+    for t, name in ((bias, "bias"), (initial_state, "initial_state")):
+        if t is not None:
+            _fdt(t, name)
     B, T, D = x.shape
     W = weight.shape[1]
     cu = None
@@ -211,11 +214,14 @@ def causal_conv1d_bwd(
         N = cu.numel() - 1
     if initial_state is not None and tuple(initial_state.shape) != (N, D, W):
         raise ValueError(f"[CausalConv1d] initial_state {tuple(initial_state.shape)} must be [N, D, W] = {(N, D, W)}")
-    b_dtype = None if bias is None else bias.dtype
     op = _conv1d_bwd_impl if _plain(x, weight, bias, dy, initial_state, cu) else torch.ops.gdn_b200.causal_conv1d_bwd
-    dx, dw, db, dh = op(x, weight.contiguous(), None if bias is None else bias.to(weight.dtype).contiguous(), dy,
+    w, b = weight.contiguous(), bias
+    if bias is not None and bias.dtype != weight.dtype:
+        # the forward's values, held in fp32: dweight and dbias come in one type, and each is rounded to its own once
+        w, b = w.float(), bias.to(weight.dtype).float()
+    dx, dw, db, dh = op(x, w, None if b is None else b.contiguous(), dy,
                         None if initial_state is None else initial_state.contiguous(), act, cu)
-    return dx, dw, None if bias is None else db.to(b_dtype), None if initial_state is None else dh
+    return (dx, dw.to(weight.dtype), None if bias is None else db.to(bias.dtype), None if initial_state is None else dh)
 
 
 class CausalConv1dFunction(torch.autograd.Function):

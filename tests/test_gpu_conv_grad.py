@@ -234,3 +234,17 @@ def test_small_sigmoids_keep_fp32_precision():
     s = torch.sigmoid(v)
     want = s * (1 + v * (1 - s))
     assert ((dx.double().cpu() - want).abs() <= 16 * F32 * want.abs()).all()
+
+
+@pytest.mark.parametrize("wdtype,bdtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32),
+                                           (torch.float32, torch.bfloat16)])
+def test_bias_of_another_type(wdtype, bdtype):
+    """The gradient of a bias is rounded to the bias's type only."""
+    x, dy, w, b, _ = make([300], 64, 4, torch.bfloat16, wdtype, True, False, seed=8)
+    b = (b.float() + 0.001).to(bdtype)
+    rx, rw, rb, _ = reference(x, dy, w, b.to(wdtype), None, [300], True)  # the forward takes the bias in the weight's type
+    dx, dw, db, _ = ops.causal_conv1d_bwd(x.cuda()[None], w.cuda(), b.cuda(), dy.cuda()[None], activation="silu")
+    assert dw.dtype == wdtype and db.dtype == bdtype
+    assert rel(dx[0], rx) <= U[torch.bfloat16] + 64 * F32
+    assert rel(dw, rw) <= U[wdtype] + F32 * (64 + 4 * 300 ** 0.5)
+    assert rel(db, rb) <= U[bdtype] + F32 * (64 + 4 * 300 ** 0.5)
