@@ -34,7 +34,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .gdn import _DT, _IDT, _addr, _cuda, _launch, _plain, _ptr, _stream
+from .gdn import _DT, _IDT, _addr, _cuda, _first_order, _launch, _plain, _ptr, _stream
 
 
 def _act(activation):
@@ -237,6 +237,7 @@ class CausalConv1dFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
         x, weight, bias, initial_state, cu = ctx.saved_tensors
         dx, dw, db, dh = causal_conv1d_bwd(x, weight, bias, dy, initial_state, ctx.activation, cu)
@@ -263,7 +264,7 @@ def causal_conv1d(
     sequence (column j = token j - W).  Returns ``(y, None)``
     (``triton_ops.py:287-363``).  ``backend`` is accepted for signature
     compatibility ('triton' is the reference's only value; the work runs in
-    CUDA here).  Differentiable in x, weight, bias, residual and initial_state
+    CUDA here).  Differentiable once in x, weight, bias, residual and initial_state
     (:func:`causal_conv1d_bwd`)."""
     if cp_context is not None:
         raise ValueError("[CausalConv1d] CP Context not supported.")

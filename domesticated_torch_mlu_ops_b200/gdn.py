@@ -45,6 +45,7 @@ Differences from the reference, all supersets:
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -171,6 +172,38 @@ def _launch(fn, packed, dev):
             rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc)
+
+
+class _SecondOrder(torch.autograd.Function):
+    """Passes gradients on; differentiating them is an error."""
+
+    @staticmethod
+    def forward(ctx, name, requires, *grads):
+        ctx.name = name
+        return tuple(g.detach() if isinstance(g, torch.Tensor) else g for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} is differentiable once: its gradients have no derivative")
+
+
+def _first_order(backward):
+    """Decorator of an autograd node's backward that runs a kernel: under
+    ``create_graph=True`` its gradients raise when they are differentiated.
+    (torch's ``once_differentiable`` does so only where the incoming gradient
+    requires grad; a penalty on ``op(x).sum()``'s gradient would lose the op's
+    part without an error.)"""
+    name = backward.__qualname__.split(".")[0]
+
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        if torch.compiler.is_compiling() or not torch.is_grad_enabled():  # a compiled backward refuses it by itself
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        return _SecondOrder.apply(name, torch.empty(0, requires_grad=True), *out)
+
+    return wrapped
 
 
 # ---------------------------------------------------------------------------
@@ -515,6 +548,7 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
         return o, (ht if output_final_state else None)
 
     @staticmethod
+    @_first_order
     def backward(ctx, do, dht):
         q, k, v, g32, b32, h0, cu = ctx.saved_tensors
         scale, svf, l2, g_dt, b_dt, h0_dt = ctx.meta

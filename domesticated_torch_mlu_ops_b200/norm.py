@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .gdn import _DT, _addr, _cuda, _launch, _plain
+from .gdn import _DT, _addr, _cuda, _first_order, _launch, _plain
 
 Tensor = torch.Tensor
 _GATE = {"silu": _lib.GDN_GATE_SILU, "swish": _lib.GDN_GATE_SILU, "sigmoid": _lib.GDN_GATE_SIGMOID}
@@ -201,6 +201,7 @@ class GatedRMSNormFunction(torch.autograd.Function):
         return (y, total) if residual is not None else y
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, dsum=None):
         x, weight, z = ctx.saved_tensors
         dtype = z.dtype if z is not None else dy.dtype
@@ -235,8 +236,8 @@ def gated_rms_norm(
     slices are read in place), residual ``[..., D]`` of x's dtype or float32,
     weight ``[D]`` of any float type.  Returns y in x's dtype, or
     ``(y, r)`` with r in the residual's dtype when a residual is given.  The
-    norm is taken of the unrounded fp32 sum.  Differentiable in x, weight, z
-    and residual (the backward takes r as it was stored)."""
+    norm is taken of the unrounded fp32 sum.  Differentiable once in x, weight,
+    z and residual (the backward takes r as it was stored)."""
     _cuda("gated_rms_norm", x, weight, z, residual)
     group, act = _check("gated_rms_norm", x, weight, z, residual, group_size, activation)
     if z is not None and z.dtype != x.dtype:
