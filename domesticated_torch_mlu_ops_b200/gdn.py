@@ -49,6 +49,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -66,6 +67,12 @@ def _stream(dev):
 
 
 def _cuda(name, *ts):
+    """Refuses tensors that are not on a GPU, and those with a forward-mode
+    tangent, which the kernels would drop without a word."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative")
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError(f"{name}: every tensor must be on a CUDA device (got {t.device})")

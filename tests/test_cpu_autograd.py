@@ -64,3 +64,34 @@ def test_delta_rule_gradient_of_a_gradient_is_refused(monkeypatch):
     dv, = torch.autograd.grad((o + v ** 3).sum(), v, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         dv.square().sum().backward()
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be dropped by a kernel: the call says so, before all other checks."""
+    from torch.autograd import forward_ad
+
+    import domesticated_torch_mlu_ops_b200 as ops
+    x, w = torch.randn(1, 4, 2, 8), torch.rand(8)
+    dt, A, cu = torch.rand(1, 4, 2), torch.rand(2), torch.tensor([0, 4])
+    taps = torch.rand(8, 4)
+
+    def calls(t):
+        yield lambda: ops.gated_rms_norm(t(x), w)
+        yield lambda: ops.gated_rms_norm(x, w, residual=t(x))
+        yield lambda: ops.gated_rms_norm_bwd(x, x, t(w))
+        yield lambda: ops.causal_conv1d(x[:, :, 0], t(taps))
+        yield lambda: ops.causal_conv1d_bwd(x[:, :, 0], taps, None, t(x[:, :, 0]))
+        yield lambda: ops.chunk_selective_scan(x, dt, t(A), x, x, cu_seqlens=cu)
+        yield lambda: ops.selective_scan_update(x[0], t(dt[0]), A, x[0], x[0], state=torch.zeros(4, 2, 8, 8))
+        yield lambda: ops.chunk_gated_delta_rule(t(x), x, x, dt, dt)
+
+    with forward_ad.dual_level():
+        for call in calls(lambda t: forward_ad.make_dual(t.contiguous(), torch.ones_like(t))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        for call in calls(lambda t: t):  # no tangent: the next check
+            with pytest.raises(ValueError, match="CUDA"):
+                call()
+    for call in calls(lambda t: t):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
