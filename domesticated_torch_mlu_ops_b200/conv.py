@@ -240,7 +240,9 @@ class CausalConv1dFunction(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         x, weight, bias, initial_state, cu = ctx.saved_tensors
-        dx, dw, db, dh = causal_conv1d_bwd(x, weight, bias, dy, initial_state, ctx.activation, cu)
+        dx = dw = db = dh = None
+        if any(ctx.needs_input_grad[i] for i in (0, 1, 2, 4)):  # the residual's gradient is dy
+            dx, dw, db, dh = causal_conv1d_bwd(x, weight, bias, dy, initial_state, ctx.activation, cu)
         return dx, dw, db, None if ctx.residual_dtype is None else dy.to(ctx.residual_dtype), dh, None, None
 
 

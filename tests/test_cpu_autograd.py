@@ -49,6 +49,15 @@ def test_conv_gradient_of_a_gradient_is_refused(monkeypatch):
         g.square().sum().backward()
 
 
+def test_conv_residual_alone_needs_no_kernel(monkeypatch):
+    monkeypatch.setattr(conv, "causal_conv1d", lambda x, w, b, r, *a, **k: (x * w[:, -1] + r, None))
+    monkeypatch.setattr(conv, "causal_conv1d_bwd", lambda *a: pytest.fail("not needed"))
+    x, w, r = torch.randn(1, 4, 8), torch.rand(8, 4), torch.randn(1, 4, 8, requires_grad=True)
+    dy = torch.randn(1, 4, 8)
+    g, = torch.autograd.grad(conv.CausalConv1dFunction.apply(x, w, None, r, None, "silu", None), r, dy)
+    assert torch.equal(g, dy)
+
+
 def test_delta_rule_gradient_of_a_gradient_is_refused(monkeypatch):
     def call(op, impl, *args):
         if impl is gdn._chunk_fwd_impl:
