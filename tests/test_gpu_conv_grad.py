@@ -248,3 +248,26 @@ def test_bias_of_another_type(wdtype, bdtype):
     assert rel(dx[0], rx) <= U[torch.bfloat16] + 64 * F32
     assert rel(dw, rw) <= U[wdtype] + F32 * (64 + 4 * 300 ** 0.5)
     assert rel(db, rb) <= U[bdtype] + F32 * (64 + 4 * 300 ** 0.5)
+
+
+def test_gradients_in_a_graph():
+    """The conv's and the norm's gradients captured once and replayed on new inputs."""
+    x, dy, w, b, h0 = (t.cuda() for t in make([90, 40], 64, 4, torch.bfloat16, torch.bfloat16, True, True, seed=9))
+    cu = torch.tensor([0, 90, 130], dtype=torch.int32).cuda()
+    nw = torch.rand(64, device="cuda")
+
+    def step(x, dy):
+        return (*ops.causal_conv1d_bwd(x[None], w, b, dy[None], h0, "silu", cu),
+                *ops.gated_rms_norm_bwd(dy, x, nw, dy)[:3])
+
+    sx, sdy = x.clone(), dy.clone()
+    step(sx, sdy)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(sx, sdy)
+    sx.copy_(x.flip(0)), sdy.copy_(dy.flip(1))
+    graph.replay()
+    want = step(x.flip(0).contiguous(), dy.flip(1).contiguous())
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, want))

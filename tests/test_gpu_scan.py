@@ -578,3 +578,47 @@ def test_small_fp32_gates():
                                      state=torch.zeros(n, 2, 20, 8, device="cuda"))
     for got in (y, u):
         assert ((got.double().cpu() - want).abs() <= 8 * F32 * want.abs()).all()
+
+
+def check_prompt(lens, H, P, G, S, seed, gate=True, init=True):
+    i = make(sum(lens), H, P, G, S, bf16, gate, seed=seed)
+    h0 = torch.randn(len(lens), H, P, S, generator=torch.Generator().manual_seed(seed + 1)) * 0.3 if init else None
+    ry, rh = ref_scan(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["dt_bias"], True, (0.0, float("inf")),
+                      h0, lens)
+    y, h = run(i, lens, h0)
+    assert rel(y, ry) <= tolerances(bf16, True) and rel(h, rh) <= 64 * F32
+    for n, length in enumerate(lens):
+        if length == 0:
+            assert torch.equal(h[n].cpu(), h0[n] if init else torch.zeros_like(h[n]).cpu())
+
+
+@pytest.mark.parametrize("H,G", [(17, 1), (33, 3), (20, 2)])
+def test_more_heads_than_one_block_of_steps(H, G):
+    """Steps are prepared for sixteen heads at a time."""
+    check_prompt([130, 3], H, 64, G, 64, 30)
+
+
+@pytest.mark.parametrize("H", [1, 20])
+def test_more_sequences_than_a_warp_looks_at(H):
+    """Sequences are found 32 at a time; with one head they are cut as well."""
+    g = torch.Generator().manual_seed(31)
+    lens = torch.randint(0, 60, (75,), generator=g).tolist()
+    lens[40] = 700 if H == 1 else 130
+    lens[33] = lens[74] = 0
+    check_prompt(lens, H, 64, 1, 64, 32)
+
+
+@pytest.mark.parametrize("lens", [[1200], [700, 650]])
+def test_segments_in_pieces(lens):
+    """Fifty heads on one long prompt: two segments, the first pass on pieces of them."""
+    check_prompt(lens, 50, 64, 2, 64, 33)
+
+
+def test_first_pass_over_a_long_prompt():
+    """Several segments of several chunks each, S = 128."""
+    check_prompt([2500], 3, 64, 1, 128, 34)
+
+
+def test_widest_heads_on_tensor_cores():
+    check_prompt([140, 0, 9], 2, 256, 1, 128, 35)
+    check_prompt([300], 2, 192, 2, 64, 36, gate=False, init=False)
