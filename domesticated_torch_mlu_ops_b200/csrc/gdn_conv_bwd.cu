@@ -31,10 +31,13 @@ constexpr int kMinRun = 64;  // tokens per run, at least
 constexpr int kThreads = 128;
 // A thread's vector in bytes, CTAs per SM, and tokens whose loads are in
 // flight together at W = 4.  Measured at 8192 tokens x 8192 bf16 channels
-// (403 MB): 89 us, 4.5 TB/s, 69 % of a plain copy's rate.  The fp32 pipe and
-// the two special functions per element set the pace, not the loads: copying
-// the blocks through shared memory (cp.async, 15 tokens ahead) took 90 us,
-// 16-byte vectors 91 us, five CTAs per SM 113 us, 4-byte vectors 154 us.
+// (403 MB): 89 us, 4.5 TB/s, 69 % of a plain copy's rate.  No pipe is full
+// (fma 26 %, alu 21 %, special functions 35 %, half of the issue slots) and
+// few warps wait for memory: with four warps per scheduler, which the 128
+// registers allow, a token's own chain (pre, sigmoid, d, the pending sums) is
+// what is left.  Copying the blocks through shared memory (cp.async, 15 tokens
+// ahead) took 90 us, 16-byte vectors 91 us, five CTAs per SM 113 us, 4-byte
+// vectors 154 us.
 constexpr int kVecBytes = 8, kResident = 4, kBlock4 = 6;
 constexpr int kMaxW = 16;
 

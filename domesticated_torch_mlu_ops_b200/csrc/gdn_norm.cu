@@ -21,7 +21,12 @@
 // (5.6 TB/s, 85 % of a plain copy's rate), backward 66 + 4 us for 336 MB (4.8
 // TB/s); 5001 bf16 rows of 2048 with an fp32 residual, forward 18 us for 123
 // MB (the sum stays partly in L2), backward 31 + 4 us for 143 MB.  A few rows
-// (64 x 32 of 128): 2.2 us, a launch and one trip to memory.
+// (64 x 32 of 128): 2.2 us, a launch and one trip to memory.  Rows above 256
+// vectors have no look-ahead (larger CTAs, 64 registers) and are slower: 33.5 M
+// bf16 values with a gate, forward and backward, 40 and 73 us in rows of 2048,
+// 53 and 191 in rows of 2560, 55 and 149 of 4096, 77 and 135 of 5120, 63 and
+// 118 of 8192; with an fp32 residual instead 66 and 89, 69 and 250, 69 and 184,
+// 86 and 168, 74 and 143.
 
 #include "conv_math.cuh"
 #include "gdn_common.cuh"
@@ -524,7 +529,7 @@ extern "C" GDN_API int gdn_norm_fwd(const gdn_norm_args* a, void* stream) {
   return GDN_OK;
 }
 
-// The parts of parts_of at its most (CTAs of 64 threads), whatever the alignment.
+// The parts of parts_of at its most (CTAs of 32 threads), whatever the alignment.
 extern "C" GDN_API size_t gdn_norm_bwd_workspace_size(const gdn_norm_args* a) {
   if (norm::check(a, true)) return 0;
   return static_cast<size_t>(std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(a->rows, 1), 148 * (norm::kBwdThreads / 32)))) * a->D * sizeof(float);

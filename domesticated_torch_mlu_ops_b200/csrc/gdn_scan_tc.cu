@@ -29,29 +29,34 @@
 // segment in one accumulator, chunks from the last to the first, each
 // weighted by the decay to the segment's end.
 //
-// What bounds it.  The products of a chunk take about 1.9 K cycles of the
-// tensor pipe (per step of 16 measured 64 at 128 columns and 48 at 64, by rate 96 at 192), a
-// chunk step 4.2 to 4.7 K: P and w x 2 K, Ya and dH 1.2 K beside the first
-// part of the outputs, the rest of them and h 1 K.  The sixteen warps' own
-// work takes as long as that chain (56 % of the issue slots, 36 % of the
-// tensor pipe), and shared memory leaves room for one CTA per SM.  64 heads of
-// 64 x 128: 8192 tokens 22 us (first pass) and 82 us, with steps and hand-over
-// 115 us for 208 MB; 29,893 packed tokens that start from states 327 us and 14
-// us of steps.  What each choice gave on those two: P through TMEM and one
-// product for dH 106 -> 105 and 417 -> 410 us (first pass 25.5 -> 22), z
-// before the next chunk's operands and in L2 88 and 351, operands as their
-// places become free 82 to 85 and 330.  Measured and set aside: w x and dH
-// before P, so that h is ready before the outputs (96 and 381), both halves of
-// the scores behind one wait (86 and 336), w x shared out by who has no block
-// of P (84 and 330), products issued by a working warp (1.7 times).
+// What bounds it.  The products of a chunk take about 2.5 K cycles of the
+// tensor pipe (per step of 16 measured 64 at 128 columns, 93 at 192, and 32 at
+// 64 with the operand in TMEM), a chunk step about 6 K: P and w x, Ya and dH
+// beside the first part of the outputs, the rest of them and h, each by all
+// sixteen warps.  Their work and that chain take the same time (41 % of the
+// issue slots, 39 % of the tensor pipe), and shared memory leaves room for one
+// CTA per SM.  64 heads of 64 x 128: 8192 tokens 21 us (first pass) and 112 us,
+// with steps and hand-over 145 us for 208 MB; 31,992 packed tokens that start
+// from states 422 us and 14 us of steps.  What each choice gave on those two
+// when it was made: P through TMEM and one product for dH 106 -> 105 and 417 ->
+// 410 us, z before the next chunk's operands and in L2 88 and 351, operands as
+// their places become free 82 to 85 and 330, decays by sums 87 -> 90 and 336 ->
+// 344, two parts of P and h 112 and 421.  Measured and set aside: w x and dH
+// before P, so that h is ready before the outputs (1.15 times), both halves of
+// the scores behind one wait, w x shared out by who has no block of P, products
+// issued by a working warp (1.7 times); of the two parts' ways: P announced
+// before w x (126 and 473), both parts of h into one accumulator, which reads C
+// twice, y stored by the warps themselves (151 and 571: the fences wait for
+// it).
 //
 // Rounding.  x, B and C are bf16 already.  P, h and w x are split into bf16
 // parts whose products are summed: two parts (16 bits) where they only feed y,
-// which is rounded to 8 bits in the end, so that an output in 64 at most rounds
-// otherwise than the exact one; three (24 bits) of w x where the state is
-// returned or handed on, so that a returned fp32 state has fp32 precision.
+// which is rounded to 8 bits in the end (one output in 1100 on the two prompts
+// above rounds otherwise than the exact one); three (24 bits) of w x where the
+// state is returned or handed on, so that a returned fp32 state has fp32
+// precision.
 // One part of P and h each would take 22 and 77 us less on the two prompts
-// above and turn a fifth of the outputs.
+// above and round a fifth of the outputs otherwise.
 //
 // Decays are products of sums that only add: the decay between two blocks' is
 // exp(a_i + the blocks between) k_j, w is k times the blocks after.  No

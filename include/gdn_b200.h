@@ -594,7 +594,7 @@ GDN_API int gdn_norm_bwd(const gdn_norm_args* args, void* stream);
  *     sequences (an empty one passes its state on; the outputs of tokens
  *     before cu_seqlens[0] or from cu_seqlens[N] on are 0); or NULL, N == B.
  *   P, S <= 256.  bf16 with S of 64 or 128 and P a multiple of 64 runs on the
- *   tensor cores (unless force_generic): bf16 products, states and sums in
+ *   tensor cores (unless force_generic): products of bf16 parts, states and sums in
  *   fp32.  The first 16 bytes of the workspace are the device error word
  *   (see gdn_chunk_check_device_error). */
 typedef struct gdn_scan_args {
