@@ -30,10 +30,11 @@ __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
 }
 
 // VEC consecutive elements <-> floats; one 128-bit access when VEC fills 16 B.
-template <typename T, int VEC>
+// RW: memory that the kernel writes later, by an ordinary load.
+template <typename T, int VEC, bool RW = false>
 __device__ __forceinline__ void ldv(const T* p, float* v) {
   if constexpr (VEC * sizeof(T) == 16) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = RW ? *reinterpret_cast<const uint4*>(p) : __ldg(reinterpret_cast<const uint4*>(p));
     const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = to_f<T>(e[i]);

@@ -43,11 +43,12 @@ template <> __device__ __forceinline__ float4 load4<__half>(const __half* p) {
   return make_float4(fa.x, fa.y, fb.x, fb.y);
 }
 
-// Streaming 128-bit state traffic: read once, write once.
+// Streaming 128-bit state traffic: read once, write once, in place where the
+// state is a cache: not a load of the read-only kind.
 __device__ __forceinline__ float4 ld_stream(const float* p) {
   float4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "l"(p) : "memory");
   return r;
 }
 __device__ __forceinline__ void st_stream(float* p, float4 v) {

@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kThreads) conv_update_vec_kernel(const UpdPara
   ldv<T, C8>(xs, xv);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    ldv<T, 8>(cache + v * 8, cf + v * 8);
+    ldv<T, 8, true>(cache + v * 8, cf + v * 8);
     ldv<T, 8>(wt + v * 8, wf + v * 8);
   }
   if (p.bias) ldv<T, C8>(static_cast<const T*>(p.bias) + d, acc);

@@ -207,10 +207,18 @@ def _kernel_source(file, name):
 
 @pytest.mark.parametrize("file,kernel,array", [("gdn_norm.cu", "norm_fwd_kernel", "p.residual"),
                                                ("gdn_scan.cu", "scan_pass_kernel", "st + j * step"),
-                                               ("gdn_scan.cu", "scan_update_kernel", ", from)")])
+                                               ("gdn_scan.cu", "scan_update_kernel", ", from)"),
+                                               ("gdn_conv.cu", "conv_update_vec_kernel", "cache + ")])
 def test_memory_that_a_kernel_writes_is_not_read_as_read_only(file, kernel, array):
     """The norm's sum may be its residual, a state is replaced in place: loads
     of the read-only kind promise that the memory does not change."""
     body = _kernel_source(file, kernel)
     loads = [line for line in body.splitlines() if array in line and ("load" in line or "ldv" in line)]
-    assert loads and all("load_rw" in line for line in loads)
+    assert loads and all("load_rw" in line or ", true>(" in line for line in loads)
+
+
+def test_states_are_streamed_by_ordinary_loads():
+    """The recurrent decode replaces cache lines that it has read by ld_stream."""
+    src = open(os.path.join(os.path.dirname(HEADER), "..", "domesticated_torch_mlu_ops_b200", "csrc", "gdn_common.cuh")).read()
+    body = src[src.index("float4 ld_stream("):]
+    assert ".nc." not in body[:body.index("}\n")]
