@@ -200,9 +200,8 @@ def causal_conv1d_bwd(
         raise ValueError(f"[CausalConv1d] bias {tuple(bias.shape)} must be ({x.shape[2]},)")
     _cuda("causal_conv1d_bwd", x, weight, bias, dy, initial_state, cu_seqlens)
     _fdt(x, "x"), _fdt(weight, "weight")
-    for t, name in ((bias, "bias"), (initial_state, "initial_state")):
-        if t is not None:
-            _fdt(t, name)
+    if initial_state is not None:
+        _fdt(initial_state, "initial_state")
     B, T, D = x.shape
     W = weight.shape[1]
     cu = None
