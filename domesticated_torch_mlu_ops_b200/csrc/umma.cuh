@@ -204,29 +204,13 @@ __device__ __forceinline__ void tmem_ld16x2(uint32_t ta, uint32_t tb, float* a, 
   }
 }
 
-// Stores of the warp's 32 lanes to 4 or 8 columns; tmem_st_wait before they
-// are announced.
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint4 v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
-               :: "r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
+// Store of the warp's 32 lanes to 8 columns; tmem_st_wait before it is
+// announced.
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, uint4 a, uint4 b) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                :: "r"(taddr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// 8 columns of the warp's 32 lanes (32x32b.x8).
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
-  uint32_t r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-  tmem_wait_ld();
-  reg_fence8(r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // Loads without a wait: issue several, then tmem_wait_ld() once and
 // reg_fence() every destination array so no use moves above the wait.
